@@ -366,6 +366,67 @@ int sgpo_daps_mh(sgpo_mlp* m, const int64_t* x0hat, int N, int L, int S, const i
                  uint64_t offset, uint64_t row_offset, int64_t* x_out, void* workspace,
                  size_t workspace_bytes, void* stream);
 
+/* ---- training operators of a denoiser ---------------------------------------------------------
+ * The reference trains its denoisers through torch autograd (models/pretraining/trainer.py); these are the pieces of such a
+ * step that torch would run as chains of memory-bound kernels or not in one piece at all.  Types: fp32 or bf16. */
+#define SGPO_DTYPE_F32 0
+#define SGPO_DTYPE_BF16 1
+
+/* Rotation of query and key heads by their positions.  Pair j < rot / 2 of a head -- elements (j, j + rot / 2), or (2j, 2j + 1)
+ * if interleaved -- turns by position * frequencies[j] (formed in 64 bits) and is multiplied by scale; elements from rot on are
+ * copied.  inverse: the transposed rotation, i.e. the gradient.  Strides in elements: batch, token, head; a head's elements
+ * are contiguous.  q_out may be q and k_out may be k (in place); otherwise outputs must not overlap inputs.  heads_k 0: no keys.
+ * positions NULL: the token's index 0 .. L-1.  positions and frequencies are device memory. */
+typedef struct {
+  const void* q; void* q_out;
+  const void* k; void* k_out;
+  int64_t q_stride[3], q_out_stride[3], k_stride[3], k_out_stride[3];
+  const int64_t* positions;
+  int64_t pos_stride_b, pos_stride_l;
+  const double* frequencies;   /* [rot / 2] */
+  int B, L, heads_q, heads_k, head_dim, rot, interleaved, inverse, dtype;
+  float scale;
+} sgpo_rotary_args;
+int sgpo_rotary(const sgpo_rotary_args* args, void* stream);
+
+/* Cross entropy of a linear head, z = hidden weight^T + bias, without its logits.
+ *   hidden [N][H] and weight [V][H] of `dtype`, rows ld_* elements apart; bias fp32 [V] or NULL (-inf closes a class);
+ *   targets int64 [N]; a token with target ignore_index has loss and gradients 0 (its hidden row may hold anything); a
+ *   target outside [0, V) gives NaN.
+ * forward: nll [N], lse [N] fp32; loss [1] and inv_count [1] unless reduction is NONE (the mean over no token is 0).
+ * backward: grad_out is [1] ([N] for NONE); lse and inv_count are the forward's; dhidden [N][H], dweight [V][H] of `dtype` and dbias fp32
+ *   [V], contiguous; any of them may be NULL.
+ * The workspace is scratch: forward and backward each ask for their own. */
+#define SGPO_REDUCE_NONE 0
+#define SGPO_REDUCE_MEAN 1
+#define SGPO_REDUCE_SUM 2
+typedef struct {
+  const void* hidden; const void* weight;
+  const float* bias;
+  const int64_t* targets;
+  int64_t ld_hidden, ld_weight, ignore_index;
+  int N, H, V, dtype, reduction;
+} sgpo_linear_ce_args;
+size_t sgpo_linear_ce_workspace_bytes(const sgpo_linear_ce_args* args, int backward);
+int sgpo_linear_ce_forward(const sgpo_linear_ce_args* args, float* nll, float* lse, float* loss, float* inv_count,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int sgpo_linear_ce_backward(const sgpo_linear_ce_args* args, const float* lse, const float* grad_out,
+                            const float* inv_count, void* dhidden, void* dweight, float* dbias, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Orthogonalised updates: X = U / (|U|_F + eps), then X <- a X + (b X X^T + c (X X^T)^2) X for each triple of `coefficients` (HOST,
+ * 3 * steps floats).  newton_schulz: update [batch][rows][cols] of `dtype`, matrices stride_b and rows ld elements apart; out bf16,
+ * contiguous.  muon_step, everything contiguous: buffer = momentum buffer + grad; U = grad + momentum buffer if nesterov, else
+ * buffer; weight = (1 - lr weight_decay) weight - lr sqrt(max(1, rows / cols)) X. */
+size_t sgpo_newton_schulz_workspace_bytes(int batch, int rows, int cols);
+int sgpo_newton_schulz(const void* update, int dtype, int batch, int rows, int cols, int64_t stride_b, int64_t ld,
+                       const float* coefficients, int steps, float eps, void* out, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int sgpo_muon_step(void* weight, int weight_dtype, const void* grad, int grad_dtype, float* momentum_buffer, int batch,
+                   int rows, int cols, float lr, float momentum, int nesterov, float weight_decay,
+                   const float* coefficients, int steps, float eps, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
 /* ---- test / bench access to the building blocks ----------------------------------- */
 /* C[M][N] (fp32) = A[M][K] (bf16) * W[N][K]^T (bf16) through the MFMA GEMM kernel. */
 int sgpo_gemm_bf16(const void* A, const void* W, float* C, int M, int N, int K, void* stream);

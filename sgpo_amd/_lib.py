@@ -12,6 +12,8 @@ LIB_PATH = os.environ.get('SGPO_HIP_LIB') or os.path.join(_HERE, 'libsgpo_hip.so
 NOISE_PHILOX, NOISE_EXPONENTIAL, NOISE_UNIFORM, NOISE_NONE = 0, 1, 2, 3
 STEP_SOFT, STEP_SOFT_CG, STEP_HARD = 0, 1, 2
 PROF_KINDS = 20
+DTYPE_F32, DTYPE_BF16 = 0, 1
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 
 
 class SgpoError(RuntimeError):
@@ -24,6 +26,20 @@ class DitConfig(C.Structure):
 
 
 _vp, _i, _f, _u64, _sz, _i64 = C.c_void_p, C.c_int, C.c_float, C.c_uint64, C.c_size_t, C.c_int64
+
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = ([(n, _vp) for n in ('q', 'q_out', 'k', 'k_out')] +
+                [(n, _i64 * 3) for n in ('q_stride', 'q_out_stride', 'k_stride', 'k_out_stride')] +
+                [('positions', _vp), ('pos_stride_b', _i64), ('pos_stride_l', _i64), ('frequencies', _vp)] +
+                [(n, _i) for n in ('B', 'L', 'heads_q', 'heads_k', 'head_dim', 'rot', 'interleaved', 'inverse', 'dtype')] + [('scale', _f)])
+
+
+class LinearCeArgs(C.Structure):
+    _fields_ = ([(n, _vp) for n in ('hidden', 'weight', 'bias', 'targets')] +
+                [(n, _i64) for n in ('ld_hidden', 'ld_weight', 'ignore_index')] + [(n, _i) for n in ('N', 'H', 'V', 'dtype', 'reduction')])
+
 
 # name -> (restype, argtypes); must list every symbol include/sgpo_hip.h declares
 SIGNATURES = {
@@ -87,6 +103,13 @@ SIGNATURES = {
     'sgpo_daps_mh_workspace_bytes': (_sz, []),
     'sgpo_daps_mh': (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _f, _f, _f, _i, _i, _vp, _vp, _vp, _u64, _u64, _u64,
                           _vp, _vp, _sz, _vp]),
+    'sgpo_rotary': (_i, [C.POINTER(RotaryArgs), _vp]),
+    'sgpo_linear_ce_workspace_bytes': (_sz, [C.POINTER(LinearCeArgs), _i]),
+    'sgpo_linear_ce_forward': (_i, [C.POINTER(LinearCeArgs), _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    'sgpo_linear_ce_backward': (_i, [C.POINTER(LinearCeArgs), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    'sgpo_newton_schulz_workspace_bytes': (_sz, [_i, _i, _i]),
+    'sgpo_newton_schulz': (_i, [_vp, _i, _i, _i, _i, _i64, _i64, C.POINTER(_f), _i, _f, _vp, _vp, _sz, _vp]),
+    'sgpo_muon_step': (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _f, _f, _i, _f, C.POINTER(_f), _i, _f, _vp, _sz, _vp]),
     'sgpo_gemm_bf16': (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
     'sgpo_f32_to_bf16': (_i, [_vp, _vp, _sz, _vp]),
     'sgpo_prof_enable': (_i, [_i, _i]),

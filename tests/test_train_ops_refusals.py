@@ -1,0 +1,97 @@
+"""CPU: what the training operators refuse, before anything reaches a device."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+def test_host_tensors_are_refused():
+    from sgpo_amd import _lib as L
+    from sgpo_amd import train_ops as T
+    q = torch.zeros(1, 2, 2, 8)
+    f = torch.zeros(4, dtype=torch.float64)
+    h, w, t = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(3, dtype=torch.int64)
+    for call in (lambda: T.rotary_positions(q, q, f), lambda: T.rotary_positions_(q, None, f), lambda: T.linear_cross_entropy(h, w, t),
+                 lambda: T.newton_schulz(w), lambda: T.muon_step(w, w, w, 0.1)):
+        with pytest.raises(L.SgpoError, match='host tensor'):
+            call()
+
+
+def test_frequencies():
+    from sgpo_amd import _lib as L
+    from sgpo_amd import train_ops as T
+    f, s = T.rotary_frequencies(64, device='cpu')
+    assert s == 1.0 and f.dtype == torch.float64
+    torch.testing.assert_close(f, 10000.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64), rtol=1e-15, atol=0)
+    lin, _ = T.rotary_frequencies(64, scaling='linear', factor=4.0, device='cpu')
+    torch.testing.assert_close(lin, f / 4, rtol=1e-15, atol=0)
+    ntk, _ = T.rotary_frequencies(64, scaling='ntk', factor=4.0, device='cpu')
+    assert float(ntk[0]) == 1.0 and abs(float(ntk[-1] / f[-1]) - 0.25) < 1e-12
+    yarn, s = T.rotary_frequencies(64, scaling='yarn', factor=4.0, device='cpu')
+    assert float(yarn[0]) == 1.0 and abs(float(yarn[-1] / f[-1]) - 0.25) < 1e-12 and abs(s - (1 + 0.1 * 1.3862943611198906)) < 1e-12
+    assert bool((yarn <= f).all()) and bool((yarn >= f / 4 * (1 - 1e-12)).all())
+    assert T.rotary_frequencies(0, device='cpu')[0].numel() == 0
+    for bad in (dict(rotary_dim=7), dict(rotary_dim=8, factor=0.5), dict(rotary_dim=8, scaling='cubic'), dict(rotary_dim=8, base=0.0),
+                dict(rotary_dim=8, scaling='yarn', beta_fast=1.0, beta_slow=2.0)):
+        with pytest.raises(L.SgpoError):
+            T.rotary_frequencies(device='cpu', **bad)
+
+
+def test_library_refuses_bad_arguments_without_a_device():
+    from sgpo_amd import _lib as L
+    lib = L.load()
+
+    def refused(rc, text):
+        assert rc < 0 and text in lib.sgpo_last_error().decode()
+
+    refused(lib.sgpo_rotary(None, None), 'null')
+    a = L.RotaryArgs(B=1, L=2, heads_q=1, head_dim=8, rot=10)
+    refused(lib.sgpo_rotary(C.byref(a), None), 'rot=10')
+    a = L.RotaryArgs(B=1, L=2, heads_q=1, head_dim=8, rot=3)
+    refused(lib.sgpo_rotary(C.byref(a), None), 'rot=3')
+    a = L.RotaryArgs(B=1, L=2, heads_q=1, head_dim=8, rot=8, dtype=7)
+    refused(lib.sgpo_rotary(C.byref(a), None), 'dtype')
+    a = L.RotaryArgs(B=1, L=2, heads_q=1, head_dim=8, rot=8)
+    refused(lib.sgpo_rotary(C.byref(a), None), 'frequencies')
+    a = L.RotaryArgs(B=1 << 16, L=1 << 16, heads_q=1, head_dim=8, rot=0)
+    refused(lib.sgpo_rotary(C.byref(a), None), 'tokens')
+    a = L.RotaryArgs(B=0, L=2, heads_q=1, head_dim=8, rot=8)
+    assert lib.sgpo_rotary(C.byref(a), None) == 0                # nothing to do
+
+    def loss(**kw):
+        v = dict(N=4, H=8, V=5, ld_hidden=8, ld_weight=8, reduction=1)
+        v.update(kw)
+        return C.byref(L.LinearCeArgs(**v))
+
+    for kw, text in ((dict(H=0), 'sizes'), (dict(V=0), 'sizes'), (dict(N=-1), 'sizes'), (dict(dtype=3), 'dtype'), (dict(reduction=4), 'reduction'),
+                     (dict(ld_hidden=7), 'pitch'), (dict(ld_weight=1 << 22), 'pitch')):
+        refused(lib.sgpo_linear_ce_forward(loss(**kw), None, None, None, None, None, 0, None), text)
+        refused(lib.sgpo_linear_ce_backward(loss(**kw), None, None, None, None, None, None, None, 0, None), text)
+        assert lib.sgpo_linear_ce_workspace_bytes(loss(**kw), 1) == 0
+    refused(lib.sgpo_linear_ce_forward(loss(), None, None, None, None, None, 0, None), 'null')
+    one = C.c_void_p(4096)                                       # never read: the workspace is refused first
+    refused(lib.sgpo_linear_ce_forward(C.byref(L.LinearCeArgs(hidden=4096, weight=4096, targets=4096, N=4, H=8, V=5, ld_hidden=8, ld_weight=8)),
+                                       one, one, one, one, one, 16, None), 'workspace')
+    coef = (C.c_float * 3)(1, 0, 0)
+    refused(lib.sgpo_newton_schulz(one, 0, 1, 4, 4, 16, 4, coef, 0, 1e-7, one, one, 1 << 30, None), 'triples')
+    refused(lib.sgpo_newton_schulz(one, 5, 1, 4, 4, 16, 4, coef, 1, 1e-7, one, one, 1 << 30, None), 'dtype')
+    refused(lib.sgpo_newton_schulz(one, 0, 1, 4, 4, 16, 3, coef, 1, 1e-7, one, one, 1 << 30, None), 'pitch')
+    refused(lib.sgpo_newton_schulz(one, 0, 1, 4, 4, 16, 4, coef, 1, 1e-7, one, one, 16, None), 'workspace')
+    refused(lib.sgpo_newton_schulz(one, 0, 1, -4, 4, 16, 4, coef, 1, 1e-7, one, one, 16, None), 'negative')
+    refused(lib.sgpo_muon_step(one, 0, one, 9, one, 1, 4, 4, 0.1, 0.9, 1, 0.0, coef, 1, 1e-7, one, 1 << 30, None), 'dtype')
+    refused(lib.sgpo_muon_step(one, 0, None, 0, one, 1, 4, 4, 0.1, 0.9, 1, 0.0, coef, 1, 1e-7, one, 1 << 30, None), 'null')
+    assert lib.sgpo_newton_schulz(None, 0, 0, 4, 4, 16, 4, coef, 1, 1e-7, None, None, 0, None) == 0
+
+
+def test_workspace_covers_every_split():
+    """Sizes that grow with the problem: positive, and never above a few copies of the operands and one piece of the vocabulary."""
+    from sgpo_amd import _lib as L
+    lib = L.load()
+    for dtype in (0, 1):
+        for N, H, V in ((1, 1, 1), (7, 517, 31), (1003, 517, 50021), (8192, 2048, 131072), (200000, 512, 31)):
+            a = L.LinearCeArgs(N=N, H=H, V=V, ld_hidden=H, ld_weight=H, dtype=dtype, reduction=1)
+            for backward in (0, 1):
+                got = lib.sgpo_linear_ce_workspace_bytes(C.byref(a), backward)
+                pad = lambda n: n + 64                           # noqa: E731
+                operands = 6 * (pad(N) + V) * pad(H)
+                assert 0 < got <= operands + (6 * max(1 << 27, pad(N) * 1088) + 4 * 64 * (pad(N) + 1024) * pad(H) + (1 << 28)), (dtype, N, H, V, backward, got)
