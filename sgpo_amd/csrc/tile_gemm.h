@@ -3,7 +3,7 @@
 //
 // Numbers.  An operand is stored as PL bf16 PLANES whose sum is the value: one plane is a plain bf16 matrix, two planes leave a
 // rest of at most 2^-17 |x|, three of 2^-26 |x| (an fp32 value's own half step is 2^-24).  Products of bf16 are exact in fp32.  The plane
-// pairs (i, j) with i + j < PL are multiplied -- 1, 3 or 6 MFMAs per product, smallest first; the pairs left out are below 2^-16 |x y| (two planes)
+// pairs (i, j) with i + j < PL are multiplied -- 1, 3 or 6 MFMAs per product; the pairs left out are below 2^-16 |x y| (two planes)
 // and 2^-24 |x y| (three).  The matrix cores run 16 bf16 MFMAs in the time of one fp32 MFMA of the same shape, so six bf16
 // products are 2.6 times the rate of native fp32.
 //
@@ -17,6 +17,7 @@
 // row on the source address and again on the read.
 #pragma once
 #include "common.h"
+#include <type_traits>
 
 namespace tg {
 
@@ -28,9 +29,9 @@ typedef __attribute__((address_space(3))) s16x4* lds_tr_t;
 
 enum { KC = 0, KM = 1 };
 
-// ld: stored elements between rows.  KC: `rows` rows may be read (indexes beyond are clamped: the caller masks what they give),
-// and every row holds k up to the last step, zero beyond the true k.  KM: `rows` k may be read (clamped likewise; the OTHER operand is zero
-// there), `cols` stored elements per row (a multiple of 8; chunks beyond are clamped, the caller masks what they give).
+// ld: stored elements between rows.  KC: `rows` rows exist (rows beyond read as zero), and every row holds k up to the last step, zero
+// beyond the true k.  KM: `rows` k exist (rows beyond read as zero), `cols` stored elements per row may be read (a multiple of 8; chunks
+// beyond are clamped, the caller masks what they give).  A tile's rows, or a step's, span less than 4 GiB.
 struct Operand {
   const bf16_t* p;
   int64_t ld;
@@ -65,60 +66,57 @@ __device__ __forceinline__ int km_swz(int row) {
 template <int PL>
 __device__ __forceinline__ int kc_swz(int row) { return PL == 3 ? (row >> 2) & 3 : (row >> 1) & 7; }
 
-// stages one operand's part of a step: R rows (KC) or columns (KM) of the tile
+// stages one operand's part of a step: R rows (KC) or columns (KM) of the tile, by buffer loads to LDS, whose bounds check gives the zeros
+// beyond the operand's rows without a branch in the loop
 template <class S, int R, int KIND>
 struct Stager {
   static constexpr int CH = KIND == KC ? S::ROWB / 16 : R * S::PL / 8;   // 16-B chunks per LDS row
   static constexpr int PIECES = R * S::ROWB / (16 * S::THREADS);
-  const char* base;       // uniform
+  uint64_t base;          // uniform: the step's first byte
+  int64_t left, step;     // bytes of the operand from there on; bytes between steps
   uint32_t off[PIECES];   // per lane, bytes
-  int64_t step;           // bytes per K step
-  int64_t ldb;
-  int krow0, krows;       // KM: first k row of this lane's pieces is row(j); k rows of the operand
 
   __device__ __forceinline__ void init(const Operand& o, int r0, int k0) {
     const int tid = threadIdx.x;
-    ldb = o.ld * 2;
+    const int64_t ldb = o.ld * 2;
     if constexpr (KIND == KC) {
-      base = reinterpret_cast<const char*>(o.p + (int64_t)r0 * o.ld + (int64_t)k0 * S::PL);
+      base = (uint64_t)(o.p + (int64_t)r0 * o.ld + (int64_t)k0 * S::PL);
+      left = (int64_t)(o.rows - r0) * ldb - (int64_t)k0 * S::PL * 2;
       step = S::ROWB;
-      const int last = o.rows - 1 - r0;
-#pragma unroll
-      for (int j = 0; j < PIECES; ++j) {
-        const int ci = j * S::THREADS + tid, row = ci / CH, c = (ci % CH) ^ kc_swz<S::PL>(row);
-        off[j] = (uint32_t)min(row, last) * (uint32_t)ldb + c * 16;
-      }
     } else {
-      base = reinterpret_cast<const char*>(o.p + (int64_t)k0 * o.ld + (int64_t)r0 * S::PL);
+      base = (uint64_t)(o.p + (int64_t)k0 * o.ld + (int64_t)r0 * S::PL);
+      left = (int64_t)(o.rows - k0) * ldb - (int64_t)r0 * S::PL * 2;
       step = S::KSTEP * ldb;
-      krow0 = k0; krows = o.rows;
-      const int last = (o.cols - r0 * S::PL) / 8 - 1;
+    }
 #pragma unroll
-      for (int j = 0; j < PIECES; ++j) {
-        const int ci = j * S::THREADS + tid, row = ci / CH, c = (ci % CH) ^ (km_swz<CH * 16>(row) << 1);
-        off[j] = (uint32_t)row * (uint32_t)ldb + min(c, last) * 16;
-      }
+    for (int j = 0; j < PIECES; ++j) {
+      const int ci = j * S::THREADS + tid, row = ci / CH;
+      int c;
+      if constexpr (KIND == KC) c = (ci % CH) ^ kc_swz<S::PL>(row);
+      else c = min((ci % CH) ^ (km_swz<CH * 16>(row) << 1), (o.cols - r0 * S::PL) / 8 - 1);
+      off[j] = (uint32_t)row * (uint32_t)ldb + c * 16;
     }
   }
-  // the next step, into `dst` (uniform)
-  __device__ __forceinline__ void next(char* dst) {
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
+    const uint32_t n = left > 0xffffffffll ? 0xffffffffu : left < 0 ? 0u : (uint32_t)left;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, n, 0x00027000);
+  }
+  __device__ __forceinline__ void piece(__amdgpu_buffer_rsrc_t r, int j, char* dst) const {   // dst: uniform
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    if (KIND == KC || krow0 + S::KSTEP <= krows) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr_t)(dst + (j * S::THREADS + wave * 64) * 16), 16, off[j], 0, 0, 0);
+  }
+  __device__ __forceinline__ void advance() { base += step; left -= step; }
+  __device__ __forceinline__ void next(char* dst) {   // the whole step
+    const __amdgpu_buffer_rsrc_t r = rsrc();
 #pragma unroll
-      for (int j = 0; j < PIECES; ++j)
-        __builtin_amdgcn_global_load_lds((gptr_t)(base + off[j]), (lptr_t)(dst + (j * S::THREADS + wave * 64) * 16), 16, 0, 0);
-    } else {
-#pragma unroll
-      for (int j = 0; j < PIECES; ++j) {
-        const int row = (j * S::THREADS + (int)threadIdx.x) / CH;
-        const int over = max(row - (krows - 1 - krow0), 0);   // rows past the last one read the last one
-        __builtin_amdgcn_global_load_lds((gptr_t)(base + off[j] - over * ldb), (lptr_t)(dst + (j * S::THREADS + wave * 64) * 16), 16, 0, 0);
-      }
-    }
-    base += step;
-    if constexpr (KIND == KM) krow0 += S::KSTEP;
+    for (int j = 0; j < PIECES; ++j) piece(r, j, dst);
+    advance();
   }
 };
+
+// The compiler drains the DMA queue (vmcnt 0) in front of a transposed LDS read unless the read carries alias information; `restrict` on
+// an inlined parameter gives it some.  What orders these reads after the DMA that fills their slot are the loop's own waits and barriers.
+__device__ __forceinline__ s16x4 read_tr(lds_tr_t __restrict__ p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
 
 // the 16 rows (columns) `g16` of the operand's tile, k slice or plane f
 template <class S, int R, int KIND>
@@ -131,25 +129,18 @@ __device__ __forceinline__ bf16x8 fragment(const char* img, int g16, int f, int 
     const int blk = S::PL == 1 ? g16 : (g16 >> 1) * (2 * S::PL) + f * 2 + (g16 & 1);
     const int row = (S::PL == 1 ? f * 32 : 0) + 8 * l4 + (l16 >> 2);
     const int at = row * RB + ((blk ^ km_swz<RB>(8 * l4 + (l16 >> 2))) * 32) + (l16 & 3) * 8;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t)(img + at));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t)(img + at + 4 * RB));
+    const s16x4 lo = read_tr((lds_tr_t)(img + at));
+    const s16x4 hi = read_tr((lds_tr_t)(img + at + 4 * RB));
     const s16x8 v = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     return *reinterpret_cast<const bf16x8*>(&v);
   }
 }
 
-// acc[mt][nt][q] += C[m = m0 + (wm MT + mt) 16 + l16][n = n0 + (wn NT + nt) 16 + 4 l4 + q], k steps [kt0, kt0 + nk).
-// Every thread of the workgroup calls it; smem is free again when it returns.
+// K loop with a ring of NST > 2 slots, for small tiles: NST - 1 steps in flight, one barrier a step.
 template <class S, int KA, int KB>
-__device__ __forceinline__ void run(const Operand& a, const Operand& b, int m0, int n0, int kt0, int nk, char* smem,
-                                    f32x4 (&acc)[S::MT][S::NT]) {
-  constexpr int D = S::NST - 1;
-  Stager<S, S::BM, KA> sa;
-  Stager<S, S::BN, KB> sb;
-  constexpr int OPS = Stager<S, S::BM, KA>::PIECES + Stager<S, S::BN, KB>::PIECES;
-  static_assert(OPS * (D > 1 ? D - 1 : 0) < 64, "vmcnt range");
-  sa.init(a, m0, kt0 * S::KSTEP);
-  sb.init(b, n0, kt0 * S::KSTEP);
+__device__ __forceinline__ void run_ring(Stager<S, S::BM, KA>& sa, Stager<S, S::BN, KB>& sb, int nk, char* smem, f32x4 (&acc)[S::MT][S::NT]) {
+  constexpr int D = S::NST - 1, OPS = Stager<S, S::BM, KA>::PIECES + Stager<S, S::BN, KB>::PIECES, NF = S::PL == 1 ? 2 : S::PL;
+  static_assert(D >= 2 && OPS * 2 < 64, "vmcnt range");
   const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
 #pragma unroll
@@ -158,8 +149,8 @@ __device__ __forceinline__ void run(const Operand& a, const Operand& b, int m0, 
   int slot = 0;
   for (int kt = 0; kt < nk; ++kt) {
     const int ahead = min(D - 1, nk - 1 - kt);   // younger steps in flight
-    if (D > 2 && ahead >= 2) wait_vm<(D > 2 ? 2 * OPS : 0)>();
-    else if (D > 1 && ahead >= 1) wait_vm<(D > 1 ? OPS : 0)>();
+    if (ahead >= 2) wait_vm<2 * OPS>();
+    else if (ahead >= 1) wait_vm<OPS>();
     else wait_vm<0>();
     __builtin_amdgcn_s_barrier();   // step kt is in LDS for everybody; everybody has read step kt - 1
     asm volatile("" ::: "memory");
@@ -171,43 +162,146 @@ __device__ __forceinline__ void run(const Operand& a, const Operand& b, int m0, 
     }
     const char* ia = smem + slot * S::STAGE;
     const char* ib = ia + S::A_BYTES;
-    constexpr int NF = S::PL == 1 ? 2 : S::PL;
-    if constexpr (S::PL == 1) {
+    bf16x8 fa[NF][S::MT], fb[NF][S::NT];
 #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        bf16x8 fa[S::MT], fb[S::NT];
+    for (int f = 0; f < NF; ++f) {
 #pragma unroll
-        for (int t = 0; t < S::NT; ++t) fb[t] = fragment<S, S::BN, KB>(ib, wn * S::NT + t, f, l16, l4);
+      for (int t = 0; t < S::NT; ++t) fb[f][t] = fragment<S, S::BN, KB>(ib, wn * S::NT + t, f, l16, l4);
 #pragma unroll
-        for (int t = 0; t < S::MT; ++t) fa[t] = fragment<S, S::BM, KA>(ia, wm * S::MT + t, f, l16, l4);
-#pragma unroll
-        for (int x = 0; x < S::MT; ++x)
-#pragma unroll
-          for (int y = 0; y < S::NT; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[y], fa[x], acc[x][y], 0, 0, 0);
-      }
-    } else {
-      // the planes of one side stay in registers, the other side's pass by in groups of rows
-      bf16x8 fb[NF][S::NT];
-#pragma unroll
-      for (int f = 0; f < NF; ++f)
-#pragma unroll
-        for (int t = 0; t < S::NT; ++t) fb[f][t] = fragment<S, S::BN, KB>(ib, wn * S::NT + t, f, l16, l4);
-#pragma unroll
-      for (int x = 0; x < S::MT; ++x) {
-        bf16x8 fa[NF];
-#pragma unroll
-        for (int f = 0; f < NF; ++f) fa[f] = fragment<S, S::BM, KA>(ia, wm * S::MT + x, f, l16, l4);
-#pragma unroll
-        for (int s = NF - 1; s >= 0; --s)   // plane pairs i + j = s, the smallest products first
-#pragma unroll
-          for (int i = 0; i <= s; ++i)
-#pragma unroll
-            for (int y = 0; y < S::NT; ++y)
-              acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[s - i][y], fa[i], acc[x][y], 0, 0, 0);
-      }
+      for (int t = 0; t < S::MT; ++t) fa[f][t] = fragment<S, S::BM, KA>(ia, wm * S::MT + t, f, l16, l4);
     }
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j)
+        if (S::PL == 1 ? i == j : i + j < S::PL)
+#pragma unroll
+          for (int x = 0; x < S::MT; ++x)
+#pragma unroll
+            for (int y = 0; y < S::NT; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j][y], fa[i][x], acc[x][y], 0, 0, 0);
     if (++slot == S::NST) slot = 0;
   }
+}
+
+// K loop for large tiles: two slots, and the fragments of the next products read while the present ones multiply.
+//
+// A step is 2 (one plane), 3 or 6 PHASES; a phase multiplies the fragments it holds, row block by row block, and between the row
+// blocks issues the LDS reads of what the next phases need.  The last reads of a slot belong to the last phase but one; then comes the
+// step's one barrier (the next step has landed: its DMA went out a whole step earlier; everybody's reads of this slot are done), and
+// the last phase issues the DMA of the step after next into the slot, piece by piece between its products: issued in one go the
+// pieces stall every wave of the CU at once for about a third of the step.
+// Measured on 8192 x 2048 x 8192, one plane, 256 x 256 tiles: 1060 TFLOP/s with DMA, reads and products in turn, 1380 this way
+// (KM operands 1130 - 1210); products alone, with nothing to load, 1720, the rate at which the card's power limit holds the clock.
+template <class S, int KA, int KB>
+__device__ __forceinline__ void run_phased(Stager<S, S::BM, KA>& sa, Stager<S, S::BN, KB>& sb, int nk, char* smem, f32x4 (&acc)[S::MT][S::NT]) {
+  constexpr int MT = S::MT, NT = S::NT, NPA = Stager<S, S::BM, KA>::PIECES, NP = NPA + Stager<S, S::BN, KB>::PIECES;
+  static_assert(S::NST == 2 && NP < 64, "two slots");
+  typedef bf16x8 FA[MT];
+  typedef bf16x8 FB[NT];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  auto read_a = [&](FA& f, int t, const char* img, int plane) { f[t] = fragment<S, S::BM, KA>(img, wm * MT + t, plane, l16, l4); };
+  auto read_b = [&](FB& f, int t, const char* img, int plane) { f[t] = fragment<S, S::BN, KB>(img + S::A_BYTES, wn * NT + t, plane, l16, l4); };
+  // products of (a, b), and of what follows: na from plane pa if WA, nb from plane pb if WB, both of image `img`; DMA into `dst`
+  auto phase = [&](const FA& a, const FB& b, auto wa, FA& na, int pa, auto wb, FB& nb, int pb, const char* img, auto dma, char* dst) {
+    constexpr int RB = decltype(wb)::value ? NT : 0, R = RB + (decltype(wa)::value ? MT : 0);
+    __amdgpu_buffer_rsrc_t ra, rb;
+    if constexpr (decltype(dma)::value) { ra = sa.rsrc(); rb = sb.rsrc(); }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < MT; ++x) {
+      if constexpr (decltype(dma)::value) {
+#pragma unroll
+        for (int j = x * NP / MT; j < (x + 1) * NP / MT; ++j) {
+          if (j < NPA) sa.piece(ra, j, dst);
+          else sb.piece(rb, j - NPA, dst + S::A_BYTES);
+        }
+      }
+#pragma unroll
+      for (int i = x * R / MT; i < (x + 1) * R / MT; ++i) {
+        if (i < RB) read_b(nb, i, img, pb);
+        else read_a(na, i - RB, img, pa);
+      }
+#pragma unroll
+      for (int y = 0; y < NT; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[y], a[x], acc[x][y], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (decltype(dma)::value) { sa.advance(); sb.advance(); }
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  auto meet = [&]() {
+    wait_vm<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  sa.next(smem); sb.next(smem + S::A_BYTES);
+  if (nk > 1) {
+    sa.next(smem + S::STAGE); sb.next(smem + S::STAGE + S::A_BYTES);
+    wait_vm<NP>();
+  } else {
+    wait_vm<0>();
+  }
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  // The order of a step's products lets the next step start in the same registers as this one.  The reads that a last step makes for the
+  // step after it find what lies in the other slot; nothing uses them.
+  FA a0, a1;
+  FB b0, b1;
+  auto first = [&](FB& fb, int pb) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) read_b(fb, t, smem, pb);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) read_a(a0, t, smem, 0);
+  };
+  auto all = [&](auto step) {
+    int kt = 0;
+    for (; kt + 2 < nk; ++kt) step(smem + (kt & 1) * S::STAGE, smem + (~kt & 1) * S::STAGE, yes);
+    for (; kt < nk; ++kt) step(smem + (kt & 1) * S::STAGE, smem + (~kt & 1) * S::STAGE, no);
+  };
+  if constexpr (S::PL == 1) {   // "planes" 0 and 1 are the two halves of the 64 k
+    first(b0, 0);
+    all([&](char* cur, char* nxt, auto dma) {
+      phase(a0, b0, yes, a1, 1, yes, b1, 1, cur, no, cur);
+      meet();
+      phase(a1, b1, yes, a0, 0, yes, b0, 0, nxt, dma, cur);
+    });
+  } else if constexpr (S::PL == 2) {
+    first(b1, 1);
+    all([&](char* cur, char* nxt, auto dma) {
+      phase(a0, b1, no, a1, 0, yes, b0, 0, cur, no, cur);
+      phase(a0, b0, yes, a1, 1, no, b1, 0, cur, no, cur);
+      meet();
+      phase(a1, b0, yes, a0, 0, yes, b1, 1, nxt, dma, cur);
+    });
+  } else {
+    FA a2;
+    FB b2;
+    first(b2, 2);
+    all([&](char* cur, char* nxt, auto dma) {
+      phase(a0, b2, no, a1, 0, yes, b1, 1, cur, no, cur);
+      phase(a0, b1, no, a1, 0, yes, b0, 0, cur, no, cur);
+      phase(a0, b0, yes, a1, 1, no, b2, 0, cur, no, cur);
+      phase(a1, b1, yes, a2, 2, no, b2, 0, cur, no, cur);
+      phase(a1, b0, no, a0, 0, no, b2, 0, cur, no, cur);
+      meet();
+      phase(a2, b0, yes, a0, 0, yes, b2, 2, nxt, dma, cur);
+    });
+  }
+}
+
+// acc[mt][nt][q] += C[m = m0 + (wm MT + mt) 16 + l16][n = n0 + (wn NT + nt) 16 + 4 l4 + q], k steps [kt0, kt0 + nk), nk >= 1.
+// Every thread of the workgroup calls it; smem is free again when it returns.
+template <class S, int KA, int KB>
+__device__ __forceinline__ void run(const Operand& a, const Operand& b, int m0, int n0, int kt0, int nk, char* smem, f32x4 (&acc)[S::MT][S::NT]) {
+  Stager<S, S::BM, KA> sa;
+  Stager<S, S::BN, KB> sb;
+  sa.init(a, m0, kt0 * S::KSTEP);
+  sb.init(b, n0, kt0 * S::KSTEP);
+  if constexpr (S::NST == 2) run_phased<S, KA, KB>(sa, sb, nk, smem, acc);
+  else run_ring<S, KA, KB>(sa, sb, nk, smem, acc);
   __syncthreads();
 }
 
