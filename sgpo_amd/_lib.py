@@ -103,10 +103,11 @@ SIGNATURES = {
     'sgpo_daps_mh_workspace_bytes': (_sz, []),
     'sgpo_daps_mh': (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _f, _f, _f, _i, _i, _vp, _vp, _vp, _u64, _u64, _u64,
                           _vp, _vp, _sz, _vp]),
-    'sgpo_rotary': (_i, [C.POINTER(RotaryArgs), _vp]),
-    'sgpo_linear_ce_workspace_bytes': (_sz, [C.POINTER(LinearCeArgs), _i]),
-    'sgpo_linear_ce_forward': (_i, [C.POINTER(LinearCeArgs), _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    'sgpo_linear_ce_backward': (_i, [C.POINTER(LinearCeArgs), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    # argument blocks: RotaryArgs / LinearCeArgs by reference, or the same bytes
+    'sgpo_rotary': (_i, [_vp, _vp]),
+    'sgpo_linear_ce_workspace_bytes': (_sz, [_vp, _i]),
+    'sgpo_linear_ce_forward': (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    'sgpo_linear_ce_backward': (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     'sgpo_newton_schulz_workspace_bytes': (_sz, [_i, _i, _i]),
     'sgpo_newton_schulz': (_i, [_vp, _i, _i, _i, _i, _i64, _i64, C.POINTER(_f), _i, _f, _vp, _vp, _sz, _vp]),
     'sgpo_muon_step': (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _f, _f, _i, _f, C.POINTER(_f), _i, _f, _vp, _sz, _vp]),

@@ -7,47 +7,59 @@ tape).  Every tensor is fp32 or bf16 device memory on the process's one GPU; a c
 device, allocates its outputs and scratch from torch's allocator (so it can be captured into a graph and used on any stream), and
 does not synchronise.  There is no CPU fallback: bad arguments and host tensors raise SgpoError.
 """
-import ctypes as C
 import math
+import struct
 
 import torch
 
 from . import _lib as L
-from .runtime import init
+from . import runtime
 
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)     # Newton-Schulz quintic: singular values into about [0.7, 1.2] within 5 steps
 _DTYPES = {torch.float32: L.DTYPE_F32, torch.bfloat16: L.DTYPE_BF16}
 _REDUCE = {'none': L.REDUCE_NONE, 'mean': L.REDUCE_MEAN, 'sum': L.REDUCE_SUM}
+# The argument blocks of the C calls, packed in one go: filling a ctypes structure field by field takes longer than the smallest of
+# these kernels.  Same order and padding as L.RotaryArgs and L.LinearCeArgs (checked below).
+_ROTARY = struct.Struct('=4Q12qQ2qQ9if')
+_LOSS = struct.Struct('=4Q3q5i4x')
+assert _ROTARY.size == L.C.sizeof(L.RotaryArgs) and _LOSS.size == L.C.sizeof(L.LinearCeArgs)
 
 
-def _require(ok, text):
-    if not ok:
-        raise L.SgpoError(text)
+def _refuse(text):
+    raise L.SgpoError(text)
 
 
 def _dtype(t, what):
-    _require(t.dtype in _DTYPES, f'{what} must be float32 or bfloat16, got {t.dtype}')
+    if t.dtype not in _DTYPES:
+        _refuse(f'{what} must be float32 or bfloat16, got {t.dtype}')
     return _DTYPES[t.dtype]
 
 
 def _on_device(first, *others):
     """The device of a call's tensors, all on one GPU, which is the one this process is bound to."""
     for t in (first, *others):
-        _require(t is None or isinstance(t, torch.Tensor), f'a tensor is expected, got {type(t).__name__}')
-        if t is not None and not t.is_cuda:
-            raise L.SgpoError(f'host tensor {tuple(t.shape)} {t.dtype} passed where the library expects device memory')
-        _require(t is None or t.device == first.device, f'tensors on {first.device} and on another device')
-    return init(first.device)
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            _refuse(f'a tensor is expected, got {type(t).__name__}')
+        if not t.is_cuda:
+            _refuse(f'host tensor {tuple(t.shape)} {t.dtype} passed where the library expects device memory')
+        if t.device != first.device:
+            _refuse(f'tensors on {first.device} and on {t.device}')
+    dev = first.device
+    if dev.index not in runtime._initialised:
+        runtime.init(dev)
+    return dev
 
 
-def _stream(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev.index)     # torch.cuda.current_stream(dev).cuda_stream without the object
 
 
-def _scratch(nbytes, device):
-    """Scratch of one call, 256-byte aligned; from torch's allocator, which keeps streams and captured graphs apart."""
-    buf = torch.empty(int(nbytes) + 256, dtype=torch.uint8, device=device)
-    return buf, C.c_void_p((buf.data_ptr() + 255) & ~255)
+def _scratch(nbytes, dev):
+    """(tensor, address, bytes) of one call's scratch, 256-byte aligned; from torch's allocator, which keeps streams and captured graphs apart."""
+    buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=dev)
+    return buf, (buf.data_ptr() + 255) & ~255
 
 
 # ---------------------------------------------------------------------------------------------------------------- rotation
@@ -60,14 +72,18 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
     scaling None; 'linear': every angle / factor; 'ntk': base * factor ** (rotary_dim / (rotary_dim - 2)), which keeps the fastest pair
     and divides the slowest by factor; 'yarn': pairs that turn more than beta_fast times within original_length positions stay, those
     below beta_slow turns are divided by factor, linearly in between, and rotated elements are scaled by 0.1 ln(factor) + 1."""
-    _require(rotary_dim >= 0 and rotary_dim % 2 == 0, f'rotary_dim must be even, got {rotary_dim}')
-    _require(base > 0 and factor >= 1, f'base must be positive and factor at least 1, got {base} and {factor}')
-    _require(scaling in (None, 'linear', 'ntk', 'yarn'), f'unknown scaling {scaling!r}')
+    if rotary_dim < 0 or rotary_dim % 2:
+        _refuse(f'rotary_dim must be even, got {rotary_dim}')
+    if not (base > 0 and factor >= 1):
+        _refuse(f'base must be positive and factor at least 1, got {base} and {factor}')
+    if scaling not in (None, 'linear', 'ntk', 'yarn'):
+        _refuse(f'unknown scaling {scaling!r}')
     out, scale = [], 1.0
     if scaling == 'ntk':
         base = base * factor ** (rotary_dim / max(rotary_dim - 2, 1))
     if scaling == 'yarn':
-        _require(beta_fast > beta_slow, 'beta_fast must be larger than beta_slow')
+        if beta_fast <= beta_slow:
+            _refuse('beta_fast must be larger than beta_slow')
         scale = 0.1 * math.log(factor) + 1.0
     for j in range(0, rotary_dim, 2):
         f = base ** (-j / rotary_dim)
@@ -82,53 +98,51 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
 
 def _rotate(q, k, frequencies, positions, interleaved, scale, inverse, in_place=False):
     dev = _on_device(q, k, frequencies, positions)
-    _require(q.dim() == 4, f'heads are (batch, tokens, heads, head_dim), got {tuple(q.shape)}')
-    B, Lq, Hq, D = q.shape
     dt = _dtype(q, 'q')
+    if q.dim() != 4:
+        _refuse(f'heads are (batch, tokens, heads, head_dim), got {tuple(q.shape)}')
+    B, Lq, Hq, D = q.shape
+    Hk = 0
     if k is not None:
-        _require(k.dim() == 4 and (k.shape[0], k.shape[1], k.shape[3]) == (B, Lq, D) and k.dtype == q.dtype,
-                 f'k {tuple(k.shape)} {k.dtype} does not match q {tuple(q.shape)} {q.dtype}')
-    _require(frequencies.dtype == torch.float64 and frequencies.dim() == 1 and frequencies.is_contiguous(), 'frequencies must be a contiguous float64 vector')
+        if k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], k.shape[1], k.shape[3]) != (B, Lq, D):
+            _refuse(f'k {tuple(k.shape)} {k.dtype} does not match q {tuple(q.shape)} {q.dtype}')
+        Hk = k.shape[2]
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+        _refuse('frequencies must be a contiguous float64 vector')
     rot = 2 * frequencies.numel()
-    _require(rot <= D, f'{rot} rotated elements in heads of {D}')
-    psb = psl = 0
+    if rot > D:
+        _refuse(f'{rot} rotated elements in heads of {D}')
+    pos = psb = psl = 0
     if positions is not None:
-        _require(positions.dtype == torch.int64, f'positions must be int64, got {positions.dtype}')
-        _require(tuple(positions.shape) in ((Lq,), (B, Lq), (1, Lq), (B, 1)), f'positions {tuple(positions.shape)} for {B} x {Lq} tokens')
-        if positions.dim() == 1:
-            psl = positions.stride(0)
-        else:
-            psb = positions.stride(0) if positions.shape[0] > 1 else 0
-            psl = positions.stride(1) if positions.shape[1] > 1 else 0
-            _require(positions.shape[1] == Lq, f'positions {tuple(positions.shape)} for {B} x {Lq} tokens')
-    a = L.RotaryArgs()
-    src, dst = [], []
-    for t in (q, k):
-        if t is None:
-            src.append(None)
-            dst.append(None)
-            continue
-        s = t if t.stride(3) == 1 or D == 1 or not t.numel() else t.contiguous()
-        if in_place:
-            _require(s is t, 'in place, the elements of a head must be contiguous')
-            _require(all(st > 0 or n <= 1 for st, n in zip(t.stride(), t.shape)), 'in place, heads must not be broadcast')
-        src.append(s)
-        dst.append(s if in_place else torch.empty(t.shape, dtype=t.dtype, device=dev))
-    for name, s, d in (('q', src[0], dst[0]), ('k', src[1], dst[1])):
-        if s is None:
-            continue
-        setattr(a, name, s.data_ptr())
-        setattr(a, name + '_out', d.data_ptr())
-        for i in range(3):
-            getattr(a, name + '_stride')[i] = s.stride(i)
-            getattr(a, name + '_out_stride')[i] = d.stride(i)
-    a.positions = None if positions is None else positions.data_ptr()
-    a.pos_stride_b, a.pos_stride_l = psb, psl
-    a.frequencies = frequencies.data_ptr()
-    a.B, a.L, a.heads_q, a.heads_k, a.head_dim, a.rot = B, Lq, Hq, 0 if k is None else k.shape[2], D, rot
-    a.interleaved, a.inverse, a.dtype, a.scale = int(interleaved), int(inverse), dt, float(scale)
-    L.check(L.load().sgpo_rotary(C.byref(a), _stream(dev)), 'sgpo_rotary')
-    return dst
+        ps = tuple(positions.shape)
+        if positions.dtype != torch.int64 or ps not in ((Lq,), (B, Lq), (1, Lq)):
+            _refuse(f'positions must be int64 for {B} x {Lq} tokens, got {ps} {positions.dtype}')
+        pos, psl = positions.data_ptr(), positions.stride(-1)
+        psb = positions.stride(0) if len(ps) == 2 and ps[0] > 1 else 0
+    if in_place:
+        for t in (q, k):
+            if t is not None and (t.stride(3) != 1 and D > 1 or any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape))):
+                _refuse('in place, the elements of a head must be contiguous and heads must not be broadcast')
+        qo, ko = q, k
+    else:
+        if D > 1 and q.stride(3) != 1:
+            q = q.contiguous()
+        qo, ko = q.new_empty((B, Lq, Hq, D)), None
+        if k is not None:
+            if D > 1 and k.stride(3) != 1:
+                k = k.contiguous()
+            ko = k.new_empty((B, Lq, Hk, D))
+    if k is None:
+        kp = kop = 0
+        ks = kos = (0, 0, 0)
+    else:
+        kp, kop, ks, kos = k.data_ptr(), ko.data_ptr(), k.stride()[:3], ko.stride()[:3]
+    args = _ROTARY.pack(q.data_ptr(), qo.data_ptr(), kp, kop, *q.stride()[:3], *qo.stride()[:3], *ks, *kos, pos, psb, psl, frequencies.data_ptr(),
+                        B, Lq, Hq, Hk, D, rot, interleaved, inverse, dt, scale)
+    rc = L.load().sgpo_rotary(args, _stream(dev))
+    if rc:
+        L.check(rc, 'sgpo_rotary')
+    return qo, ko
 
 
 class _Rotary(torch.autograd.Function):
@@ -136,15 +150,13 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, q, k, frequencies, positions, interleaved, scale):
         ctx.save_for_backward(frequencies, positions)
         ctx.how = interleaved, scale
-        out = _rotate(q, k, frequencies, positions, interleaved, scale, False)
-        return out[0], out[1]
+        return _rotate(q, k, frequencies, positions, interleaved, scale, False)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         frequencies, positions = ctx.saved_tensors
-        got = _rotate(dq, dk, frequencies, positions, *ctx.how, True)
-        return got[0], got[1], None, None, None, None
+        return (*_rotate(dq, dk, frequencies, positions, *ctx.how, True), None, None, None, None)
 
 
 def rotary_positions(q, k, frequencies, positions=None, interleaved=False, scale=1.0):
@@ -155,29 +167,26 @@ def rotary_positions(q, k, frequencies, positions=None, interleaved=False, scale
     (j, j + rot / 2), or (2 j, 2 j + 1) if interleaved.  q and k may be views with any strides (of one packed projection, or of
     (B, H, L, D) tensors); only heads that are not contiguous in memory are copied first."""
     if not (torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad)):
-        out = _rotate(q, k, frequencies, positions, interleaved, scale, False)
-        return out[0], out[1]
-    return _Rotary.apply(q, k, frequencies, positions, bool(interleaved), float(scale))
+        return _rotate(q, k, frequencies, positions, interleaved, scale, False)
+    return _Rotary.apply(q, k, frequencies, positions, interleaved, scale)
 
 
 def rotary_positions_(q, k, frequencies, positions=None, interleaved=False, scale=1.0):
     """rotary_positions written over q and k (as the reference's apply_rotary_emb_qkv_, dit.py:112-115); not differentiable."""
-    _require(not (torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad)), 'rotary_positions_ has no gradient: use rotary_positions')
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+        _refuse('rotary_positions_ has no gradient: use rotary_positions')
     _rotate(q, k, frequencies, positions, interleaved, scale, False, in_place=True)
+    torch.autograd.graph.increment_version(q if k is None else (q, k))     # what autograd saved of them is stale now
     return q, k
 
 
 # -------------------------------------------------------------------------------------------------------------------- loss
 
 def _loss_args(hidden, weight, targets, bias, ignore_index, reduction):
-    a = L.LinearCeArgs()
-    a.hidden, a.weight, a.targets = hidden.data_ptr(), weight.data_ptr(), targets.data_ptr()
-    a.bias = None if bias is None else bias.data_ptr()
-    (a.N, a.H), a.V = hidden.shape, weight.shape[0]
-    a.ld_hidden = hidden.stride(0) if a.N > 1 else a.H
-    a.ld_weight = weight.stride(0) if a.V > 1 else a.H
-    a.ignore_index, a.dtype, a.reduction = ignore_index, _DTYPES[hidden.dtype], _REDUCE[reduction]
-    return a
+    N, H = hidden.shape
+    V = weight.shape[0]
+    return _LOSS.pack(hidden.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), targets.data_ptr(), hidden.stride(0) if N > 1 else H,
+                      weight.stride(0) if V > 1 else H, ignore_index, N, H, V, _DTYPES[hidden.dtype], reduction)
 
 
 def _rows(t):
@@ -186,42 +195,50 @@ def _rows(t):
 
 
 def _loss_forward(hidden, weight, targets, bias, ignore_index, reduction):
+    """(loss or losses, state for the backward pass: the tokens' log-sums, the gradient's factor, and losses that are only summed)."""
     dev = hidden.device
     lib = L.load()
-    a = _loss_args(hidden, weight, targets, bias, ignore_index, reduction)
-    need = lib.sgpo_linear_ce_workspace_bytes(C.byref(a), 0)
+    N = hidden.shape[0]
+    args = _loss_args(hidden, weight, targets, bias, ignore_index, reduction)
+    need = lib.sgpo_linear_ce_workspace_bytes(args, 0)
     buf, ws = _scratch(need, dev)
-    out = torch.empty(2 * a.N + 2, dtype=torch.float32, device=dev)
-    nll, lse, loss, inv = out[:a.N], out[a.N:2 * a.N], out[2 * a.N], out[2 * a.N + 1]
-    L.check(lib.sgpo_linear_ce_forward(C.byref(a), L.ptr(nll), L.ptr(lse), L.ptr(loss), L.ptr(inv), ws, need, _stream(dev)),
-            'sgpo_linear_ce_forward')
-    return nll if reduction == 'none' else loss, lse, inv
+    state = torch.empty(2 * N + 1 if reduction else N + 1, dtype=torch.float32, device=dev)
+    out = torch.empty((N,) if reduction == 0 else (), dtype=torch.float32, device=dev)
+    lse = state.data_ptr()
+    inv, o = lse + 4 * N, out.data_ptr()
+    rc = lib.sgpo_linear_ce_forward(args, inv + 4 if reduction else o, lse, o, inv, ws, need, _stream(dev))
+    if rc:
+        L.check(rc, 'sgpo_linear_ce_forward')
+    return out, state
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, bias, ignore_index, reduction):
-        out, lse, inv = _loss_forward(hidden, weight, targets, bias, ignore_index, reduction)
-        ctx.save_for_backward(hidden, weight, targets, bias, lse, inv)
+        out, state = _loss_forward(hidden, weight, targets, bias, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, targets, bias, state)
         ctx.how = ignore_index, reduction
-        return out.clone()      # its own storage: lse and inv live behind it
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, targets, bias, lse, inv = ctx.saved_tensors
+        hidden, weight, targets, bias, state = ctx.saved_tensors
         dev = hidden.device
         lib = L.load()
-        a = _loss_args(hidden, weight, targets, bias, *ctx.how)
-        grad = grad.to(torch.float32).contiguous()
+        args = _loss_args(hidden, weight, targets, bias, *ctx.how)
+        grad = grad.contiguous()
         want = ctx.needs_input_grad
-        dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want[0] else None
-        dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want[1] else None
-        db = torch.empty(bias.shape, dtype=torch.float32, device=dev) if want[3] else None
-        need = lib.sgpo_linear_ce_workspace_bytes(C.byref(a), 1)
+        dh = hidden.new_empty(hidden.shape) if want[0] else None
+        dw = weight.new_empty(weight.shape) if want[1] else None
+        db = bias.new_empty(bias.shape) if want[3] else None
+        need = lib.sgpo_linear_ce_workspace_bytes(args, 1)
         buf, ws = _scratch(need, dev)
-        L.check(lib.sgpo_linear_ce_backward(C.byref(a), L.ptr(lse), L.ptr(grad), L.ptr(inv), L.ptr(dh), L.ptr(dw), L.ptr(db), ws, need,
-                                            _stream(dev)), 'sgpo_linear_ce_backward')
+        lse = state.data_ptr()
+        rc = lib.sgpo_linear_ce_backward(args, lse, grad.data_ptr(), lse + 4 * hidden.shape[0], None if dh is None else dh.data_ptr(),
+                                         None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), ws, need, _stream(dev))
+        if rc:
+            L.check(rc, 'sgpo_linear_ce_backward')
         return dh, dw, None, db, None, None
 
 
@@ -233,49 +250,77 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
     closes a class (the mask class of an absorbing-state model, mdlm_diffusion.py:325-341).  reduction 'none' gives fp32 losses of
     targets' shape; 'sum' and 'mean' (over the targets that are not ignore_index; 0 if there are none) give a scalar.  An ignored token has loss
     and gradients 0 whatever its features hold; a target outside [0, V) gives NaN, as no check on the host waits for the GPU."""
-    dev = _on_device(hidden, weight, targets, bias)
+    _on_device(hidden, weight, targets, bias)
     _dtype(hidden, 'hidden')
-    _require(hidden.dim() >= 1 and weight.dim() == 2 and hidden.shape[-1] == weight.shape[1] and weight.numel() > 0,
-             f'hidden {tuple(hidden.shape)} does not match weight {tuple(weight.shape)}')
-    _require(weight.dtype == hidden.dtype, f'hidden is {hidden.dtype} and weight {weight.dtype}')
-    _require(targets.dtype == torch.int64 and targets.shape == hidden.shape[:-1], f'targets {tuple(targets.shape)} {targets.dtype} for hidden {tuple(hidden.shape)}')
-    _require(bias is None or bias.dtype == torch.float32 and tuple(bias.shape) == (weight.shape[0],), 'bias must be float32 with one value per class')
-    _require(reduction in _REDUCE, f'unknown reduction {reduction!r}')
-    h, w = _rows(hidden.reshape(-1, hidden.shape[-1])), _rows(weight)
-    t = targets.reshape(-1).contiguous()
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or weight.numel() == 0:
+        _refuse(f'hidden {tuple(hidden.shape)} does not match weight {tuple(weight.shape)}')
+    if weight.dtype != hidden.dtype:
+        _refuse(f'hidden is {hidden.dtype} and weight {weight.dtype}')
+    if targets.dtype != torch.int64 or targets.shape != hidden.shape[:-1]:
+        _refuse(f'targets {tuple(targets.shape)} {targets.dtype} for hidden {tuple(hidden.shape)}')
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (weight.shape[0],)):
+        _refuse('bias must be float32 with one value per class')
+    if reduction not in _REDUCE:
+        _refuse(f'unknown reduction {reduction!r}')
+    red = _REDUCE[reduction]
+    h = _rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1]))
+    w = _rows(weight)
+    t = targets if targets.dim() == 1 and targets.is_contiguous() else targets.reshape(-1).contiguous()
     b = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (hidden, weight, bias)):
-        out = _LinearCrossEntropy.apply(h, w, t, b, int(ignore_index), reduction)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad):
+        out = _LinearCrossEntropy.apply(h, w, t, b, int(ignore_index), red)
     else:
-        out = _loss_forward(h, w, t, b, int(ignore_index), reduction)[0]
-    return out.view(targets.shape) if reduction == 'none' else out
+        out = _loss_forward(h, w, t, b, int(ignore_index), red)[0]
+    return out.view(targets.shape) if red == 0 and targets.dim() != 1 else out
 
 
 # ----------------------------------------------------------------------------------------------------------------- updates
 
+_tables = {}     # coefficients -> their C array
+
+
 def _coefficients(coefficients, steps):
-    c = [float(v) for row in (coefficients if isinstance(coefficients[0], (tuple, list)) else [coefficients] * steps) for v in row]
-    _require(len(c) == 3 * steps and steps >= 1, f'{steps} steps need {steps} coefficient triples')
-    return (C.c_float * len(c))(*c)
+    key = (tuple(map(tuple, coefficients)) if isinstance(coefficients[0], (tuple, list)) else tuple(coefficients), steps)
+    table = _tables.get(key)
+    if table is None:
+        rows = key[0] if isinstance(key[0][0], tuple) else (key[0],) * max(steps, 0)
+        flat = [float(v) for row in rows for v in row]
+        if steps < 1 or len(rows) != steps or len(flat) != 3 * steps:
+            _refuse(f'{steps} steps need {steps} coefficient triples')
+        if len(_tables) >= 64:
+            _tables.clear()
+        table = _tables[key] = (L.C.c_float * len(flat))(*flat)
+    return table
 
 
 def newton_schulz(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
     """The update (..., m, n) with every singular value moved towards 1 and its singular vectors kept: X = U / (|U|_F + eps), then
     X <- a X + (b X X^T + c (X X^T)^2) X per coefficient triple (one triple for all steps, or one each).  Leading dimensions are independent matrices.
-    update fp32 or bf16; returns bf16, contiguous.  Iterates carry 16 bits of mantissa, sums 32 bits, the norm 64.  Not differentiable."""
+    update fp32 or bf16; returns bf16, contiguous.  Iterates carry 17 bits, sums 32, the norm 64.  Not differentiable."""
     dev = _on_device(update)
     dt = _dtype(update, 'update')
-    _require(update.dim() >= 2, f'an update is a matrix or a batch of them, got {tuple(update.shape)}')
-    m, n = update.shape[-2:]
-    u = update.detach().reshape(-1, m, n) if update.numel() else update.detach().new_empty(0, m, n)
-    if u.numel() and (u.stride(2) != 1 and n > 1 or m > 1 and u.stride(1) < n):
+    if update.dim() < 2:
+        _refuse(f'an update is a matrix or a batch of them, got {tuple(update.shape)}')
+    u = update.detach()
+    m, n = u.shape[-2:]
+    out = torch.empty(u.shape, dtype=torch.bfloat16, device=dev)
+    table = _coefficients(coefficients, steps)
+    if not u.numel():
+        return out
+    if u.dim() == 2:
+        batch, sb, ld = 1, 0, u.stride(0)
+    else:
+        u = u.reshape(-1, m, n)
+        batch, sb, ld = u.shape[0], u.stride(0), u.stride(1)
+    if u.stride(-1) != 1 and n > 1 or m > 1 and ld < n:
         u = u.contiguous()
-    out = torch.empty(update.shape, dtype=torch.bfloat16, device=dev)
+        sb, ld = m * n, n
     lib = L.load()
-    need = lib.sgpo_newton_schulz_workspace_bytes(u.shape[0], m, n)
+    need = lib.sgpo_newton_schulz_workspace_bytes(batch, m, n)
     buf, ws = _scratch(need, dev)
-    L.check(lib.sgpo_newton_schulz(L.ptr(u), dt, u.shape[0], m, n, u.stride(0), u.stride(1), _coefficients(coefficients, steps), steps, float(eps),
-                                   L.ptr(out), ws, need, _stream(dev)), 'sgpo_newton_schulz')
+    rc = lib.sgpo_newton_schulz(u.data_ptr(), dt, batch, m, n, sb, ld, table, steps, eps, out.data_ptr(), ws, need, _stream(dev))
+    if rc:
+        L.check(rc, 'sgpo_newton_schulz')
     return out
 
 
@@ -286,18 +331,29 @@ def muon_step(weight, grad, momentum_buffer, lr, momentum=0.95, nesterov=True, w
 
     buffer = momentum * buffer + grad;  U = grad + momentum * buffer (nesterov) or buffer;  weight = (1 - lr * weight_decay) * weight -
     lr * sqrt(max(1, m / n)) * newton_schulz(U), the last product not rounded before it is applied.  weight and grad fp32 or bf16,
-    momentum_buffer fp32 (the caller's state, zeros at first), all contiguous.  Returns weight."""
+    momentum_buffer fp32 (the caller's state, zeros at first); weight and buffer contiguous.  Returns weight."""
     dev = _on_device(weight, grad, momentum_buffer)
     wd, gd = _dtype(weight, 'weight'), _dtype(grad, 'grad')
-    _require(weight.dim() >= 2 and weight.shape == grad.shape == momentum_buffer.shape, f'weight {tuple(weight.shape)}, grad {tuple(grad.shape)} and buffer {tuple(momentum_buffer.shape)} must agree')
-    _require(momentum_buffer.dtype == torch.float32, 'momentum_buffer must be float32')
-    _require(weight.is_contiguous() and momentum_buffer.is_contiguous(), 'weight and momentum_buffer are updated in place and must be contiguous')
+    if weight.dim() < 2 or not weight.shape == grad.shape == momentum_buffer.shape:
+        _refuse(f'weight {tuple(weight.shape)}, grad {tuple(grad.shape)} and buffer {tuple(momentum_buffer.shape)} must agree')
+    if momentum_buffer.dtype != torch.float32:
+        _refuse('momentum_buffer must be float32')
+    if not (weight.is_contiguous() and momentum_buffer.is_contiguous()):
+        _refuse('weight and momentum_buffer are updated in place and must be contiguous')
+    if torch.is_grad_enabled() and weight.requires_grad and not weight.is_leaf:
+        _refuse('weight is part of a graph: a step updates leaves')
+    table = _coefficients(coefficients, steps)
+    if not weight.numel():
+        return weight
     g = grad.detach().contiguous()
     m, n = weight.shape[-2:]
-    batch = weight.numel() // (m * n) if m * n else 0
+    batch = weight.numel() // (m * n)
     lib = L.load()
     need = lib.sgpo_newton_schulz_workspace_bytes(batch, m, n)
     buf, ws = _scratch(need, dev)
-    L.check(lib.sgpo_muon_step(L.ptr(weight), wd, L.ptr(g), gd, L.ptr(momentum_buffer), batch, m, n, float(lr), float(momentum), int(bool(nesterov)),
-                               float(weight_decay), _coefficients(coefficients, steps), steps, float(eps), ws, need, _stream(dev)), 'sgpo_muon_step')
+    rc = lib.sgpo_muon_step(weight.data_ptr(), wd, g.data_ptr(), gd, momentum_buffer.data_ptr(), batch, m, n, lr, momentum, bool(nesterov), weight_decay,
+                            table, steps, eps, ws, need, _stream(dev))
+    if rc:
+        L.check(rc, 'sgpo_muon_step')
+    torch.autograd.graph.increment_version((weight, momentum_buffer))     # what autograd saved of them is stale now
     return weight

@@ -545,7 +545,7 @@ def test_a_training_step_of_a_small_denoiser():
     want = body(p64, rot64, lambda h, w: torch.nn.functional.cross_entropy((h @ w.T + bias.double().cpu()).view(-1, V), tc.view(-1), ignore_index=-100))
     want.backward()
     # a chain of five fp32 products of up to 128 terms forward and as many back: 2 * 5 * 128 u = 2^-13.7 of a gradient's norm
-    assert abs(float(loss) - float(want)) <= 2.0 ** -14 * float(want)
+    assert abs(float(loss.detach()) - float(want.detach())) <= 2.0 ** -14 * float(want.detach())
     for k, v in leaves.items():
         d = v.grad.double().cpu() - p64[k].grad
         assert float(d.norm()) <= 2.0 ** -13 * float(p64[k].grad.norm()), k
