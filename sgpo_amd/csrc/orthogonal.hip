@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr int PARTS = 64;   // partial sums of a matrix's squared norm
+constexpr int PARTS = 512;   // partial sums of a matrix's squared norm: at most, and a multiple of 64
 
 __host__ __device__ inline int64_t round_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
@@ -46,8 +46,8 @@ __global__ __launch_bounds__(256) void square_kernel(Source s, double* part) {
   const int b = blockIdx.y;
   const int64_t total = (int64_t)s.rows * s.cols;
   double sum = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)PARTS * 256) {
-    const int r = (int)(i / s.cols), c = (int)(i - (int64_t)r * s.cols);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int r = (int)((uint32_t)i / (uint32_t)s.cols), c = (int)((uint32_t)i - (uint32_t)r * (uint32_t)s.cols);
     if (s.buf) {
       float* m = s.buf + (int64_t)b * total + i;
       *m = fmaf(s.momentum, *m, up<T>(reinterpret_cast<const T*>(s.grad)[b * s.stride_b + r * s.ld + c]));
@@ -63,8 +63,9 @@ __global__ __launch_bounds__(256) void square_kernel(Source s, double* part) {
   if (threadIdx.x == 0) part[b * PARTS + blockIdx.x] = share[0] + share[1] + share[2] + share[3];
 }
 
-__device__ __forceinline__ float inverse_norm(const double* part, double eps) {   // every lane of the wave calls it
-  double s = part[threadIdx.x & 63];
+__device__ __forceinline__ float inverse_norm(const double* part, int parts, double eps) {   // every lane of the wave calls it
+  double s = 0.0;
+  for (int i = threadIdx.x & 63; i < parts; i += 64) s += part[i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   return (float)(1.0 / (sqrt(s) + eps));
@@ -72,10 +73,10 @@ __device__ __forceinline__ float inverse_norm(const double* part, double eps) { 
 
 // X [m][n] planes of the scaled update, zero in the padding columns; TALL: X is the update transposed
 template <typename T, bool TALL>
-__global__ __launch_bounds__(256) void load_kernel(Source s, const double* part, double eps, bf16_t* X, int m, int n, int64_t ldx, int64_t bstride) {
+__global__ __launch_bounds__(256) void load_kernel(Source s, const double* part, int parts, double eps, bf16_t* X, int m, int n, int64_t ldx, int64_t bstride) {
   __shared__ float tile[64][65];
   const int b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  const float inv = inverse_norm(part + b * PARTS, eps);
+  const float inv = inverse_norm(part + b * PARTS, parts, eps);
   if constexpr (TALL) {
     for (int i = threadIdx.x; i < 64 * 64; i += 256) {
       const int c = i >> 6, r = i & 63;   // along the update's rows
@@ -99,6 +100,14 @@ struct Mats {
   int m, n;
 };
 
+// Workgroup -> (matrix, tile): workgroups with equal id % 8 share an XCD and its L2, and each XCD takes one contiguous run of the list of all
+// matrices' tiles, so that a matrix is read into few L2s (512 x 2048, eight of them: each XCD its own matrix).
+__device__ __forceinline__ void contiguous(int id, int total, int per, int& b, int& t) {
+  const int q = total >> 3, r = total & 7, x = id & 7;
+  t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
+  b = t / per;
+  t -= b * per;
+}
 // tile (i, j), i <= j, of the triangle, row by row
 __device__ __forceinline__ void triangle(int t, int tiles, int& i, int& j) {
   i = 0;
@@ -111,9 +120,10 @@ template <class S, bool POLY>
 __global__ __launch_bounds__(S::THREADS, 2) void symmetric_kernel(Mats q, int tiles, float cb, float cc) {
   static_assert(S::BM == S::BN && S::PL == 2, "square tiles of two planes");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  int i, j;
-  triangle(blockIdx.x, tiles, i, j);
-  const int b = blockIdx.y, m0 = i * S::BM, n0 = j * S::BN;
+  int i, j, b, t;
+  contiguous(blockIdx.x, gridDim.x, tiles * (tiles + 1) / 2, b, t);
+  triangle(t, tiles, i, j);
+  const int m0 = i * S::BM, n0 = j * S::BN;
   const bf16_t* src = POLY ? q.G + b * q.sg : q.X + b * q.sx;
   const int64_t ld = POLY ? q.ldg : q.ldx;
   tg::Operand o{src, ld, q.m, 0};
@@ -164,13 +174,170 @@ struct Result {
   float keep, rate;
 };
 
+__device__ __forceinline__ void store_result(const Result& r, int b, int m, int n, float v) {   // element (m, n) of X
+  const int64_t at = (int64_t)b * r.rows * r.cols + (r.tall ? (int64_t)n * r.cols + m : (int64_t)m * r.cols + n);
+  if (r.out_bf16) {
+    bf16_t* o = reinterpret_cast<bf16_t*>(r.out) + at;
+    *o = f2bf(r.step ? fmaf(-r.rate, v, r.keep * bf2f(*o)) : v);
+  } else {
+    float* o = reinterpret_cast<float*>(r.out) + at;
+    *o = fmaf(-r.rate, v, r.keep * *o);
+  }
+}
+
+// Matrices of at most 128 x 128: everything in one launch, one workgroup per matrix.  X stays in registers in fp32 (the layout of the products'
+// results); its planes, and those of G and then P, pass through LDS.  One LDS image serves both as rows (X X^T, G G, P .) and, by
+// transposed reads, as columns (. X): rows of 2 * E planes elements, their 16-B chunks permuted by a function of the row that
+// keeps both kinds of read off each other's banks.  Bound by the chain of 3 dependent products per triple, each a few LDS round trips.
+template <int E>
+struct Small {
+  static constexpr int WAVES_M = 2, WAVES_N = E == 128 ? 4 : 2, THREADS = 64 * WAVES_M * WAVES_N;
+  static constexpr int MT = E / WAVES_M / 16, NT = E / WAVES_N / 16;
+  static constexpr int ROWB = E * 4, IMAGE = E * ROWB, LDS = 2 * IMAGE;
+  typedef f32x4 Acc[MT][NT];
+  __device__ static __forceinline__ int swz(int row) { return ((row & 1) << 1) | ((row & 2) << 1) | ((row & 8)) | ((row >> 2) & 1); }
+  // byte of element (row, e) of plane 0; its 16-B chunk holds e .. e + 7 of one plane, plane 1 is 4 chunks on
+  __device__ static __forceinline__ int at(int row, int e, int plane) { return row * ROWB + ((((e >> 5) * 8 + plane * 4 + ((e >> 3) & 3)) ^ swz(row)) << 4) + (e & 7) * 2; }
+  __device__ static __forceinline__ bf16x8 row_fragment(const char* img, int row, int slice, int plane, int l4) {
+    return *reinterpret_cast<const bf16x8*>(img + at(row, slice * 32 + l4 * 8, plane));
+  }
+  __device__ static __forceinline__ bf16x8 col_fragment(const char* img, int col16, int slice, int plane, int l16, int l4) {
+    const int row = slice * 32 + l4 * 8 + (l16 >> 2), e = col16 * 16 + (l16 & 3) * 4;
+    const tg::s16x4 lo = tg::read_tr((tg::lds_tr_t)(img + at(row, e, plane)));
+    const tg::s16x4 hi = tg::read_tr((tg::lds_tr_t)(img + at(row + 4, e, plane)));
+    const tg::s16x8 v = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    return *reinterpret_cast<const bf16x8*>(&v);
+  }
+  // r = A B^T (COLS false: both images by rows) or A B (B by columns), k < 32 * slices
+  template <bool COLS>
+  __device__ static __forceinline__ void product(const char* A, const char* B, int slices, Acc& r, int wm, int wn, int l16, int l4) {
+#pragma unroll
+    for (int x = 0; x < MT; ++x)
+#pragma unroll
+      for (int y = 0; y < NT; ++y) r[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < slices; ++s) {
+      bf16x8 a[2][MT], b[2][NT];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+#pragma unroll
+        for (int x = 0; x < MT; ++x) a[p][x] = row_fragment(A, (wm * MT + x) * 16 + l16, s, p, l4);
+#pragma unroll
+        for (int y = 0; y < NT; ++y) b[p][y] = COLS ? col_fragment(B, wn * NT + y, s, p, l16, l4) : row_fragment(B, (wn * NT + y) * 16 + l16, s, p, l4);
+      }
+#pragma unroll
+      for (int k = 2; k >= 0; --k)   // the two mixed pairs, then the high one
+#pragma unroll
+        for (int x = 0; x < MT; ++x)
+#pragma unroll
+          for (int y = 0; y < NT; ++y) r[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[k == 1][y], a[k == 2][x], r[x][y], 0, 0, 0);
+    }
+  }
+  __device__ static __forceinline__ void put(char* img, const Acc& v, int wm, int wn, int l16, int l4) {
+#pragma unroll
+    for (int x = 0; x < MT; ++x)
+#pragma unroll
+      for (int y = 0; y < NT; ++y) {
+        const int row = (wm * MT + x) * 16 + l16, e = (wn * NT + y) * 16 + 4 * l4;
+        float pl[4][2];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tg::split<2>(v[x][y][q], pl[q]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          *reinterpret_cast<uint2*>(img + at(row, e, p)) = make_uint2(pack_bf16x2(pl[0][p], pl[1][p]), pack_bf16x2(pl[2][p], pl[3][p]));
+      }
+  }
+};
+
+struct Table { float v[3 * 64]; };
+
+template <typename T, int E>
+__global__ __launch_bounds__(Small<E>::THREADS, 1) void small_kernel(Source s, int m, int n, Table coef, int steps, double eps, Result res) {
+  typedef Small<E> K;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ double share[K::THREADS / 64];
+  char *X = smem, *G = smem + K::IMAGE;
+  const int b = blockIdx.x, lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave / K::WAVES_N, wn = wave % K::WAVES_N;
+  typename K::Acc x, g, h;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < K::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < K::NT; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int mm = (wm * K::MT + i) * 16 + l16, nn = (wn * K::NT + j) * 16 + 4 * l4 + q;
+        float u = 0.f;
+        if (mm < m && nn < n) {
+          const int r = res.tall ? nn : mm, c = res.tall ? mm : nn;
+          if (s.buf) {
+            float* at = s.buf + ((int64_t)b * s.rows + r) * s.cols + c;
+            *at = fmaf(s.momentum, *at, up<T>(reinterpret_cast<const T*>(s.grad)[b * s.stride_b + r * s.ld + c]));
+          }
+          u = update_at<T>(s, b, r, c);
+        }
+        x[i][j][q] = u;
+        sum += (double)u * u;
+      }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) share[wave] = sum;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < K::THREADS / 64; ++w) sum += share[w];
+  const float inv = (float)(1.0 / (sqrt(sum) + eps));
+#pragma unroll
+  for (int i = 0; i < K::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < K::NT; ++j) x[i][j] *= inv;
+  const int sm = (m + 31) >> 5, sn = (n + 31) >> 5;   // k slices
+  for (int k = 0; k < steps; ++k) {
+    const float ca = coef.v[3 * k], cb = coef.v[3 * k + 1], cc = coef.v[3 * k + 2];
+    K::put(X, x, wm, wn, l16, l4);
+    __syncthreads();
+    K::template product<false>(X, X, sn, g, wm, wn, l16, l4);
+    K::put(G, g, wm, wn, l16, l4);
+    __syncthreads();
+    K::template product<false>(G, G, sm, h, wm, wn, l16, l4);
+#pragma unroll
+    for (int i = 0; i < K::MT; ++i)
+#pragma unroll
+      for (int j = 0; j < K::NT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) h[i][j][q] = fmaf(cb, g[i][j][q], cc * h[i][j][q]);
+    __syncthreads();
+    K::put(G, h, wm, wn, l16, l4);
+    __syncthreads();
+    K::template product<true>(G, X, sm, g, wm, wn, l16, l4);
+#pragma unroll
+    for (int i = 0; i < K::MT; ++i)
+#pragma unroll
+      for (int j = 0; j < K::NT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[i][j][q] = fmaf(ca, x[i][j][q], g[i][j][q]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < K::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < K::NT; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int mm = (wm * K::MT + i) * 16 + l16, nn = (wn * K::NT + j) * 16 + 4 * l4 + q;
+        if (mm < m && nn < n) store_result(res, b, mm, nn, x[i][j][q]);
+      }
+}
+
 // Y = a X + P X;  LAST: into the result instead
 template <class S, bool LAST>
 __global__ __launch_bounds__(S::THREADS, 2) void apply_kernel(Mats q, int tm, int tn, float ca, Result res) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  int im, in;
-  tg::tile_of(blockIdx.x, tm, tn, im, in);
-  const int b = blockIdx.y, m0 = im * S::BM, n0 = in * S::BN;
+  int b, t;
+  contiguous(blockIdx.x, gridDim.x, tm * tn, b, t);
+  const int band = 8 * tn, first = t / band * 8, h = min(8, tm - first);   // bands of 8 row tiles
+  const int im = first + t % band % h, in = t % band / h;
+  const int m0 = im * S::BM, n0 = in * S::BN;
   const bf16_t* X = q.X + b * q.sx;
   f32x4 acc[S::MT][S::NT];
   tg::clear<S>(acc);
@@ -193,17 +360,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void apply_kernel(Mats q, int tm, in
         tg::store4<2>(q.Y + b * q.sx + m * q.ldx, n, v);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (n + e >= q.n) continue;
-          const int64_t at = (int64_t)b * res.rows * res.cols + (res.tall ? (int64_t)(n + e) * res.cols + m : (int64_t)m * res.cols + n + e);
-          if (res.out_bf16) {
-            bf16_t* o = reinterpret_cast<bf16_t*>(res.out) + at;
-            *o = f2bf(res.step ? fmaf(-res.rate, v[e], res.keep * bf2f(*o)) : v[e]);
-          } else {
-            float* o = reinterpret_cast<float*>(res.out) + at;
-            *o = fmaf(-res.rate, v[e], res.keep * *o);
-          }
-        }
+        for (int e = 0; e < 4; ++e) if (n + e < q.n) store_result(res, b, m, n + e, v[e]);
       }
     }
   }
@@ -228,14 +385,14 @@ template <class S, bool POLY>
 int symmetric(const Mats& q, int batch, float cb, float cc, hipStream_t st) {
   const int t = (q.m + S::BM - 1) / S::BM;
   ALLOW((symmetric_kernel<S, POLY>), S::LDS);
-  hipLaunchKernelGGL((symmetric_kernel<S, POLY>), dim3((unsigned)(t * (t + 1) / 2), batch), dim3(S::THREADS), S::LDS, st, q, t, cb, cc);
+  hipLaunchKernelGGL((symmetric_kernel<S, POLY>), dim3((unsigned)(t * (t + 1) / 2) * batch), dim3(S::THREADS), S::LDS, st, q, t, cb, cc);
   return SGPO_OK;
 }
 template <class S, bool LAST>
 int apply(const Mats& q, int batch, float ca, const Result& r, hipStream_t st) {
   const int tm = (q.m + S::BM - 1) / S::BM, tn = (q.n + S::BN - 1) / S::BN;
   ALLOW((apply_kernel<S, LAST>), S::LDS);
-  hipLaunchKernelGGL((apply_kernel<S, LAST>), dim3((unsigned)tm * tn, batch), dim3(S::THREADS), S::LDS, st, q, tm, tn, ca, r);
+  hipLaunchKernelGGL((apply_kernel<S, LAST>), dim3((unsigned)tm * tn * batch), dim3(S::THREADS), S::LDS, st, q, tm, tn, ca, r);
   return SGPO_OK;
 }
 
@@ -265,16 +422,32 @@ Sizes sizes(int batch, int rows, int cols) {
   return s;
 }
 
+template <typename T, int E>
+int orthogonalise_small(const Source& src, int batch, const float* coef, int steps, double eps, const Result& res, hipStream_t st) {
+  Table t = {};
+  for (int i = 0; i < 3 * steps; ++i) t.v[i] = coef[i];
+  ALLOW((small_kernel<T, E>), Small<E>::LDS);
+  hipLaunchKernelGGL((small_kernel<T, E>), dim3(batch), dim3(Small<E>::THREADS), Small<E>::LDS, st, src, src.rows < src.cols ? src.rows : src.cols,
+                     src.rows < src.cols ? src.cols : src.rows, t, steps, eps, res);
+  SGPO_CHECK_HIP(hipGetLastError());
+  return SGPO_OK;
+}
+
 template <typename T>
 int orthogonalise(const Source& src, int batch, const float* coef, int steps, double eps, Result res, char* ws, hipStream_t st) {
   const Sizes z = sizes(batch, src.rows, src.cols);
   double* part = reinterpret_cast<double*>(ws);
   Mats q{(bf16_t*)(ws + z.off_x), (bf16_t*)(ws + z.off_y), (bf16_t*)(ws + z.off_g), (bf16_t*)(ws + z.off_p), z.ldx, z.ldg, (int64_t)z.x, (int64_t)z.g, z.m, z.n};
   res.tall = src.rows > src.cols; res.rows = src.rows; res.cols = src.cols;
-  hipLaunchKernelGGL((square_kernel<T>), dim3(PARTS, batch), dim3(256), 0, st, src, part);
+  if (z.n <= 64) return orthogonalise_small<T, 64>(src, batch, coef, steps, eps, res, st);
+  if (z.n <= 128) return orthogonalise_small<T, 128>(src, batch, coef, steps, eps, res, st);
+  // about 16 elements a thread
+  const int64_t want = ((int64_t)src.rows * src.cols + 4095) / 4096;
+  const int parts = want < PARTS ? (int)want : PARTS;
+  hipLaunchKernelGGL((square_kernel<T>), dim3(parts, batch), dim3(256), 0, st, src, part);
   const dim3 grid((unsigned)((z.ldx / 2 + 63) / 64), (unsigned)((z.m + 63) / 64), batch);
-  if (res.tall) hipLaunchKernelGGL((load_kernel<T, true>), grid, dim3(256), 0, st, src, part, eps, q.X, z.m, z.n, z.ldx, (int64_t)z.x);
-  else hipLaunchKernelGGL((load_kernel<T, false>), grid, dim3(256), 0, st, src, part, eps, q.X, z.m, z.n, z.ldx, (int64_t)z.x);
+  if (res.tall) hipLaunchKernelGGL((load_kernel<T, true>), grid, dim3(256), 0, st, src, part, parts, eps, q.X, z.m, z.n, z.ldx, (int64_t)z.x);
+  else hipLaunchKernelGGL((load_kernel<T, false>), grid, dim3(256), 0, st, src, part, parts, eps, q.X, z.m, z.n, z.ldx, (int64_t)z.x);
   const int cs = pick_symmetric(z.m, batch), cf = pick_full(z.m, z.n, batch);
   for (int k = 0; k < steps; ++k) {
     const float a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
@@ -293,7 +466,8 @@ int orthogonalise(const Source& src, int batch, const float* coef, int steps, do
 
 int check_sizes(int batch, int rows, int cols, int steps, const float* coef) {
   SGPO_REQUIRE(batch >= 0 && rows >= 0 && cols >= 0, "newton_schulz: negative size");
-  SGPO_REQUIRE(batch <= 65535 && rows <= (1 << 17) && cols <= (1 << 17), "newton_schulz: %d matrices of %d x %d over the supported range", batch, rows, cols);
+  SGPO_REQUIRE(batch <= 65535 && (int64_t)rows * cols <= 0x7fffffff && (int64_t)batch * rows * cols <= ((int64_t)1 << 40), "newton_schulz: %d matrices of %d x %d over the supported range",
+               batch, rows, cols);
   SGPO_REQUIRE(steps >= 1 && steps <= 64 && coef, "newton_schulz: 1 to 64 coefficient triples are needed, got %d", steps);
   return SGPO_OK;
 }

@@ -138,11 +138,13 @@ int launch(Args& p, int heads, hipStream_t st) {
   p.units = INTER && VEC > 1 ? p.D / VEC : half / VEC + (p.D - p.rot) / VEC;
   p.by_units = fast_div(p.units);
   p.by_heads = fast_div(heads);
-  // tokens per workgroup: about 16 units per thread, the table within 32 KiB, and no fewer workgroups than four per CU
-  int64_t t = 4096 / ((int64_t)heads * p.units);
-  const int64_t fit = half ? 4096 / half : 64, spread = p.tokens / 1024;
+  // Tokens per workgroup: about two units per thread, so that a CU's workgroups overlap one's angles with another's copying (30464 tokens
+  // of 16 bf16 heads of 64: 24.5 us with 8 tokens, 29.5 with 64; 41 with one, where too few units share a token's angles), but at most
+  // 65536 workgroups, whose dispatch takes longer than their work (131072 tokens of 40 heads of 128: 498 us with one token, 456 with two).
+  const int64_t per_token = (int64_t)heads * p.units, fit = half ? 4096 / half : 4096, fewest = (p.tokens + 65535) / 65536;
+  int64_t t = (512 + per_token - 1) / per_token;
+  if (t < fewest) t = fewest;
   if (t > fit) t = fit;
-  if (t > spread) t = spread;
   if (t < 1) t = 1;
   p.per_block = (int)t;
   const int64_t grid = (p.tokens + t - 1) / t;

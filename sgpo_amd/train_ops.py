@@ -52,8 +52,16 @@ def _on_device(first, *others):
     return dev
 
 
-def _stream(dev):
-    return torch._C._cuda_getCurrentRawStream(dev.index)     # torch.cuda.current_stream(dev).cuda_stream without the object
+def _call(dev, name, *args):
+    """One C call on the stream that is current on the tensors' device, which need not be the current device."""
+    fn = getattr(L.load(), name)
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))    # torch.cuda.current_stream(dev).cuda_stream without the object
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        L.check(rc, name)
 
 
 def _scratch(nbytes, dev):
@@ -139,9 +147,7 @@ def _rotate(q, k, frequencies, positions, interleaved, scale, inverse, in_place=
         kp, kop, ks, kos = k.data_ptr(), ko.data_ptr(), k.stride()[:3], ko.stride()[:3]
     args = _ROTARY.pack(q.data_ptr(), qo.data_ptr(), kp, kop, *q.stride()[:3], *qo.stride()[:3], *ks, *kos, pos, psb, psl, frequencies.data_ptr(),
                         B, Lq, Hq, Hk, D, rot, interleaved, inverse, dt, scale)
-    rc = L.load().sgpo_rotary(args, _stream(dev))
-    if rc:
-        L.check(rc, 'sgpo_rotary')
+    _call(dev, 'sgpo_rotary', args)
     return qo, ko
 
 
@@ -197,18 +203,15 @@ def _rows(t):
 def _loss_forward(hidden, weight, targets, bias, ignore_index, reduction):
     """(loss or losses, state for the backward pass: the tokens' log-sums, the gradient's factor, and losses that are only summed)."""
     dev = hidden.device
-    lib = L.load()
     N = hidden.shape[0]
     args = _loss_args(hidden, weight, targets, bias, ignore_index, reduction)
-    need = lib.sgpo_linear_ce_workspace_bytes(args, 0)
+    need = L.load().sgpo_linear_ce_workspace_bytes(args, 0)
     buf, ws = _scratch(need, dev)
     state = torch.empty(2 * N + 1 if reduction else N + 1, dtype=torch.float32, device=dev)
     out = torch.empty((N,) if reduction == 0 else (), dtype=torch.float32, device=dev)
     lse = state.data_ptr()
     inv, o = lse + 4 * N, out.data_ptr()
-    rc = lib.sgpo_linear_ce_forward(args, inv + 4 if reduction else o, lse, o, inv, ws, need, _stream(dev))
-    if rc:
-        L.check(rc, 'sgpo_linear_ce_forward')
+    _call(dev, 'sgpo_linear_ce_forward', args, inv + 4 if reduction else o, lse, o, inv, ws, need)
     return out, state
 
 
@@ -225,20 +228,17 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def backward(ctx, grad):
         hidden, weight, targets, bias, state = ctx.saved_tensors
         dev = hidden.device
-        lib = L.load()
         args = _loss_args(hidden, weight, targets, bias, *ctx.how)
         grad = grad.contiguous()
         want = ctx.needs_input_grad
         dh = hidden.new_empty(hidden.shape) if want[0] else None
         dw = weight.new_empty(weight.shape) if want[1] else None
         db = bias.new_empty(bias.shape) if want[3] else None
-        need = lib.sgpo_linear_ce_workspace_bytes(args, 1)
+        need = L.load().sgpo_linear_ce_workspace_bytes(args, 1)
         buf, ws = _scratch(need, dev)
         lse = state.data_ptr()
-        rc = lib.sgpo_linear_ce_backward(args, lse, grad.data_ptr(), lse + 4 * hidden.shape[0], None if dh is None else dh.data_ptr(),
-                                         None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), ws, need, _stream(dev))
-        if rc:
-            L.check(rc, 'sgpo_linear_ce_backward')
+        _call(dev, 'sgpo_linear_ce_backward', args, lse, grad.data_ptr(), lse + 4 * hidden.shape[0], None if dh is None else dh.data_ptr(),
+              None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), ws, need)
         return dh, dw, None, db, None, None
 
 
@@ -315,12 +315,9 @@ def newton_schulz(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
     if u.stride(-1) != 1 and n > 1 or m > 1 and ld < n:
         u = u.contiguous()
         sb, ld = m * n, n
-    lib = L.load()
-    need = lib.sgpo_newton_schulz_workspace_bytes(batch, m, n)
+    need = L.load().sgpo_newton_schulz_workspace_bytes(batch, m, n)
     buf, ws = _scratch(need, dev)
-    rc = lib.sgpo_newton_schulz(u.data_ptr(), dt, batch, m, n, sb, ld, table, steps, eps, out.data_ptr(), ws, need, _stream(dev))
-    if rc:
-        L.check(rc, 'sgpo_newton_schulz')
+    _call(dev, 'sgpo_newton_schulz', u.data_ptr(), dt, batch, m, n, sb, ld, table, steps, eps, out.data_ptr(), ws, need)
     return out
 
 
@@ -348,12 +345,9 @@ def muon_step(weight, grad, momentum_buffer, lr, momentum=0.95, nesterov=True, w
     g = grad.detach().contiguous()
     m, n = weight.shape[-2:]
     batch = weight.numel() // (m * n)
-    lib = L.load()
-    need = lib.sgpo_newton_schulz_workspace_bytes(batch, m, n)
+    need = L.load().sgpo_newton_schulz_workspace_bytes(batch, m, n)
     buf, ws = _scratch(need, dev)
-    rc = lib.sgpo_muon_step(weight.data_ptr(), wd, g.data_ptr(), gd, momentum_buffer.data_ptr(), batch, m, n, lr, momentum, bool(nesterov), weight_decay,
-                            table, steps, eps, ws, need, _stream(dev))
-    if rc:
-        L.check(rc, 'sgpo_muon_step')
+    _call(dev, 'sgpo_muon_step', weight.data_ptr(), wd, g.data_ptr(), gd, momentum_buffer.data_ptr(), batch, m, n, lr, momentum, bool(nesterov), weight_decay,
+                            table, steps, eps, ws, need)
     torch.autograd.graph.increment_version((weight, momentum_buffer))     # what autograd saved of them is stale now
     return weight
