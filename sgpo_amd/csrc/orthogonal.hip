@@ -1,7 +1,8 @@
 // Orthogonalised updates by Newton-Schulz products, and the optimiser step around them.
 //
-//   X_0 = U / (|U|_F + eps)          (U transposed where it has more rows than columns, so that X is m x n with m <= n)
-//   G = X X^T,  P = b G + c G G,  X <- a X + P X          once per coefficient triple (a, b, c)
+//   X_0 = U / (|U|_F + eps)
+//   G = X X^T,  P = a I + b G + c G G,  X <- P X          once per coefficient triple (a, b, c)
+//   (G = X^T X and X <- X P where X has more rows than columns: the products' operands are read by rows or by columns as stored, nothing is transposed)
 // which moves every singular value of X towards 1 by the odd polynomial a s + b s^3 + c s^5 and leaves the singular vectors.
 //   step:  buf <- mu buf + grad,  U = grad + mu buf (or buf),  W <- (1 - lr wd) W - lr sqrt(max(1, rows / cols)) X
 //
@@ -71,33 +72,25 @@ __device__ __forceinline__ float inverse_norm(const double* part, int parts, dou
   return (float)(1.0 / (sqrt(s) + eps));
 }
 
-// X [m][n] planes of the scaled update, zero in the padding columns; TALL: X is the update transposed
-template <typename T, bool TALL>
-__global__ __launch_bounds__(256) void load_kernel(Source s, const double* part, int parts, double eps, bf16_t* X, int m, int n, int64_t ldx, int64_t bstride) {
-  __shared__ float tile[64][65];
-  const int b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+// X planes of the scaled update, zero in the padding columns
+template <typename T>
+__global__ __launch_bounds__(256) void load_kernel(Source s, const double* part, int parts, double eps, bf16_t* X, int64_t ldx, int64_t bstride) {
+  const int b = blockIdx.y;
   const float inv = inverse_norm(part + b * PARTS, parts, eps);
-  if constexpr (TALL) {
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-      const int c = i >> 6, r = i & 63;   // along the update's rows
-      if (r0 + r < m && c0 + c < n) tile[r][c] = update_at<T>(s, b, c0 + c, r0 + r);
-    }
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-    const int r = r0 + (i >> 4), c = c0 + (i & 15) * 4;
-    if (r >= m || c >= ldx / 2) continue;
+  const uint32_t quads = (uint32_t)(ldx / 8), total = (uint32_t)s.rows * quads;
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
+    const int r = (int)(i / quads), c = (int)(i - (uint32_t)r * quads) * 4;
     float v[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = c + q < n ? inv * (TALL ? tile[r - r0][c - c0 + q] : update_at<T>(s, b, r, c + q)) : 0.f;
+    for (int q = 0; q < 4; ++q) v[q] = c + q < s.cols ? inv * update_at<T>(s, b, r, c + q) : 0.f;
     tg::store4<2>(X + b * bstride + r * ldx, c, v);
   }
 }
 
 struct Mats {
-  bf16_t *X, *Y, *G, *P;   // planes
+  bf16_t *X, *Y, *G, *P;      // planes: X, Y [rows][cols], G, P [d][d], d the shorter side
   int64_t ldx, ldg, sx, sg;   // row pitch and batch stride, stored elements
-  int m, n;
+  int rows, cols, d;
 };
 
 // Workgroup -> (matrix, tile): workgroups with equal id % 8 share an XCD and its L2, and each XCD takes one contiguous run of the list of all
@@ -115,48 +108,54 @@ __device__ __forceinline__ void triangle(int t, int tiles, int& i, int& j) {
   j = i + t;
 }
 
-// G = X X^T (POLY false)  or  P = b G + c G G (POLY true): one triangle of tiles, each also written transposed
-template <class S, bool POLY>
-__global__ __launch_bounds__(S::THREADS, 2) void symmetric_kernel(Mats q, int tiles, float cb, float cc) {
+enum { WIDE = 0, TALL = 1, POLY = 2 };   // G = X X^T;  G = X^T X;  P = a I + b G + c G G
+
+// one triangle of tiles, each also written transposed
+template <class S, int MODE>
+__global__ __launch_bounds__(S::WG_THREADS, 2) void symmetric_kernel(Mats q, int tiles, float ca, float cb, float cc) {
   static_assert(S::BM == S::BN && S::PL == 2, "square tiles of two planes");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int i, j, b, t;
   contiguous(blockIdx.x, gridDim.x, tiles * (tiles + 1) / 2, b, t);
   triangle(t, tiles, i, j);
   const int m0 = i * S::BM, n0 = j * S::BN;
-  const bf16_t* src = POLY ? q.G + b * q.sg : q.X + b * q.sx;
-  const int64_t ld = POLY ? q.ldg : q.ldx;
-  tg::Operand o{src, ld, q.m, 0};
+  const bf16_t* G = q.G + b * q.sg;
   f32x4 acc[S::MT][S::NT];
   tg::clear<S>(acc);
-  tg::run<S, tg::KC, tg::KC>(o, o, m0, n0, 0, (int)(ld / 64), smem, acc);
-  bf16_t* dst = (POLY ? q.P : q.G) + b * q.sg;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
-  const int wave = (int)threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+  if constexpr (MODE == TALL) {
+    const tg::Operand o{q.X + b * q.sx, q.ldx, q.rows, (int)q.ldx};
+    tg::run<S, tg::KM, tg::KM>(o, o, m0, n0, 0, (q.rows + 31) / 32, smem, acc);
+  } else {
+    const tg::Operand o{MODE == POLY ? G : q.X + b * q.sx, MODE == POLY ? q.ldg : q.ldx, q.d, 0};
+    tg::run<S, tg::KC, tg::KC>(o, o, m0, n0, 0, (int)(o.ld / 64), smem, acc);
+  }
+  bf16_t* dst = (MODE == POLY ? q.P : q.G) + b * q.sg;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4, wm = S::wave() / S::WN, wn = S::wave() % S::WN;
 #pragma unroll
   for (int x = 0; x < S::MT; ++x) {
     const int m = m0 + (wm * S::MT + x) * 16 + l16;
 #pragma unroll
     for (int y = 0; y < S::NT; ++y) {
+      if (!S::owns(x, y)) continue;
       const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4;
       float v[4] = {acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]};
-      if (m < q.m && n < q.ldg / 2) {
-        if constexpr (POLY) {
+      if (m < q.d && n < q.ldg / 2) {
+        if constexpr (MODE == POLY) {
           float g[4];
-          tg::load4<2>(q.G + b * q.sg + m * q.ldg, n, g);
+          tg::load4<2>(G + m * q.ldg, n, g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(cb, g[e], cc * v[e]);
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(cb, g[e], cc * v[e]) + (m == n + e ? ca : 0.f);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (n + e >= q.m) v[e] = 0.f;
+        for (int e = 0; e < 4; ++e) if (n + e >= q.d) v[e] = 0.f;
         tg::store4<2>(dst + m * q.ldg, n, v);
       }
       if (i != j && m < q.ldg / 2) {   // the mirror image: row n + e, column m
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (n + e < q.m) {
+          if (n + e < q.d) {
             float pl[2];
-            tg::split<2>(m < q.m ? v[e] : 0.f, pl);
+            tg::split<2>(m < q.d ? v[e] : 0.f, pl);
             bf16_t* at = dst + (n + e) * q.ldg + (m >> 5) * 64 + (m & 31);
             at[0] = f2bf(pl[0]);
             at[32] = f2bf(pl[1]);
@@ -169,19 +168,36 @@ __global__ __launch_bounds__(S::THREADS, 2) void symmetric_kernel(Mats q, int ti
 struct Result {
   void* out;               // bf16 [batch][rows][cols], or the weight
   int out_bf16;
-  int tall, rows, cols;
+  int rows, cols;
   int step;                // 0: out = X;  1: out = keep * out - rate * X
+  int vec;                 // rows start aligned to four elements
   float keep, rate;
 };
 
-__device__ __forceinline__ void store_result(const Result& r, int b, int m, int n, float v) {   // element (m, n) of X
-  const int64_t at = (int64_t)b * r.rows * r.cols + (r.tall ? (int64_t)n * r.cols + m : (int64_t)m * r.cols + n);
+__device__ __forceinline__ float result(const Result& r, float old, float v) { return r.step ? fmaf(-r.rate, v, r.keep * old) : v; }
+// elements (m, n .. n + 3) of X, those that exist
+__device__ __forceinline__ void store_result(const Result& r, int b, int m, int n, const float (&v)[4]) {
+  const int64_t at = ((int64_t)b * r.rows + m) * r.cols + n;
   if (r.out_bf16) {
     bf16_t* o = reinterpret_cast<bf16_t*>(r.out) + at;
-    *o = f2bf(r.step ? fmaf(-r.rate, v, r.keep * bf2f(*o)) : v);
-  } else {
+    if (r.vec && n + 4 <= r.cols) {
+      uint2 w = make_uint2(0, 0);
+      if (r.step) w = *reinterpret_cast<const uint2*>(o);
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(result(r, bf2f(w.x & 0xffff), v[0]), result(r, bf2f(w.x >> 16), v[1])),
+                                                pack_bf16x2(result(r, bf2f(w.y & 0xffff), v[2]), result(r, bf2f(w.y >> 16), v[3])));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (n + e < r.cols) o[e] = f2bf(result(r, r.step ? bf2f(o[e]) : 0.f, v[e]));
+    }
+  } else {   // only a step writes fp32
     float* o = reinterpret_cast<float*>(r.out) + at;
-    *o = fmaf(-r.rate, v, r.keep * *o);
+    if (r.vec && n + 4 <= r.cols) {
+      const f32x4 w = *reinterpret_cast<const f32x4*>(o);
+      *reinterpret_cast<f32x4*>(o) = f32x4{result(r, w[0], v[0]), result(r, w[1], v[1]), result(r, w[2], v[2]), result(r, w[3], v[3])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (n + e < r.cols) o[e] = result(r, o[e], v[e]);
+    }
   }
 }
 
@@ -251,7 +267,7 @@ struct Small {
 struct Table { float v[3 * 64]; };
 
 template <typename T, int E>
-__global__ __launch_bounds__(Small<E>::THREADS, 1) void small_kernel(Source s, int m, int n, Table coef, int steps, double eps, Result res) {
+__global__ __launch_bounds__(Small<E>::THREADS, 1) void small_kernel(Source s, int m, int n, int tall, Table coef, int steps, double eps, Result res) {
   typedef Small<E> K;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ double share[K::THREADS / 64];
@@ -269,7 +285,7 @@ __global__ __launch_bounds__(Small<E>::THREADS, 1) void small_kernel(Source s, i
         const int mm = (wm * K::MT + i) * 16 + l16, nn = (wn * K::NT + j) * 16 + 4 * l4 + q;
         float u = 0.f;
         if (mm < m && nn < n) {
-          const int r = res.tall ? nn : mm, c = res.tall ? mm : nn;
+          const int r = tall ? nn : mm, c = tall ? mm : nn;
           if (s.buf) {
             float* at = s.buf + ((int64_t)b * s.rows + r) * s.cols + c;
             *at = fmaf(s.momentum, *at, up<T>(reinterpret_cast<const T*>(s.grad)[b * s.stride_b + r * s.ld + c]));
@@ -325,50 +341,55 @@ __global__ __launch_bounds__(Small<E>::THREADS, 1) void small_kernel(Source s, i
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int mm = (wm * K::MT + i) * 16 + l16, nn = (wn * K::NT + j) * 16 + 4 * l4 + q;
-        if (mm < m && nn < n) store_result(res, b, mm, nn, x[i][j][q]);
+        if (mm >= m || nn >= n) continue;
+        const int64_t at = ((int64_t)b * s.rows + (tall ? nn : mm)) * s.cols + (tall ? mm : nn);
+        if (res.out_bf16) {
+          bf16_t* o = reinterpret_cast<bf16_t*>(res.out) + at;
+          *o = f2bf(result(res, res.step ? bf2f(*o) : 0.f, x[i][j][q]));
+        } else {
+          float* o = reinterpret_cast<float*>(res.out) + at;
+          *o = result(res, *o, x[i][j][q]);
+        }
       }
 }
 
-// Y = a X + P X;  LAST: into the result instead
-template <class S, bool LAST>
-__global__ __launch_bounds__(S::THREADS, 2) void apply_kernel(Mats q, int tm, int tn, float ca, Result res) {
+// Y = P X, or X P if TALLX;  LAST: into the result instead
+template <class S, bool TALLX, bool LAST>
+__global__ __launch_bounds__(S::WG_THREADS, 2) void apply_kernel(Mats q, int tm, int tn, Result res) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int b, t;
   contiguous(blockIdx.x, gridDim.x, tm * tn, b, t);
   const int band = 8 * tn, first = t / band * 8, h = min(8, tm - first);   // bands of 8 row tiles
   const int im = first + t % band % h, in = t % band / h;
   const int m0 = im * S::BM, n0 = in * S::BN;
-  const bf16_t* X = q.X + b * q.sx;
+  const bf16_t *X = q.X + b * q.sx, *P = q.P + b * q.sg;
   f32x4 acc[S::MT][S::NT];
   tg::clear<S>(acc);
-  tg::run<S, tg::KC, tg::KM>(tg::Operand{q.P + b * q.sg, q.ldg, q.m, 0}, tg::Operand{X, q.ldx, q.m, (int)q.ldx}, m0, n0, 0, (int)(q.ldg / 64), smem, acc);
-  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
-  const int wave = (int)threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+  if constexpr (TALLX) tg::run<S, tg::KC, tg::KC>(tg::Operand{X, q.ldx, q.rows, 0}, tg::Operand{P, q.ldg, q.d, 0}, m0, n0, 0, (int)(q.ldg / 64), smem, acc);   // P is symmetric
+  else tg::run<S, tg::KC, tg::KM>(tg::Operand{P, q.ldg, q.d, 0}, tg::Operand{X, q.ldx, q.d, (int)q.ldx}, m0, n0, 0, (int)(q.ldg / 64), smem, acc);
+  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4, wm = S::wave() / S::WN, wn = S::wave() % S::WN;
 #pragma unroll
   for (int x = 0; x < S::MT; ++x) {
     const int m = m0 + (wm * S::MT + x) * 16 + l16;
-    if (m >= q.m) continue;
+    if (m >= q.rows) continue;
 #pragma unroll
     for (int y = 0; y < S::NT; ++y) {
+      if (!S::owns(x, y)) continue;
       const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4;
       if (n >= q.ldx / 2) continue;
       float v[4];
-      tg::load4<2>(X + m * q.ldx, n, v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = n + e < q.n ? fmaf(ca, v[e], acc[x][y][e]) : 0.f;
-      if constexpr (!LAST) {
-        tg::store4<2>(q.Y + b * q.sx + m * q.ldx, n, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) if (n + e < q.n) store_result(res, b, m, n + e, v[e]);
-      }
+      for (int e = 0; e < 4; ++e) v[e] = n + e < q.cols ? acc[x][y][e] : 0.f;
+      if constexpr (LAST) store_result(res, b, m, n, v);
+      else tg::store4<2>(q.Y + b * q.sx + m * q.ldx, n, v);
     }
   }
 }
 
 typedef tg::Shape<256, 256, 2, 4, 2, 2> ShapeL;
+typedef tg::Shape<192, 192, 2, 4, 2, 2> ShapeN;
 typedef tg::Shape<128, 128, 2, 2, 2, 2> ShapeM;
-typedef tg::Shape<64, 64, 2, 2, 2, 4> ShapeS;
+typedef tg::Shape<64, 64, 2, 2, 2, 2, 4> ShapeS;
 
 template <typename K>
 int allow_lds(K kernel, int bytes) {
@@ -381,38 +402,63 @@ int allow_lds(K kernel, int bytes) {
     if (!done) { const int rc_ = allow_lds(kernel, bytes); if (rc_) return rc_; done = true; } \
   } while (0)
 
-template <class S, bool POLY>
-int symmetric(const Mats& q, int batch, float cb, float cc, hipStream_t st) {
-  const int t = (q.m + S::BM - 1) / S::BM;
-  ALLOW((symmetric_kernel<S, POLY>), S::LDS);
-  hipLaunchKernelGGL((symmetric_kernel<S, POLY>), dim3((unsigned)(t * (t + 1) / 2) * batch), dim3(S::THREADS), S::LDS, st, q, t, cb, cc);
+template <class S, int MODE>
+int symmetric(const Mats& q, int batch, const float* coef, hipStream_t st) {
+  const int t = (q.d + S::BM - 1) / S::BM;
+  ALLOW((symmetric_kernel<S, MODE>), S::LDS);
+  hipLaunchKernelGGL((symmetric_kernel<S, MODE>), dim3((unsigned)(t * (t + 1) / 2) * batch), dim3(S::WG_THREADS), S::LDS, st, q, t, coef[0], coef[1], coef[2]);
   return SGPO_OK;
 }
-template <class S, bool LAST>
-int apply(const Mats& q, int batch, float ca, const Result& r, hipStream_t st) {
-  const int tm = (q.m + S::BM - 1) / S::BM, tn = (q.n + S::BN - 1) / S::BN;
-  ALLOW((apply_kernel<S, LAST>), S::LDS);
-  hipLaunchKernelGGL((apply_kernel<S, LAST>), dim3((unsigned)tm * tn * batch), dim3(S::THREADS), S::LDS, st, q, tm, tn, ca, r);
+template <class S, bool TALLX, bool LAST>
+int apply(const Mats& q, int batch, const Result& r, hipStream_t st) {
+  const int tm = (q.rows + S::BM - 1) / S::BM, tn = (q.cols + S::BN - 1) / S::BN;
+  ALLOW((apply_kernel<S, TALLX, LAST>), S::LDS);
+  hipLaunchKernelGGL((apply_kernel<S, TALLX, LAST>), dim3((unsigned)tm * tn * batch), dim3(S::WG_THREADS), S::LDS, st, q, tm, tn, r);
   return SGPO_OK;
 }
 
-int pick_symmetric(int64_t m, int64_t batch) {
-  auto tri = [&](int64_t s) { const int64_t t = (m + s - 1) / s; return batch * t * (t + 1) / 2; };
-  return tri(256) >= 160 ? 2 : tri(128) >= 160 ? 1 : 0;
+// The tile side with the least rounds x work per round: `count` tiles of side s on 256 CUs, two workgroups of the 128 tile to a CU; the small
+// tiles move more bytes per product (measured rates of one CU, relative: 1, 0.93, 0.9, 0.45).
+template <typename F>
+int pick(F count) {
+  const struct { int side, per_cu; double rate; } c[4] = {{256, 1, 1.0}, {192, 1, 0.93}, {128, 2, 0.9}, {64, 1, 0.45}};
+  int best = 0;
+  double least = 1e300;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = count(c[i].side), slots = 256 * c[i].per_cu;
+    const double t = (double)((n + slots - 1) / slots) * c[i].side * c[i].side * (n > 256 ? c[i].per_cu : 1) / c[i].rate;
+    if (t < least) { least = t; best = c[i].side; }
+  }
+  return best;
 }
-int pick_full(int64_t m, int64_t n, int64_t batch) {
-  auto cnt = [&](int64_t s) { return batch * ((m + s - 1) / s) * ((n + s - 1) / s); };
-  return cnt(256) >= 160 ? 2 : cnt(128) >= 160 ? 1 : 0;
+template <int MODE>
+int symmetric_any(int side, const Mats& q, int batch, const float* coef, hipStream_t st) {
+  switch (side) {
+    case 256: return symmetric<ShapeL, MODE>(q, batch, coef, st);
+    case 192: return symmetric<ShapeN, MODE>(q, batch, coef, st);
+    case 128: return symmetric<ShapeM, MODE>(q, batch, coef, st);
+    default: return symmetric<ShapeS, MODE>(q, batch, coef, st);
+  }
+}
+template <bool TALLX, bool LAST>
+int apply_any(int side, const Mats& q, int batch, const Result& r, hipStream_t st) {
+  switch (side) {
+    case 256: return apply<ShapeL, TALLX, LAST>(q, batch, r, st);
+    case 192: return apply<ShapeN, TALLX, LAST>(q, batch, r, st);
+    case 128: return apply<ShapeM, TALLX, LAST>(q, batch, r, st);
+    default: return apply<ShapeS, TALLX, LAST>(q, batch, r, st);
+  }
 }
 
-struct Sizes { int m, n; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, bytes; };
+struct Sizes { int d, longer; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, bytes; };
 Sizes sizes(int batch, int rows, int cols) {
-  Sizes s;
-  s.m = rows < cols ? rows : cols;
-  s.n = rows < cols ? cols : rows;
-  s.ldx = round_up(s.n, 32) * 2;
-  s.ldg = round_up(s.m, 32) * 2;
-  s.x = (size_t)s.m * s.ldx; s.g = (size_t)s.m * s.ldg;
+  Sizes s = {};
+  s.d = rows < cols ? rows : cols;
+  s.longer = rows < cols ? cols : rows;
+  if (s.longer <= 128) return s;   // one launch, no scratch
+  s.ldx = round_up(cols, 32) * 2;
+  s.ldg = round_up(s.d, 32) * 2;
+  s.x = (size_t)rows * s.ldx; s.g = (size_t)s.d * s.ldg;
   size_t at = 0;
   auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t)255; return o; };
   take((size_t)batch * PARTS * 8);
@@ -428,7 +474,7 @@ int orthogonalise_small(const Source& src, int batch, const float* coef, int ste
   for (int i = 0; i < 3 * steps; ++i) t.v[i] = coef[i];
   ALLOW((small_kernel<T, E>), Small<E>::LDS);
   hipLaunchKernelGGL((small_kernel<T, E>), dim3(batch), dim3(Small<E>::THREADS), Small<E>::LDS, st, src, src.rows < src.cols ? src.rows : src.cols,
-                     src.rows < src.cols ? src.cols : src.rows, t, steps, eps, res);
+                     src.rows < src.cols ? src.cols : src.rows, src.rows > src.cols, t, steps, eps, res);
   SGPO_CHECK_HIP(hipGetLastError());
   return SGPO_OK;
 }
@@ -436,27 +482,29 @@ int orthogonalise_small(const Source& src, int batch, const float* coef, int ste
 template <typename T>
 int orthogonalise(const Source& src, int batch, const float* coef, int steps, double eps, Result res, char* ws, hipStream_t st) {
   const Sizes z = sizes(batch, src.rows, src.cols);
+  res.rows = src.rows; res.cols = src.cols;
+  res.vec = src.cols % 4 == 0 && (uintptr_t)res.out % (res.out_bf16 ? 8 : 16) == 0;
+  if (z.longer <= 64) return orthogonalise_small<T, 64>(src, batch, coef, steps, eps, res, st);
+  if (z.longer <= 128) return orthogonalise_small<T, 128>(src, batch, coef, steps, eps, res, st);
   double* part = reinterpret_cast<double*>(ws);
-  Mats q{(bf16_t*)(ws + z.off_x), (bf16_t*)(ws + z.off_y), (bf16_t*)(ws + z.off_g), (bf16_t*)(ws + z.off_p), z.ldx, z.ldg, (int64_t)z.x, (int64_t)z.g, z.m, z.n};
-  res.tall = src.rows > src.cols; res.rows = src.rows; res.cols = src.cols;
-  if (z.n <= 64) return orthogonalise_small<T, 64>(src, batch, coef, steps, eps, res, st);
-  if (z.n <= 128) return orthogonalise_small<T, 128>(src, batch, coef, steps, eps, res, st);
+  Mats q{(bf16_t*)(ws + z.off_x), (bf16_t*)(ws + z.off_y), (bf16_t*)(ws + z.off_g), (bf16_t*)(ws + z.off_p), z.ldx, z.ldg, (int64_t)z.x, (int64_t)z.g, src.rows, src.cols, z.d};
+  const bool tall = src.rows > src.cols;
   // about 16 elements a thread
   const int64_t want = ((int64_t)src.rows * src.cols + 4095) / 4096;
   const int parts = want < PARTS ? (int)want : PARTS;
   hipLaunchKernelGGL((square_kernel<T>), dim3(parts, batch), dim3(256), 0, st, src, part);
-  const dim3 grid((unsigned)((z.ldx / 2 + 63) / 64), (unsigned)((z.m + 63) / 64), batch);
-  if (res.tall) hipLaunchKernelGGL((load_kernel<T, true>), grid, dim3(256), 0, st, src, part, parts, eps, q.X, z.m, z.n, z.ldx, (int64_t)z.x);
-  else hipLaunchKernelGGL((load_kernel<T, false>), grid, dim3(256), 0, st, src, part, parts, eps, q.X, z.m, z.n, z.ldx, (int64_t)z.x);
-  const int cs = pick_symmetric(z.m, batch), cf = pick_full(z.m, z.n, batch);
+  const int64_t blocks = ((int64_t)src.rows * (z.ldx / 8) + 255) / 256;
+  hipLaunchKernelGGL((load_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), batch), dim3(256), 0, st, src, part, parts, eps, q.X, z.ldx, (int64_t)z.x);
+  auto up = [](int64_t n, int64_t s) { return (n + s - 1) / s; };
+  const int cs = pick([&](int s) { return batch * up(z.d, s) * (up(z.d, s) + 1) / 2; });
+  const int cf = pick([&](int s) { return batch * up(src.rows, s) * up(src.cols, s); });
   for (int k = 0; k < steps; ++k) {
-    const float a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
-    int rc = cs == 2 ? symmetric<ShapeL, false>(q, batch, b, c, st) : cs == 1 ? symmetric<ShapeM, false>(q, batch, b, c, st) : symmetric<ShapeS, false>(q, batch, b, c, st);
-    if (rc) return rc;
-    rc = cs == 2 ? symmetric<ShapeL, true>(q, batch, b, c, st) : cs == 1 ? symmetric<ShapeM, true>(q, batch, b, c, st) : symmetric<ShapeS, true>(q, batch, b, c, st);
-    if (rc) return rc;
-    if (k + 1 < steps) rc = cf == 2 ? apply<ShapeL, false>(q, batch, a, res, st) : cf == 1 ? apply<ShapeM, false>(q, batch, a, res, st) : apply<ShapeS, false>(q, batch, a, res, st);
-    else rc = cf == 2 ? apply<ShapeL, true>(q, batch, a, res, st) : cf == 1 ? apply<ShapeM, true>(q, batch, a, res, st) : apply<ShapeS, true>(q, batch, a, res, st);
+    int rc = tall ? symmetric_any<TALL>(cs, q, batch, coef + 3 * k, st) : symmetric_any<WIDE>(cs, q, batch, coef + 3 * k, st);
+    if (!rc) rc = symmetric_any<POLY>(cs, q, batch, coef + 3 * k, st);
+    if (!rc) {
+      if (k + 1 < steps) rc = tall ? apply_any<true, false>(cf, q, batch, res, st) : apply_any<false, false>(cf, q, batch, res, st);
+      else rc = tall ? apply_any<true, true>(cf, q, batch, res, st) : apply_any<false, true>(cf, q, batch, res, st);
+    }
     if (rc) return rc;
     bf16_t* t = q.X; q.X = q.Y; q.Y = t;
   }
@@ -485,10 +533,10 @@ extern "C" int sgpo_newton_schulz(const void* update, int dtype, int batch, int 
   if (rc) return rc;
   SGPO_REQUIRE(dtype == SGPO_DTYPE_F32 || dtype == SGPO_DTYPE_BF16, "newton_schulz: unknown dtype %d", dtype);
   if (!batch || !rows || !cols) return SGPO_OK;
-  SGPO_REQUIRE(update && out && workspace, "newton_schulz: null argument");
+  SGPO_REQUIRE(update && out, "newton_schulz: null argument");
   SGPO_REQUIRE(ld >= cols || rows == 1, "newton_schulz: row pitch %lld below %d columns", (long long)ld, cols);
   const size_t need = sgpo_newton_schulz_workspace_bytes(batch, rows, cols);
-  if (workspace_bytes < need) { sgpo_set_error("newton_schulz: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
+  if (need && (!workspace || workspace_bytes < need)) { sgpo_set_error("newton_schulz: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
   const Source s{update, nullptr, 0.f, 0, stride_b, ld, rows, cols};
   const Result r{out, 1, 0, 0, 0, 0, 0.f, 0.f};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -504,12 +552,12 @@ extern "C" int sgpo_muon_step(void* weight, int weight_dtype, const void* grad, 
   SGPO_REQUIRE((weight_dtype == SGPO_DTYPE_F32 || weight_dtype == SGPO_DTYPE_BF16) && (grad_dtype == SGPO_DTYPE_F32 || grad_dtype == SGPO_DTYPE_BF16),
                "muon_step: unknown dtype %d / %d", weight_dtype, grad_dtype);
   if (!batch || !rows || !cols) return SGPO_OK;
-  SGPO_REQUIRE(weight && grad && momentum_buffer && workspace, "muon_step: null argument");
+  SGPO_REQUIRE(weight && grad && momentum_buffer, "muon_step: null argument");
   const size_t need = sgpo_newton_schulz_workspace_bytes(batch, rows, cols);
-  if (workspace_bytes < need) { sgpo_set_error("muon_step: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
+  if (need && (!workspace || workspace_bytes < need)) { sgpo_set_error("muon_step: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
   const Source s{grad, momentum_buffer, momentum, nesterov != 0, (int64_t)rows * cols, cols, rows, cols};
   const double ratio = rows > cols ? (double)rows / cols : 1.0;
-  const Result r{weight, weight_dtype == SGPO_DTYPE_BF16, 0, 0, 0, 1, (float)(1.0 - (double)lr * weight_decay), (float)(lr * sqrt(ratio))};
+  const Result r{weight, weight_dtype == SGPO_DTYPE_BF16, 0, 0, 1, 0, (float)(1.0 - (double)lr * weight_decay), (float)(lr * sqrt(ratio))};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return grad_dtype == SGPO_DTYPE_BF16 ? orthogonalise<bf16_t>(s, batch, coefficients, steps, eps, r, (char*)workspace, st)
                                        : orthogonalise<float>(s, batch, coefficients, steps, eps, r, (char*)workspace, st);

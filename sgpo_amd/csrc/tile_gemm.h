@@ -44,17 +44,26 @@ __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <int BM_, int BN_, int WM_, int WN_, int PL_, int NST_>
+// KG > 1: KG groups of WM x WN waves share the K loop of one tile, each with LDS slots of its own, and add up at the end (in the order of the groups).
+// A small tile's step is a chain of latencies -- barrier, LDS, products -- that more waves on the CU hide and more groups shorten.
+template <int BM_, int BN_, int WM_, int WN_, int PL_, int NST_, int KG_ = 1>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, PL = PL_, NST = NST_;
-  static constexpr int THREADS = 64 * WM * WN;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, PL = PL_, NST = NST_, KG = KG_;
+  static constexpr int THREADS = 64 * WM * WN, WG_THREADS = THREADS * KG;   // of a group, of the workgroup
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;   // 16x16 products of a wave
   static constexpr int KSTEP = PL == 1 ? 64 : 32;
   static constexpr int ROWB = PL == 3 ? 192 : 128;             // bytes of a KC row in a step
   static constexpr int A_BYTES = BM * ROWB, B_BYTES = BN * ROWB, STAGE = A_BYTES + B_BYTES;
-  static constexpr int LDS = NST * STAGE;
+  static constexpr int SLOTS = NST * STAGE, LDS = KG * SLOTS;
   static_assert(A_BYTES % (16 * THREADS) == 0 && B_BYTES % (16 * THREADS) == 0, "whole DMA pieces");
   static_assert(LDS <= 163840, "LDS of a CU");
+  static_assert(KG == 1 || (MT * NT % KG == 0 && MT * NT * 1024 * WM * WN <= SLOTS), "the groups' sums pass through the slots");
+  // this thread within its group; its wave there; its group (uniform)
+  __device__ static __forceinline__ int tid() { return KG == 1 ? (int)threadIdx.x : (int)threadIdx.x % THREADS; }
+  __device__ static __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) % (WM * WN); }
+  __device__ static __forceinline__ int group() { return KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) / (WM * WN); }
+  // whether this wave holds the finished 16x16 product (x, y) of its part of the tile
+  __device__ static __forceinline__ bool owns(int x, int y) { return KG == 1 || (x * NT + y) % KG == group(); }
 };
 
 // chunk permutation of a KM row: the 16 rows that one transposed read touches ({0..3} + 8 l4) go to different banks
@@ -75,9 +84,11 @@ struct Stager {
   uint64_t base;          // uniform: the step's first byte
   int64_t left, step;     // bytes of the operand from there on; bytes between steps
   uint32_t off[PIECES];   // per lane, bytes
+  int valid;              // steps of this group that exist; further ones read as zero
 
-  __device__ __forceinline__ void init(const Operand& o, int r0, int k0) {
-    const int tid = threadIdx.x;
+  __device__ __forceinline__ void init(const Operand& o, int r0, int k0, int steps) {
+    const int tid = S::tid();
+    valid = steps;
     const int64_t ldb = o.ld * 2;
     if constexpr (KIND == KC) {
       base = (uint64_t)(o.p + (int64_t)r0 * o.ld + (int64_t)k0 * S::PL);
@@ -98,14 +109,13 @@ struct Stager {
     }
   }
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
-    const uint32_t n = left > 0xffffffffll ? 0xffffffffu : left < 0 ? 0u : (uint32_t)left;
+    const uint32_t n = (S::KG > 1 && valid <= 0) || left < 0 ? 0u : left > 0xffffffffll ? 0xffffffffu : (uint32_t)left;
     return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, n, 0x00027000);
   }
   __device__ __forceinline__ void piece(__amdgpu_buffer_rsrc_t r, int j, char* dst) const {   // dst: uniform
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr_t)(dst + (j * S::THREADS + wave * 64) * 16), 16, off[j], 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr_t)(dst + (j * S::THREADS + S::wave() * 64) * 16), 16, off[j], 0, 0, 0);
   }
-  __device__ __forceinline__ void advance() { base += step; left -= step; }
+  __device__ __forceinline__ void advance() { base += step; left -= step; if (S::KG > 1) --valid; }
   __device__ __forceinline__ void next(char* dst) {   // the whole step
     const __amdgpu_buffer_rsrc_t r = rsrc();
 #pragma unroll
@@ -142,7 +152,7 @@ __device__ __forceinline__ void run_ring(Stager<S, S::BM, KA>& sa, Stager<S, S::
   constexpr int D = S::NST - 1, OPS = Stager<S, S::BM, KA>::PIECES + Stager<S, S::BN, KB>::PIECES, NF = S::PL == 1 ? 2 : S::PL;
   static_assert(D >= 2 && OPS * 2 < 64, "vmcnt range");
   const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  const int wave = S::wave(), wm = wave / S::WN, wn = wave % S::WN;
 #pragma unroll
   for (int s = 0; s < D; ++s)
     if (s < nk) { sa.next(smem + s * S::STAGE); sb.next(smem + s * S::STAGE + S::A_BYTES); }
@@ -199,7 +209,7 @@ __device__ __forceinline__ void run_phased(Stager<S, S::BM, KA>& sa, Stager<S, S
   typedef bf16x8 FA[MT];
   typedef bf16x8 FB[NT];
   const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  const int wave = S::wave(), wm = wave / S::WN, wn = wave % S::WN;
   auto read_a = [&](FA& f, int t, const char* img, int plane) { f[t] = fragment<S, S::BM, KA>(img, wm * MT + t, plane, l16, l4); };
   auto read_b = [&](FB& f, int t, const char* img, int plane) { f[t] = fragment<S, S::BN, KB>(img + S::A_BYTES, wn * NT + t, plane, l16, l4); };
   // products of (a, b), and of what follows: na from plane pa if WA, nb from plane pb if WB, both of image `img`; DMA into `dst`
@@ -292,17 +302,39 @@ __device__ __forceinline__ void run_phased(Stager<S, S::BM, KA>& sa, Stager<S, S
   }
 }
 
-// acc[mt][nt][q] += C[m = m0 + (wm MT + mt) 16 + l16][n = n0 + (wn NT + nt) 16 + 4 l4 + q], k steps [kt0, kt0 + nk), nk >= 1.
-// Every thread of the workgroup calls it; smem is free again when it returns.
+// acc[mt][nt][q] += C[m = m0 + (wm MT + mt) 16 + l16][n = n0 + (wn NT + nt) 16 + 4 l4 + q], k steps [kt0, kt0 + nk), nk >= 1; with several
+// groups, in the products that the wave owns.  Every thread of the workgroup calls it; smem is free again when it returns.
 template <class S, int KA, int KB>
 __device__ __forceinline__ void run(const Operand& a, const Operand& b, int m0, int n0, int kt0, int nk, char* smem, f32x4 (&acc)[S::MT][S::NT]) {
   Stager<S, S::BM, KA> sa;
   Stager<S, S::BN, KB> sb;
-  sa.init(a, m0, kt0 * S::KSTEP);
-  sb.init(b, n0, kt0 * S::KSTEP);
-  if constexpr (S::NST == 2) run_phased<S, KA, KB>(sa, sb, nk, smem, acc);
-  else run_ring<S, KA, KB>(sa, sb, nk, smem, acc);
+  const int each = (nk + S::KG - 1) / S::KG, g = S::group(), own = min(each, nk - g * each);
+  sa.init(a, m0, (kt0 + g * each) * S::KSTEP, own);
+  sb.init(b, n0, (kt0 + g * each) * S::KSTEP, own);
+  char* slots = smem + g * S::SLOTS;
+  if constexpr (S::NST == 2) run_phased<S, KA, KB>(sa, sb, each, slots, acc);
+  else run_ring<S, KA, KB>(sa, sb, each, slots, acc);
   __syncthreads();
+  if constexpr (S::KG > 1) {
+    f32x4* mine = reinterpret_cast<f32x4*>(slots);   // [wave][product][lane]
+    const int at = S::wave() * S::MT * S::NT * 64 + (threadIdx.x & 63);
+#pragma unroll
+    for (int x = 0; x < S::MT; ++x)
+#pragma unroll
+      for (int y = 0; y < S::NT; ++y) mine[at + (x * S::NT + y) * 64] = acc[x][y];
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < S::MT; ++x)
+#pragma unroll
+      for (int y = 0; y < S::NT; ++y) {
+        if (!S::owns(x, y)) continue;
+        f32x4 v = *reinterpret_cast<const f32x4*>(smem + (at + (x * S::NT + y) * 64) * 16);
+#pragma unroll
+        for (int k = 1; k < S::KG; ++k) v += *reinterpret_cast<const f32x4*>(smem + k * S::SLOTS + (at + (x * S::NT + y) * 64) * 16);
+        acc[x][y] = v;
+      }
+    __syncthreads();
+  }
 }
 
 template <class S>

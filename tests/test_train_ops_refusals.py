@@ -76,7 +76,7 @@ def test_library_refuses_bad_arguments_without_a_device():
     refused(lib.sgpo_newton_schulz(one, 0, 1, 4, 4, 16, 4, coef, 0, 1e-7, one, one, 1 << 30, None), 'triples')
     refused(lib.sgpo_newton_schulz(one, 5, 1, 4, 4, 16, 4, coef, 1, 1e-7, one, one, 1 << 30, None), 'dtype')
     refused(lib.sgpo_newton_schulz(one, 0, 1, 4, 4, 16, 3, coef, 1, 1e-7, one, one, 1 << 30, None), 'pitch')
-    refused(lib.sgpo_newton_schulz(one, 0, 1, 4, 4, 16, 4, coef, 1, 1e-7, one, one, 16, None), 'workspace')
+    refused(lib.sgpo_newton_schulz(one, 0, 1, 400, 4, 1600, 4, coef, 1, 1e-7, one, one, 16, None), 'workspace')
     refused(lib.sgpo_newton_schulz(one, 0, 1, -4, 4, 16, 4, coef, 1, 1e-7, one, one, 16, None), 'negative')
     refused(lib.sgpo_muon_step(one, 0, one, 9, one, 1, 4, 4, 0.1, 0.9, 1, 0.0, coef, 1, 1e-7, one, 1 << 30, None), 'dtype')
     refused(lib.sgpo_muon_step(one, 0, None, 0, one, 1, 4, 4, 0.1, 0.9, 1, 0.0, coef, 1, 1e-7, one, 1 << 30, None), 'null')
