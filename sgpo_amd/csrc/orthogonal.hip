@@ -386,11 +386,6 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void apply_kernel(Mats q, int tm,
   }
 }
 
-typedef tg::Shape<256, 256, 2, 4, 2, 2> ShapeL;
-typedef tg::Shape<192, 192, 2, 4, 2, 2> ShapeN;
-typedef tg::Shape<128, 128, 2, 2, 2, 2> ShapeM;
-typedef tg::Shape<64, 64, 2, 2, 2, 2, 4> ShapeS;
-
 template <typename K>
 int allow_lds(K kernel, int bytes) {
   SGPO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
@@ -417,37 +412,49 @@ int apply(const Mats& q, int batch, const Result& r, hipStream_t st) {
   return SGPO_OK;
 }
 
-// The tile side with the least rounds x work per round: `count` tiles of side s on 256 CUs, two workgroups of the 128 tile to a CU; the small
-// tiles move more bytes per product (measured rates of one CU, relative: 1, 0.93, 0.9, 0.45).
+// Tile shapes, and what one tile costs (us): `symmetric` and `apply` + `step` per 32 k, one workgroup on a CU, measured at 1 x 1536 x 512 and
+// 8 x 512 x 2048.  Small tiles spread a small product over the CUs and read more bytes for it; large ones the other way round.
+struct Kind { int side, per_cu; double symmetric, apply, step; };
+constexpr Kind KINDS[] = {{256, 1, 30., 18., 1.40}, {192, 1, 17., 11., 0.90}, {129, 1, 11., 8.2, 0.46}, {128, 2, 11., 5.3, 0.575},
+                          {96, 1, 8.5, 7.0, 0.276}, {64, 2, 4.5, 4.2, 0.21}, {32, 2, 3.6, 3.6, 0.08}};
+typedef tg::Shape<256, 256, 2, 4, 2, 2> Shape256;
+typedef tg::Shape<192, 192, 2, 4, 2, 2> Shape192;
+typedef tg::Shape<128, 128, 2, 2, 2, 2, 2> Shape129;   // 128 x 128 with two groups over K: one workgroup fills a CU
+typedef tg::Shape<128, 128, 2, 2, 2, 2> Shape128;
+typedef tg::Shape<96, 96, 2, 2, 2, 2, 3> Shape96;
+typedef tg::Shape<64, 64, 2, 2, 2, 2, 2> Shape64;
+typedef tg::Shape<32, 32, 1, 1, 2, 2, 4> Shape32;
+
+// the kind with the least rounds of the 256 CUs x cost of a tile; count(side) tiles of `steps` K steps
 template <typename F>
-int pick(F count) {
-  const struct { int side, per_cu; double rate; } c[4] = {{256, 1, 1.0}, {192, 1, 0.93}, {128, 2, 0.9}, {64, 1, 0.45}};
+int pick(F count, int64_t steps, bool sym) {
   int best = 0;
   double least = 1e300;
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = count(c[i].side), slots = 256 * c[i].per_cu;
-    const double t = (double)((n + slots - 1) / slots) * c[i].side * c[i].side * (n > 256 ? c[i].per_cu : 1) / c[i].rate;
-    if (t < least) { least = t; best = c[i].side; }
+  for (const Kind& k : KINDS) {
+    const int64_t n = count(k.side == 129 ? 128 : k.side);
+    const double rounds = k.per_cu == 1 ? (double)((n + 255) / 256) : n <= 256 ? 1. : (n + 127) / 128 * 0.5;
+    const double t = rounds * ((sym ? k.symmetric : k.apply) + steps * k.step);
+    if (t < least) { least = t; best = k.side; }
   }
   return best;
 }
-template <int MODE>
-int symmetric_any(int side, const Mats& q, int batch, const float* coef, hipStream_t st) {
-  switch (side) {
-    case 256: return symmetric<ShapeL, MODE>(q, batch, coef, st);
-    case 192: return symmetric<ShapeN, MODE>(q, batch, coef, st);
-    case 128: return symmetric<ShapeM, MODE>(q, batch, coef, st);
-    default: return symmetric<ShapeS, MODE>(q, batch, coef, st);
+#define FOR_KIND(K, CALL)                                              \
+  switch (K) {                                                         \
+    case 256: { typedef Shape256 S; return CALL; }                     \
+    case 192: { typedef Shape192 S; return CALL; }                     \
+    case 129: { typedef Shape129 S; return CALL; }                     \
+    case 128: { typedef Shape128 S; return CALL; }                     \
+    case 96: { typedef Shape96 S; return CALL; }                       \
+    case 64: { typedef Shape64 S; return CALL; }                       \
+    default: { typedef Shape32 S; return CALL; }                       \
   }
+template <int MODE>
+int symmetric_any(int kind, const Mats& q, int batch, const float* coef, hipStream_t st) {
+  FOR_KIND(kind, (symmetric<S, MODE>(q, batch, coef, st)))
 }
 template <bool TALLX, bool LAST>
-int apply_any(int side, const Mats& q, int batch, const Result& r, hipStream_t st) {
-  switch (side) {
-    case 256: return apply<ShapeL, TALLX, LAST>(q, batch, r, st);
-    case 192: return apply<ShapeN, TALLX, LAST>(q, batch, r, st);
-    case 128: return apply<ShapeM, TALLX, LAST>(q, batch, r, st);
-    default: return apply<ShapeS, TALLX, LAST>(q, batch, r, st);
-  }
+int apply_any(int kind, const Mats& q, int batch, const Result& r, hipStream_t st) {
+  FOR_KIND(kind, (apply<S, TALLX, LAST>(q, batch, r, st)))
 }
 
 struct Sizes { int d, longer; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, bytes; };
@@ -496,14 +503,15 @@ int orthogonalise(const Source& src, int batch, const float* coef, int steps, do
   const int64_t blocks = ((int64_t)src.rows * (z.ldx / 8) + 255) / 256;
   hipLaunchKernelGGL((load_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), batch), dim3(256), 0, st, src, part, parts, eps, q.X, z.ldx, (int64_t)z.x);
   auto up = [](int64_t n, int64_t s) { return (n + s - 1) / s; };
-  const int cs = pick([&](int s) { return batch * up(z.d, s) * (up(z.d, s) + 1) / 2; });
-  const int cf = pick([&](int s) { return batch * up(src.rows, s) * up(src.cols, s); });
+  auto triangles = [&](int s) { return batch * up(z.d, s) * (up(z.d, s) + 1) / 2; };
+  const int kg = pick(triangles, up(z.longer, 32), true), kp = pick(triangles, up(z.d, 32), true);
+  const int ka = pick([&](int s) { return batch * up(src.rows, s) * up(src.cols, s); }, up(z.d, 32), false);
   for (int k = 0; k < steps; ++k) {
-    int rc = tall ? symmetric_any<TALL>(cs, q, batch, coef + 3 * k, st) : symmetric_any<WIDE>(cs, q, batch, coef + 3 * k, st);
-    if (!rc) rc = symmetric_any<POLY>(cs, q, batch, coef + 3 * k, st);
+    int rc = tall ? symmetric_any<TALL>(kg, q, batch, coef + 3 * k, st) : symmetric_any<WIDE>(kg, q, batch, coef + 3 * k, st);
+    if (!rc) rc = symmetric_any<POLY>(kp, q, batch, coef + 3 * k, st);
     if (!rc) {
-      if (k + 1 < steps) rc = tall ? apply_any<true, false>(cf, q, batch, res, st) : apply_any<false, false>(cf, q, batch, res, st);
-      else rc = tall ? apply_any<true, true>(cf, q, batch, res, st) : apply_any<false, true>(cf, q, batch, res, st);
+      if (k + 1 < steps) rc = tall ? apply_any<true, false>(ka, q, batch, res, st) : apply_any<false, false>(ka, q, batch, res, st);
+      else rc = tall ? apply_any<true, true>(ka, q, batch, res, st) : apply_any<false, true>(ka, q, batch, res, st);
     }
     if (rc) return rc;
     bf16_t* t = q.X; q.X = q.Y; q.Y = t;

@@ -57,7 +57,7 @@ struct Shape {
   static constexpr int SLOTS = NST * STAGE, LDS = KG * SLOTS;
   static_assert(A_BYTES % (16 * THREADS) == 0 && B_BYTES % (16 * THREADS) == 0, "whole DMA pieces");
   static_assert(LDS <= 163840, "LDS of a CU");
-  static_assert(KG == 1 || (MT * NT % KG == 0 && MT * NT * 1024 * WM * WN <= SLOTS), "the groups' sums pass through the slots");
+  static_assert(KG == 1 || BM * BN * 4 <= SLOTS, "the groups' sums pass through the slots");
   // this thread within its group; its wave there; its group (uniform)
   __device__ static __forceinline__ int tid() { return KG == 1 ? (int)threadIdx.x : (int)threadIdx.x % THREADS; }
   __device__ static __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) % (WM * WN); }
