@@ -47,6 +47,24 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t ld, int
   }
 }
 
+// dst [cols_out][rows_out] = src transposed, bf16, with the same zeros; 64 x 64 tiles through LDS
+__global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* src, int64_t ld, int rows, int cols, bf16_t* dst, int64_t rows_out,
+                                                        const int64_t* targets, int64_t ignore) {
+  __shared__ bf16_t tile[64][66];
+  const int64_t r0 = (int64_t)blockIdx.x * 64;
+  const int c0 = blockIdx.y * 64;
+  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+    const int r = i >> 6, c = i & 63;
+    const bool in = r0 + r < rows && c0 + c < cols && targets[r0 + r] != ignore;
+    tile[c][r] = in ? src[(r0 + r) * ld + c0 + c] : (bf16_t)0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * 32; i += 256) {
+    const int c = i >> 5, r = (i & 31) * 2;
+    *reinterpret_cast<uint32_t*>(dst + (int64_t)(c0 + c) * rows_out + r0 + r) = *reinterpret_cast<const uint32_t*>(&tile[c][r]);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------ forward
 struct LossArgs {
   tg::Operand h, w;
@@ -64,16 +82,27 @@ __device__ __forceinline__ void logits(const LossArgs& p, int m0, int n0, char* 
   tg::run<S, tg::KC, tg::KC>(p.h, p.w, m0, n0, 0, p.nk, smem, acc);
   const int lane = threadIdx.x & 63, l4 = lane >> 4;
   const int wave = (int)threadIdx.x >> 6, wn = wave % S::WN;
+  const int c0 = n0 + wn * S::NT * 16 + 4 * l4;
+  if (p.bias) {
 #pragma unroll
-  for (int y = 0; y < S::NT; ++y)
+    for (int y = 0; y < S::NT; ++y)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4 + q;
-      const bool in = n < p.n_cls;
-      const float b = in && p.bias ? p.bias[p.v0 + n] : 0.f;
+      for (int q = 0; q < 4; ++q) {
+        const float b = p.bias[p.v0 + min(c0 + y * 16 + q, p.n_cls - 1)];
 #pragma unroll
-      for (int x = 0; x < S::MT; ++x) acc[x][y][q] = in ? acc[x][y][q] + b : -INFINITY;
-    }
+        for (int x = 0; x < S::MT; ++x) acc[x][y][q] += b;
+      }
+  }
+  if (n0 + S::BN > p.n_cls) {   // the last column of tiles: classes that do not exist
+#pragma unroll
+    for (int y = 0; y < S::NT; ++y)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (c0 + y * 16 + q >= p.n_cls) {
+#pragma unroll
+          for (int x = 0; x < S::MT; ++x) acc[x][y][q] = -INFINITY;
+        }
+  }
 }
 
 __device__ __forceinline__ float lanes4_max(float v) {   // over the four lanes that share l16
@@ -89,6 +118,12 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
   s = s * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * LOG2E);
   m = top;
+}
+
+__device__ __forceinline__ void store_loss(float l, float at_target, int64_t t, int64_t ignore, int V, float* nll, float* lse) {
+  *lse = l;
+  // a target that is no class has no loss: NaN, so that the step shows it
+  *nll = t == ignore ? 0.f : (t < 0 || t >= V) ? __builtin_nanf("") : l - at_target;
 }
 
 // part[tile column][row of the chunk] = (max, sum);  at_target[row] = the target's logit
@@ -121,13 +156,14 @@ __global__ __launch_bounds__(S::THREADS, 2) void lse_kernel(LossArgs p, int tm, 
     s = lanes4_sum(s);
     if (l4 == 0) share[wn * S::BM + lm] = make_float2(top, s);
     if (m < p.n_rows) {
-      const int64_t t = p.targets[p.r0 + m] - p.v0 - n0;
-      if (t >= 0 && t < S::BN && p.targets[p.r0 + m] != p.ignore) {
+      const int64_t t = p.targets[p.r0 + m] - p.v0;
+      const int64_t tq = t - n0 - wn * S::NT * 16 - 4 * l4;   // 16 y + q, if the class lies with this lane
+      if (tq >= 0 && tq < S::NT * 16 && (tq & 12) == 0 && t < p.n_cls) {
 #pragma unroll
         for (int y = 0; y < S::NT; ++y)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            if ((wn * S::NT + y) * 16 + 4 * l4 + q == (int)t && n0 + (int)t < p.n_cls) at_target[m] = acc[x][y][q];
+            if (16 * y + q == (int)tq) at_target[m] = acc[x][y][q];
       }
     }
   }
@@ -143,28 +179,24 @@ __global__ __launch_bounds__(S::THREADS, 2) void lse_kernel(LossArgs p, int tm, 
   }
 }
 
-// joins a token's pairs: 64 tokens per workgroup, four waves share a token's tile columns
+// joins a token's pairs: 16 tokens per workgroup, 16 threads share a token's tile columns
 __global__ __launch_bounds__(256) void finish_kernel(const float2* part, int n_rows, int tn, const float* at_target, const int64_t* targets,
                                                      int64_t ignore, int V, float* nll, float* lse) {
-  __shared__ float2 share[4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int m = blockIdx.x * 64 + lane;
+  __shared__ float2 share[16][17];
+  const int r = threadIdx.x & 15, w = threadIdx.x >> 4;
+  const int m = blockIdx.x * 16 + r;
   float a = -INFINITY, s = 0.f;
   if (m < n_rows)
-    for (int i = w; i < tn; i += 4) {
+    for (int i = w; i < tn; i += 16) {
       const float2 b = part[(int64_t)i * n_rows + m];
       join(a, s, b.x, b.y);
     }
-  share[w][lane] = make_float2(a, s);
+  share[w][r] = make_float2(a, s);
   __syncthreads();
   if (w == 0 && m < n_rows) {
 #pragma unroll
-    for (int i = 1; i < 4; ++i) join(a, s, share[i][lane].x, share[i][lane].y);
-    const float l = a + logf(s);
-    const int64_t t = targets[m];
-    lse[m] = l;
-    // a target that is no class has no loss: NaN, so that the step shows it
-    nll[m] = t == ignore ? 0.f : (t < 0 || t >= V) ? __builtin_nanf("") : l - at_target[m];
+    for (int i = 1; i < 16; ++i) join(a, s, share[i][r].x, share[i][r].y);
+    store_loss(a + logf(s), at_target[m], targets[m], ignore, V, nll + m, lse + m);
   }
 }
 
@@ -210,30 +242,60 @@ __global__ __launch_bounds__(S::THREADS, 2) void grad_kernel(LossArgs p, int tm,
   for (int y = 0; y < S::NT; ++y)
 #pragma unroll
     for (int q = 0; q < 4; ++q) cs[y][q] = 0.f;
+  // The planes of XG row blocks at a time pass through this wave's part of the LDS, so that they leave in whole lines: from the registers a
+  // row would go out in pieces of 32 bytes (a piece of 8192 x 16384: 610 us with those).
+  constexpr int RB = S::NT * 32 * S::PL, CH = RB / 16, MASK = CH % 8 == 0 ? 7 : 3;   // bytes and 16-B chunks of a wave's row
+  constexpr int PART = S::LDS / (S::WM * S::WN), FIT = PART / (16 * RB), XG = FIT >= S::MT ? S::MT : FIT >= S::MT / 2 ? S::MT / 2 : 1;
+  static_assert(XG * 16 * RB <= PART && S::MT % XG == 0, "a row block fits the wave's part");
+  char* mine = smem + wave * PART;
+  const int nb = n0 + wn * S::NT * 16;   // the wave's first column
 #pragma unroll
-  for (int x = 0; x < S::MT; ++x) {
-    const int m = m0 + (wm * S::MT + x) * 16 + l16;
-    const bool in_rows = m < p.n_rows;
-    const int64_t t = in_rows ? p.targets[m] : p.ignore;
-    const bool keep = in_rows && t != p.ignore;
-    const bool bad = keep && (t < 0 || t >= (int64_t)p.w.rows + p.v0);
-    const float l = keep ? lse[m] : 0.f;
-    const float gm = keep ? (bad ? __builtin_nanf("") : g[g_rows ? m : 0] * f) : 0.f;
-    const int tl = (int)(keep ? (t - p.v0 < 0 || t - p.v0 > 0x7fffffff ? -1 : t - p.v0) : -1);
+  for (int g0 = 0; g0 < S::MT; g0 += XG) {
 #pragma unroll
-    for (int y = 0; y < S::NT; ++y) {
-      const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4;
-      float v[4];
+    for (int xx = 0; xx < XG; ++xx) {
+      const int x = g0 + xx, m = m0 + (wm * S::MT + x) * 16 + l16;
+      const bool in_rows = m < p.n_rows;
+      const int64_t t = in_rows ? p.targets[m] : p.ignore;
+      const bool keep = in_rows && t != p.ignore;
+      const bool bad = keep && (t < 0 || t >= (int64_t)p.w.rows + p.v0);
+      const float l = keep ? lse[m] : 0.f;
+      const float gm = keep ? (bad ? __builtin_nanf("") : g[g_rows ? m : 0] * f) : 0.f;
+      const int64_t tw = t - p.v0 - nb - 4 * l4;
+      const int tq = tw >= 0 && tw < S::NT * 16 ? (int)tw : -1;   // 16 y + q, if the class lies with this lane
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float e = __builtin_amdgcn_exp2f((acc[x][y][q] - l) * LOG2E);
-        v[q] = keep && n + q < p.n_cls ? gm * (e - (n + q == tl ? 1.f : 0.f)) : 0.f;
-        cs[y][q] += v[q];
+      for (int y = 0; y < S::NT; ++y) {
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float e = __builtin_amdgcn_exp2f((acc[x][y][q] - l) * LOG2E);
+          v[q] = gm * (16 * y + q == tq ? e - 1.f : e);
+          v[q] = keep ? v[q] : 0.f;
+          cs[y][q] += v[q];
+        }
+        float pl[4][S::PL];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tg::split<S::PL>(v[q], pl[q]);
+        const int r = xx * 16 + l16, e0 = y * 16 + 4 * l4;   // element within the wave's row
+#pragma unroll
+        for (int k = 0; k < S::PL; ++k) {
+          const int at = (e0 >> 5) * (64 * S::PL) + k * 64 + (e0 & 31) * 2;   // bytes
+          *reinterpret_cast<uint2*>(mine + r * RB + (((at >> 4) ^ (r & MASK)) << 4) + (at & 15)) =
+              make_uint2(pack_bf16x2(pl[0][k], pl[1][k]), pack_bf16x2(pl[2][k], pl[3][k]));
+        }
       }
-      if (m < rows_pad && n < cols_pad) tg::store4<S::PL>(d + (int64_t)m * cols_pad * S::PL, n, v);
     }
+    __builtin_amdgcn_wave_barrier();   // one wave's LDS accesses run in order: nothing to wait for but the data
+#pragma unroll 4
+    for (int i = lane; i < XG * 16 * CH; i += 64) {
+      const int r = i / CH, c = i - r * CH, m = m0 + (wm * S::MT + g0) * 16 + r;
+      const uint4 v = *reinterpret_cast<const uint4*>(mine + r * RB + ((c ^ (r & MASK)) << 4));
+      if (m < rows_pad && nb < cols_pad)
+        *reinterpret_cast<uint4*>(reinterpret_cast<char*>(d + ((int64_t)m * cols_pad + nb) * S::PL) + c * 16) = v;
+    }
+    __builtin_amdgcn_wave_barrier();
   }
   if (!col_sums) return;
+  __syncthreads();
   float* share = reinterpret_cast<float*>(smem);   // [WM][BN]
 #pragma unroll
   for (int y = 0; y < S::NT; ++y)
@@ -253,6 +315,186 @@ __global__ __launch_bounds__(S::THREADS, 2) void grad_kernel(LossArgs p, int tm,
   }
 }
 
+// ------------------------------------------------------------------------------------ small vocabularies (up to 64 classes)
+// A head of at most 64 classes is bound by reading the features.  A wave takes 16 tokens and all classes; operands go from memory straight
+// into fragments (fp32 ones are cut into planes in registers), so there is no LDS staging, no packed copy and, all of a token's
+// classes being in one wave, no second kernel.  KS = 4: the four waves of a workgroup share the features of 16 tokens (few tokens: four times the
+// workgroups and a quarter of the chain), KS = 1: 16 tokens each.
+// GRAD: d instead of the loss, and on the way the packed copy of the features that dweight's product reads.
+struct HeadArgs {
+  const void *h, *w;
+  int64_t ldh, ldw;
+  const float* bias;
+  const int64_t* targets;
+  int64_t ignore;
+  int N, H, V, vec;          // vec: rows may be read 16 bytes at a time
+  float *nll, *lse;          // forward's outputs; GRAD reads lse
+  const float *g, *inv;
+  int g_rows, rows_pad, h_pad;
+  bf16_t *d, *hp;            // [rows_pad][64], [rows_pad][h_pad] planes
+  float* col_sums;           // [workgroup][V], or null
+};
+
+template <typename T> struct PlanesOf { static constexpr int value = 1; };
+template <> struct PlanesOf<float> { static constexpr int value = 3; };
+
+// eight consecutive features of a row as fragments of each plane
+template <typename T, int PL>
+__device__ __forceinline__ void load8(const T* row, int e, int H, bool vec, bool live, bf16x8 (&f)[PL]) {
+  if constexpr (PL == 1) {
+    if (vec) {
+      f[0] = live ? *reinterpret_cast<const bf16x8*>(row + e) : bf16x8{};
+    } else {
+      tg::s16x8 v = {};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) if (live && e + i < H) v[i] = (short)row[e + i];
+      f[0] = *reinterpret_cast<const bf16x8*>(&v);
+    }
+  } else {
+    float x[8];
+    if (vec) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(row + e), b = *reinterpret_cast<const f32x4*>(row + e + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { x[i] = live ? a[i] : 0.f; x[4 + i] = live ? b[i] : 0.f; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = live && e + i < H ? row[e + i] : 0.f;
+    }
+    uint32_t w[PL][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float p0[PL], p1[PL];
+      tg::split<PL>(x[2 * i], p0);
+      tg::split<PL>(x[2 * i + 1], p1);
+#pragma unroll
+      for (int p = 0; p < PL; ++p) w[p][i] = pack_bf16x2(p0[p], p1[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < PL; ++p) f[p] = *reinterpret_cast<const bf16x8*>(&w[p]);
+  }
+}
+
+template <typename T, int NB, int KS, bool GRAD>
+__global__ __launch_bounds__(256) void head_kernel(HeadArgs p) {
+  constexpr int PL = PlanesOf<T>::value;
+  __shared__ f32x4 share[KS > 1 ? KS - 1 : 1][NB][64];
+  __shared__ float sums[KS > 1 ? 1 : 4][64];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), ks = KS > 1 ? wave : 0;
+  const int m = ((int)blockIdx.x * (4 / KS) + (KS > 1 ? 0 : wave)) * 16 + l16;
+  const int64_t t = m < p.N ? p.targets[m] : p.ignore;
+  const bool keep = m < p.N && t != p.ignore;
+  const T* hr = reinterpret_cast<const T*>(p.h) + (int64_t)min(m, p.N - 1) * p.ldh;
+  const T* wr[NB];
+#pragma unroll
+  for (int y = 0; y < NB; ++y) wr[y] = reinterpret_cast<const T*>(p.w) + (int64_t)min(y * 16 + l16, p.V - 1) * p.ldw;
+  f32x4 acc[NB];
+#pragma unroll
+  for (int y = 0; y < NB; ++y) acc[y] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int H = p.H, slices = (H + 31) >> 5;
+  const bool vec = p.vec;
+  auto slice = [&](int s, bool whole) {
+    const int e = s * 32 + l4 * 8;
+    bf16x8 a[PL], b[NB][PL];
+    const bool in = whole || (vec ? e < H : true);   // with 16-byte rows H is a multiple of 8
+    load8<T, PL>(hr, in ? e : 0, H, vec, in && (GRAD ? keep : true), a);
+#pragma unroll
+    for (int y = 0; y < NB; ++y) load8<T, PL>(wr[y], in ? e : 0, H, vec, in, b[y]);
+    if constexpr (GRAD) {
+      if (p.hp && m < p.rows_pad) {
+#pragma unroll
+        for (int q = 0; q < PL; ++q) *reinterpret_cast<bf16x8*>(p.hp + (int64_t)m * p.h_pad * PL + s * 32 * PL + q * 32 + l4 * 8) = a[q];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PL; ++i)
+#pragma unroll
+      for (int j = 0; i + j < PL; ++j)
+#pragma unroll
+        for (int y = 0; y < NB; ++y) acc[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[y][j], a[i], acc[y], 0, 0, 0);
+  };
+  int s = ks;
+  if (vec)
+    for (; (s + 1) * 32 <= H; s += KS) slice(s, true);
+  for (; s < slices; s += KS) slice(s, false);
+  if constexpr (GRAD) {   // the packed features' last padding
+    const int ps = p.h_pad >> 5;
+    for (; s < ps; s += KS)
+      if (p.hp && m < p.rows_pad)
+#pragma unroll
+        for (int q = 0; q < PL; ++q) *reinterpret_cast<bf16x8*>(p.hp + (int64_t)m * p.h_pad * PL + s * 32 * PL + q * 32 + l4 * 8) = bf16x8{};
+  }
+  if constexpr (KS > 1) {
+    if (ks > 0)
+#pragma unroll
+      for (int y = 0; y < NB; ++y) share[ks - 1][y][lane] = acc[y];
+    __syncthreads();
+    if (ks > 0) return;
+#pragma unroll
+    for (int k = 1; k < KS; ++k)
+#pragma unroll
+      for (int y = 0; y < NB; ++y) acc[y] += share[k - 1][y][lane];
+  }
+  float top = -INFINITY, at = 0.f;
+  const bool cls = t >= 0 && t < p.V;
+#pragma unroll
+  for (int y = 0; y < NB; ++y)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = y * 16 + 4 * l4 + q;
+      const bool in = n < p.V;
+      const float z = in ? acc[y][q] + (p.bias ? p.bias[n] : 0.f) : -INFINITY;
+      acc[y][q] = z;
+      top = fmaxf(top, z);
+      if (cls && n == (int)t) at = z;
+    }
+  if constexpr (!GRAD) {
+    top = lanes4_max(top);
+    at = lanes4_sum(at);   // three of the four lanes hold 0
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int y = 0; y < NB; ++y)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f((acc[y][q] - ref) * LOG2E);
+    sum = lanes4_sum(sum);
+    if (l4 == 0 && m < p.N) store_loss(top + logf(sum), at, t, p.ignore, p.V, p.nll + m, p.lse + m);
+  } else {
+    const float l = keep ? p.lse[m] : 0.f;
+    const float gm = keep ? (cls ? p.g[p.g_rows ? m : 0] * (p.inv ? p.inv[0] : 1.f) : __builtin_nanf("")) : 0.f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int n = y * 16 + 4 * l4;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (y < NB) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float e = __builtin_amdgcn_exp2f((acc[y < NB ? y : 0][q] - l) * LOG2E);
+          v[q] = keep && n + q < p.V ? gm * (e - (cls && n + q == (int)t ? 1.f : 0.f)) : 0.f;
+        }
+      }
+      if (m < p.rows_pad) tg::store4<PL>(p.d + (int64_t)m * 64 * PL, n, v);
+      if (p.col_sums && y < NB) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) v[q] += __shfl_xor(v[q], o);
+          if (l16 == 0) {
+            if constexpr (KS > 1) { if (n + q < p.V) p.col_sums[(int64_t)blockIdx.x * p.V + n + q] = v[q]; }
+            else sums[wave][n + q] = v[q];
+          }
+        }
+      }
+    }
+    if constexpr (KS == 1) {
+      if (!p.col_sums) return;
+      __syncthreads();
+      const int n = threadIdx.x;
+      if (n < p.V) p.col_sums[(int64_t)blockIdx.x * p.V + n] = (sums[0][n] + sums[1][n]) + (sums[2][n] + sums[3][n]);
+    }
+  }
+}
+
 // C tile of a product, K split over gridDim.y slabs: fp32 (added to what is there if `add`) or rounded to bf16
 struct MmArgs {
   tg::Operand a, b;
@@ -263,7 +505,7 @@ struct MmArgs {
 };
 
 template <class S, int KA, int KB>
-__global__ __launch_bounds__(S::THREADS, 2) void mm_kernel(MmArgs p, int tm, int tn) {
+__global__ __launch_bounds__(S::WG_THREADS, 2) void mm_kernel(MmArgs p, int tm, int tn) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int im, in;
   tg::tile_of(blockIdx.x, tm, tn, im, in);
@@ -273,13 +515,14 @@ __global__ __launch_bounds__(S::THREADS, 2) void mm_kernel(MmArgs p, int tm, int
   tg::clear<S>(acc);
   tg::run<S, KA, KB>(p.a, p.b, m0, n0, k0, nk, smem, acc);
   const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
-  const int wave = (int)threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+  const int wm = S::wave() / S::WN, wn = S::wave() % S::WN;
 #pragma unroll
   for (int x = 0; x < S::MT; ++x) {
     const int m = m0 + (wm * S::MT + x) * 16 + l16;
     if (m >= p.M) continue;
 #pragma unroll
     for (int y = 0; y < S::NT; ++y) {
+      if (!S::owns(x, y)) continue;
       const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4;
       f32x4 v = acc[x][y];
       if (p.out_bf16) {
@@ -301,15 +544,40 @@ __global__ __launch_bounds__(S::THREADS, 2) void mm_kernel(MmArgs p, int tm, int
   }
 }
 
-// out[r][c] = sum over slabs of src[s][r][c]; src rows have ld elements
-__global__ __launch_bounds__(256) void sum_kernel(const float* src, int64_t slab, int n_slabs, int rows, int cols, int64_t ld, void* out, int out_bf16) {
-  const int64_t total = (int64_t)rows * cols;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / cols, c = i - r * cols;
+// out[r][c] = sum over slabs of src[slab][r][c], up to three such sums in a launch.  `spread` threads share an output's slabs (few outputs of
+// many slabs would leave the card to a chain of loads) and add up in a fixed order.
+struct SumJob {
+  const float* src;
+  void* out;
+  int64_t slab, ld, total;   // ld: src's row pitch; total = rows * cols
+  int n_slabs, cols, out_bf16, spread, blocks;
+};
+struct SumJobs { SumJob j[3]; };
+__global__ __launch_bounds__(256) void sum_kernel(SumJobs jobs) {
+  __shared__ float share[256];
+  int b = blockIdx.x, k = 0;
+  while (k < 2 && b >= jobs.j[k].blocks) b -= jobs.j[k++].blocks;
+  const SumJob& p = jobs.j[k];
+  const int per = 256 / p.spread, o = threadIdx.x % per, g = threadIdx.x / per;
+  for (int64_t i0 = (int64_t)b * per; i0 < p.total; i0 += (int64_t)p.blocks * per) {
+    const int64_t i = i0 + o;
     float s = 0.f;
-    for (int k = 0; k < n_slabs; ++k) s += src[k * slab + r * ld + c];
-    if (out_bf16) reinterpret_cast<bf16_t*>(out)[i] = f2bf(s);
-    else reinterpret_cast<float*>(out)[i] = s;
+    if (i < p.total) {
+      const int64_t r = i / p.cols;
+      const float* src = p.src + r * p.ld + (i - r * p.cols);
+      for (int k2 = g; k2 < p.n_slabs; k2 += p.spread) s += src[k2 * p.slab];
+    }
+    if (p.spread > 1) {
+      __syncthreads();
+      share[threadIdx.x] = s;
+      __syncthreads();
+      if (g == 0)
+        for (int q = 1; q < p.spread; ++q) s += share[q * per + o];
+    }
+    if (g == 0 && i < p.total) {
+      if (p.out_bf16) reinterpret_cast<bf16_t*>(p.out)[i] = f2bf(s);
+      else reinterpret_cast<float*>(p.out)[i] = s;
+    }
   }
 }
 
@@ -318,25 +586,48 @@ __global__ __launch_bounds__(256) void fill_kernel(float* p, int64_t n, float v)
 }
 
 // ---------------------------------------------------------------------------------------------------------- host side
+// Tile shapes by planes: L, M, S for the kernels that reduce over a tile's rows, and for the products P (S with two groups over K).
 template <int PL> struct Shapes;
 template <> struct Shapes<1> {
   typedef tg::Shape<256, 256, 2, 4, 1, 2> L;
   typedef tg::Shape<128, 128, 2, 2, 1, 2> M;
   typedef tg::Shape<64, 64, 2, 2, 1, 4> S;
+  typedef tg::Shape<64, 64, 2, 2, 1, 2, 2> P;
 };
 template <> struct Shapes<3> {
   typedef tg::Shape<256, 128, 4, 2, 3, 2> L;
   typedef tg::Shape<128, 128, 2, 4, 3, 2> M;
   typedef tg::Shape<64, 64, 2, 2, 3, 2> S;
+  typedef tg::Shape<64, 64, 2, 2, 3, 2, 2> P;
 };
+int config_bn(int PL, int c) { return PL == 1 ? (c == 2 ? 256 : c == 1 ? 128 : 64) : (c ? 128 : 64); }
+int config_bm(int PL, int c) { return c == 2 ? 256 : c == 1 ? 128 : 64; }
 
 inline int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
 
 // the largest tile that still gives most of the CUs one
-template <int PL>
-int pick(int64_t M, int64_t N) {
-  if (tiles(M, N, Shapes<PL>::L::BM, Shapes<PL>::L::BN) >= 160) return 2;
-  return tiles(M, N, Shapes<PL>::M::BM, Shapes<PL>::M::BN) >= 160 ? 1 : 0;
+int pick(int PL, int64_t M, int64_t N) {
+  for (int c = 2; c > 0; --c)
+    if (tiles(M, N, config_bm(PL, c), config_bn(PL, c)) >= 160) return c;
+  return 0;
+}
+
+// A product's tile shape and the slabs its K is cut into: the least of rounds of the 256 CUs x (fixed + steps x step), and the slabs' sum at
+// 4 TB/s.  Costs of one tile in us, measured at 8192 x 2048 x 8192 (one plane) and x 2048 (three).
+struct Cut { int shape, splits; };
+Cut cut_for(int PL, int64_t M, int64_t N, int64_t nk) {
+  static const double step[2][3] = {{0.15, 0.50, 1.45}, {0.55, 1.16, 2.1}}, fixed[3] = {3.5, 5., 10.};
+  static const int cuts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  Cut best = {0, 1};
+  double least = 1e300;
+  for (int c = 0; c < 3; ++c)
+    for (int s : cuts) {
+      if (s > 1 && nk / s < 2) break;
+      const int64_t n = tiles(M, N, config_bm(PL, c), config_bn(PL, c)) * s;
+      const double t = (double)((n + 255) / 256) * (fixed[c] + (double)((nk + s - 1) / s) * step[PL == 3][c]) + (s > 1 ? 3. + (double)s * M * N * 8. / 4e6 : 0.);
+      if (t < least) { least = t; best = {c, s}; }
+    }
+  return best;
 }
 
 template <typename K>
@@ -350,25 +641,12 @@ struct Plan {
   int PL, n_kstep, h_pad;                    // h_pad: features padded for a K step
   bool h_direct, w_direct;
   int64_t rows_pad;                          // tokens padded
-  int64_t chunk, tn;                         // forward: tokens per chunk, tile columns
+  int64_t chunk;                             // forward: tokens per chunk
   int64_t piece, piece_pad, n_pieces;        // backward: classes
-  int h_splits, w_splits;                    // K splits of the two products
-  size_t off_h, off_w, off_part, off_at, off_d, off_acc, off_wacc, off_cs, bytes;
+  Cut h_cut, w_cut;                          // the two products
+  bool head, turned;                         // at most 64 classes; the features also transposed
+  size_t off_h, off_w, off_t, off_part, off_at, off_d, off_acc, off_wacc, off_cs, bytes;
 };
-
-int config_bn(int PL, int c) { return PL == 1 ? (c == 2 ? 256 : c == 1 ? 128 : 64) : (c ? 128 : 64); }
-int config_bm(int PL, int c) { return c == 2 ? 256 : c == 1 ? 128 : 64; }
-int pick_pl(int PL, int64_t M, int64_t N) { return PL == 1 ? pick<1>(M, N) : pick<3>(M, N); }
-
-// enough slabs of K to give every CU work, at least four steps each
-int splits_for(int PL, int64_t M, int64_t N, int64_t nk) {
-  const int c = pick_pl(PL, M, N);
-  const int64_t t = tiles(M, N, config_bm(PL, c), config_bn(PL, c));
-  int64_t s = 384 / t;
-  if (s > nk / 4) s = nk / 4;
-  if (s > 64) s = 64;
-  return s < 1 ? 1 : (int)s;
-}
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -380,26 +658,28 @@ Plan make_plan(const sgpo_linear_ce_args* a, bool backward) {
   q.h_pad = (int)round_up(a->H, 64);
   q.n_kstep = q.h_pad / kstep;
   const bool whole = bf && a->H % 64 == 0;
+  q.head = a->V <= 64;
+  q.turned = backward && bf && !q.head;      // both operands of dweight read by rows of k would be 1110 TFLOP/s, one of them 1440
   q.w_direct = whole && a->ld_weight % 8 == 0 && aligned16(a->weight);
-  q.h_direct = !backward && whole && a->ld_hidden % 8 == 0 && aligned16(a->hidden);
+  // a product that reads the features by k (dweight's) needs zeros for ignored tokens: a packed copy, unless the transposed one has them
+  q.h_direct = (!backward || q.turned) && whole && a->ld_hidden % 8 == 0 && aligned16(a->hidden);
+  if (q.head && !backward) q.w_direct = q.h_direct = true;
   q.rows_pad = round_up(a->N, 64);
   size_t at = 0;
   auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t)255; return o; };
   q.off_h = take(q.h_direct ? 0 : (size_t)q.rows_pad * q.h_pad * q.PL * 2);
   q.off_w = take(q.w_direct ? 0 : (size_t)a->V * q.h_pad * q.PL * 2);
+  q.off_t = take(q.turned ? (size_t)q.rows_pad * q.h_pad * 2 : 0);
   if (!backward) {
+    if (q.head) return q;
     const int64_t tn_max = (a->V + 63) / 64;
     q.chunk = ((int64_t)1 << 24) / tn_max & ~(int64_t)255;
     if (q.chunk < 4096) q.chunk = 4096;
     if (q.chunk > a->N) q.chunk = a->N;
-    const int c = pick_pl(q.PL, q.chunk, a->V);
-    q.tn = (a->V + config_bn(q.PL, c) - 1) / config_bn(q.PL, c);
-    // the last, shorter chunk may take smaller tiles: room for their columns
-    const int64_t rest = a->N % q.chunk;
-    size_t part = (size_t)q.tn * q.chunk * 8;
-    if (rest) {
-      const int c2 = pick_pl(q.PL, rest, a->V);
-      const size_t p2 = (size_t)((a->V + config_bn(q.PL, c2) - 1) / config_bn(q.PL, c2)) * rest * 8;
+    auto columns = [&](int64_t n) { const int bn = config_bn(q.PL, pick(q.PL, n, a->V)); return (a->V + bn - 1) / bn; };
+    size_t part = (size_t)columns(q.chunk) * q.chunk * 8;
+    if (const int64_t rest = a->N % q.chunk) {   // the last, shorter chunk may take smaller tiles
+      const size_t p2 = (size_t)columns(rest) * rest * 8;
       if (p2 > part) part = p2;
     }
     q.off_part = take(part);
@@ -412,13 +692,13 @@ Plan make_plan(const sgpo_linear_ce_args* a, bool backward) {
     q.piece_pad = round_up(piece, 64);
     q.n_pieces = (a->V + piece - 1) / piece;
     q.off_d = take((size_t)q.rows_pad * q.piece_pad * q.PL * 2);
-    q.h_splits = splits_for(q.PL, a->N, a->H, q.piece_pad / kstep);
-    q.w_splits = splits_for(q.PL, piece, a->H, q.rows_pad / kstep);
-    q.off_acc = take(q.h_splits > 1 || q.n_pieces > 1 ? (size_t)q.h_splits * a->N * round_up(a->H, 4) * 4 : 0);
-    q.off_wacc = take(q.w_splits > 1 ? (size_t)q.w_splits * piece * round_up(a->H, 4) * 4 : 0);
-    const int c = pick_pl(q.PL, a->N, piece);
-    int bm = config_bm(q.PL, c);
-    if (a->V % piece) { const int b2 = config_bm(q.PL, pick_pl(q.PL, a->N, a->V % piece)); if (b2 < bm) bm = b2; }
+    q.h_cut = cut_for(q.PL, a->N, a->H, q.piece_pad / kstep);
+    q.w_cut = cut_for(q.PL, piece, a->H, q.rows_pad / kstep);
+    q.off_acc = take(q.h_cut.splits > 1 || q.n_pieces > 1 ? (size_t)q.h_cut.splits * a->N * round_up(a->H, 4) * 4 : 0);
+    q.off_wacc = take(q.w_cut.splits > 1 ? (size_t)q.w_cut.splits * piece * round_up(a->H, 4) * 4 : 0);
+    int bm = config_bm(q.PL, pick(q.PL, a->N, piece));
+    if (a->V % piece) { const int b2 = config_bm(q.PL, pick(q.PL, a->N, a->V % piece)); if (b2 < bm) bm = b2; }
+    if (q.head) bm = 16;
     q.off_cs = take((size_t)((a->N + bm - 1) / bm) * piece * 4);
   }
   q.bytes = at;
@@ -462,8 +742,43 @@ int pack(const void* src, int64_t ld, int rows, int cols, bf16_t* dst, int64_t r
     if (!done) { const int rc_ = allow_lds(kernel, bytes); if (rc_) return rc_; done = true; } \
   } while (0)
 
+template <typename T, bool GRAD>
+int head(const HeadArgs& p, hipStream_t st) {
+  // few tokens: four waves to 16 of them
+  const bool share = p.N <= 8192;
+  const int rows = share ? 16 : 64;
+  const dim3 grid((unsigned)(((GRAD ? (int64_t)p.rows_pad : (int64_t)p.N) + rows - 1) / rows));
+#define HEAD(NB)                                                                                                       \
+  case NB:                                                                                                             \
+    if (share) hipLaunchKernelGGL((head_kernel<T, NB, 4, GRAD>), grid, dim3(256), 0, st, p);                           \
+    else hipLaunchKernelGGL((head_kernel<T, NB, 1, GRAD>), grid, dim3(256), 0, st, p);                                 \
+    break;
+  switch ((p.V + 15) / 16) { HEAD(1) HEAD(2) HEAD(3) HEAD(4) }
+#undef HEAD
+  SGPO_CHECK_HIP(hipGetLastError());
+  return SGPO_OK;
+}
+HeadArgs head_args(const sgpo_linear_ce_args* a, const Plan& q) {
+  HeadArgs p = {};
+  const int n = 16 / (q.PL == 1 ? 2 : 4);
+  p.h = a->hidden; p.w = a->weight; p.ldh = a->ld_hidden; p.ldw = a->ld_weight; p.bias = a->bias; p.targets = a->targets; p.ignore = a->ignore_index;
+  p.N = a->N; p.H = a->H; p.V = a->V;
+  p.vec = a->H % 8 == 0 && a->ld_hidden % n == 0 && a->ld_weight % n == 0 && aligned16(a->hidden) && aligned16(a->weight);
+  return p;
+}
+
 template <int PL>
 int forward(const sgpo_linear_ce_args* a, const Plan& q, float* nll, float* lse, float* loss, float* inv, char* ws, hipStream_t st) {
+  if (q.head) {
+    HeadArgs p = head_args(a, q);
+    p.nll = nll; p.lse = lse;
+    const int rc = PL == 1 ? head<bf16_t, false>(p, st) : head<float, false>(p, st);
+    if (rc) return rc;
+    if (a->reduction != SGPO_REDUCE_NONE)
+      hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, nll, a->targets, a->ignore_index, a->N, a->reduction == SGPO_REDUCE_MEAN, loss, inv);
+    SGPO_CHECK_HIP(hipGetLastError());
+    return SGPO_OK;
+  }
   tg::Operand h{(const bf16_t*)a->hidden, a->ld_hidden, a->N, 0}, w{(const bf16_t*)a->weight, a->ld_weight, a->V, 0};
   int rc;
   if (!q.h_direct) {
@@ -482,13 +797,13 @@ int forward(const sgpo_linear_ce_args* a, const Plan& q, float* nll, float* lse,
     const int n = (int)(a->N - r0 < q.chunk ? a->N - r0 : q.chunk);
     LossArgs p{{h.p + r0 * h.ld, h.ld, n, 0}, w, a->bias, a->targets, a->ignore_index, (int)r0, n, 0, a->V, q.n_kstep};
     int tn = 0;
-    FOR_SHAPE(PL, pick<PL>(n, a->V), {
+    FOR_SHAPE(PL, pick(PL, n, a->V), {
       const int tm = (n + S::BM - 1) / S::BM;
       tn = (a->V + S::BN - 1) / S::BN;
       ALLOW((lse_kernel<S>), S::LDS);
       hipLaunchKernelGGL((lse_kernel<S>), dim3((unsigned)tm * tn), dim3(S::THREADS), S::LDS, st, p, tm, tn, part, at);
     })
-    hipLaunchKernelGGL(finish_kernel, dim3((n + 63) / 64), dim3(256), 0, st, part, n, tn, at, a->targets + r0, a->ignore_index, a->V, nll + r0, lse + r0);
+    hipLaunchKernelGGL(finish_kernel, dim3((n + 15) / 16), dim3(256), 0, st, part, n, tn, at, a->targets + r0, a->ignore_index, a->V, nll + r0, lse + r0);
   }
   if (a->reduction != SGPO_REDUCE_NONE)
     hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, nll, a->targets, a->ignore_index, a->N, a->reduction == SGPO_REDUCE_MEAN, loss, inv);
@@ -497,72 +812,109 @@ int forward(const sgpo_linear_ce_args* a, const Plan& q, float* nll, float* lse,
 }
 
 template <int PL, int KA, int KB>
-int product(MmArgs p, int splits, hipStream_t st) {
+int product(MmArgs p, int shape, int splits, hipStream_t st) {
   p.nk_split = (p.nk + splits - 1) / splits;
   const int used = (p.nk + p.nk_split - 1) / p.nk_split;
-  FOR_SHAPE(PL, pick<PL>(p.M, p.N), {
-    const int tm = (p.M + S::BM - 1) / S::BM, tn = (p.N + S::BN - 1) / S::BN;
-    ALLOW((mm_kernel<S, KA, KB>), S::LDS);
-    hipLaunchKernelGGL((mm_kernel<S, KA, KB>), dim3((unsigned)tm * tn, used), dim3(S::THREADS), S::LDS, st, p, tm, tn);
-  })
+#define PRODUCT(K)                                                                                                                            \
+  {                                                                                                                                           \
+    typedef typename Shapes<PL>::K S;                                                                                                         \
+    const int tm = (p.M + S::BM - 1) / S::BM, tn = (p.N + S::BN - 1) / S::BN;                                                                 \
+    ALLOW((mm_kernel<S, KA, KB>), S::LDS);                                                                                                    \
+    hipLaunchKernelGGL((mm_kernel<S, KA, KB>), dim3((unsigned)tm * tn, used), dim3(S::WG_THREADS), S::LDS, st, p, tm, tn);                    \
+  }
+  if (shape == 2) PRODUCT(L) else if (shape == 1) PRODUCT(M) else PRODUCT(P)
+#undef PRODUCT
   SGPO_CHECK_HIP(hipGetLastError());
   return used;
 }
+
+struct Sums {
+  SumJobs jobs = {};
+  int n = 0;
+  void add(const float* src, int64_t slab, int n_slabs, int64_t rows, int cols, int64_t ld, void* out, int out_bf16) {
+    const int64_t total = rows * cols;
+    const int spread = total >= 65536 || n_slabs < 8 ? 1 : n_slabs < 64 ? 8 : 32;
+    const int64_t blocks = (total * spread + 255) / 256;
+    jobs.j[n++] = SumJob{src, out, slab, ld, total, n_slabs, cols, out_bf16, spread, (int)(blocks < 8192 ? blocks : 8192)};
+  }
+  void run(hipStream_t st) {
+    int blocks = 0;
+    for (int i = 0; i < n; ++i) blocks += jobs.j[i].blocks;
+    if (blocks) hipLaunchKernelGGL(sum_kernel, dim3(blocks), dim3(256), 0, st, jobs);
+    *this = Sums();
+  }
+};
 
 template <int PL>
 int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, const float* g, const float* inv, void* dh, void* dw, float* db, char* ws, hipStream_t st) {
   const bool bf = PL == 1;
   const int kstep = bf ? 64 : 32, esz = bf ? 2 : 4;
   int rc;
-  bf16_t* hp = (bf16_t*)(ws + q.off_h);
-  if ((rc = pack<PL>(a->hidden, a->ld_hidden, a->N, a->H, hp, q.rows_pad, q.h_pad, a->targets, a->ignore_index, st))) return rc;
-  tg::Operand h{hp, (int64_t)q.h_pad * PL, a->N, 0}, w{(const bf16_t*)a->weight, a->ld_weight, a->V, 0};
-  if (!q.w_direct) {
-    bf16_t* d = (bf16_t*)(ws + q.off_w);
-    if ((rc = pack<PL>(a->weight, a->ld_weight, a->V, a->H, d, a->V, q.h_pad, nullptr, 0, st))) return rc;
-    w.p = d; w.ld = (int64_t)q.h_pad * PL;
+  bf16_t *hp = (bf16_t*)(ws + q.off_h), *ht = (bf16_t*)(ws + q.off_t), *d = (bf16_t*)(ws + q.off_d);
+  tg::Operand h{(const bf16_t*)a->hidden, a->ld_hidden, a->N, 0}, w{(const bf16_t*)a->weight, a->ld_weight, a->V, 0};
+  if (!q.h_direct) {
+    if (!q.head && (rc = pack<PL>(a->hidden, a->ld_hidden, a->N, a->H, hp, q.rows_pad, q.h_pad, a->targets, a->ignore_index, st))) return rc;
+    h.p = hp; h.ld = (int64_t)q.h_pad * PL;
   }
-  bf16_t* d = (bf16_t*)(ws + q.off_d);
-  float* acc = (float*)(ws + q.off_acc);
-  float* wacc = (float*)(ws + q.off_wacc);
-  float* cs = (float*)(ws + q.off_cs);
+  if (q.turned && dw) {
+    SGPO_REQUIRE(q.h_pad / 64 <= 65535, "linear_ce_backward: H=%d", a->H);
+    hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)(q.rows_pad / 64), q.h_pad / 64), dim3(256), 0, st, (const bf16_t*)a->hidden, a->ld_hidden, a->N, a->H, ht, q.rows_pad,
+                       a->targets, a->ignore_index);
+  }
+  if (!q.w_direct && (dh || !q.head)) {
+    bf16_t* p = (bf16_t*)(ws + q.off_w);
+    if ((rc = pack<PL>(a->weight, a->ld_weight, a->V, a->H, p, a->V, q.h_pad, nullptr, 0, st))) return rc;
+    w.p = p; w.ld = (int64_t)q.h_pad * PL;
+  }
+  float *acc = (float*)(ws + q.off_acc), *wacc = (float*)(ws + q.off_wacc), *cs = (float*)(ws + q.off_cs);
   const int64_t ldf = round_up(a->H, 4);
-  const bool via = q.h_splits > 1 || q.n_pieces > 1;
+  const bool via = q.h_cut.splits > 1 || q.n_pieces > 1;
   int h_used = 1;
+  Sums sums;
   for (int64_t v0 = 0; v0 < a->V; v0 += q.piece) {
     const int nc = (int)(a->V - v0 < q.piece ? a->V - v0 : q.piece);
     const int nc_pad = (int)round_up(nc, 64);
-    LossArgs p{h, {w.p + v0 * w.ld, w.ld, (int)(a->V - v0), 0}, a->bias, a->targets, a->ignore_index, 0, a->N, (int)v0, nc, q.n_kstep};
-    int tm = 0;
-    FOR_SHAPE(PL, pick<PL>(a->N, nc), {
-      tm = (a->N + S::BM - 1) / S::BM;
-      const int tn = (nc + S::BN - 1) / S::BN;
-      ALLOW((grad_kernel<S>), S::LDS);
-      hipLaunchKernelGGL((grad_kernel<S>), dim3((unsigned)tm * tn), dim3(S::THREADS), S::LDS, st, p, tm, tn, lse, g, a->reduction == SGPO_REDUCE_NONE, inv, d,
-                         (int)q.rows_pad, nc_pad, db ? cs : nullptr);
-    })
-    if (db) hipLaunchKernelGGL(sum_kernel, dim3(blocks_for(nc)), dim3(256), 0, st, cs, (int64_t)nc, tm, 1, nc, (int64_t)nc, db + v0, 0);
+    int parts = 0;
+    if (q.head) {
+      HeadArgs p = head_args(a, q);
+      p.lse = const_cast<float*>(lse); p.g = g; p.g_rows = a->reduction == SGPO_REDUCE_NONE; p.inv = inv;
+      p.rows_pad = (int)q.rows_pad; p.h_pad = q.h_pad; p.d = d; p.hp = dw ? hp : nullptr; p.col_sums = db ? cs : nullptr;
+      if ((rc = PL == 1 ? head<bf16_t, true>(p, st) : head<float, true>(p, st))) return rc;
+      parts = (int)(a->N <= 8192 ? (a->N + 15) / 16 : (a->N + 63) / 64);
+    } else {
+      LossArgs p{h, {w.p + v0 * w.ld, w.ld, (int)(a->V - v0), 0}, a->bias, a->targets, a->ignore_index, 0, a->N, (int)v0, nc, q.n_kstep};
+      FOR_SHAPE(PL, pick(PL, a->N, nc), {
+        parts = (a->N + S::BM - 1) / S::BM;
+        const int tn = (nc + S::BN - 1) / S::BN;
+        ALLOW((grad_kernel<S>), S::LDS);
+        hipLaunchKernelGGL((grad_kernel<S>), dim3((unsigned)parts * tn), dim3(S::THREADS), S::LDS, st, p, parts, tn, lse, g, a->reduction == SGPO_REDUCE_NONE, inv, d,
+                           (int)q.rows_pad, nc_pad, db ? cs : nullptr);
+      })
+    }
+    if (db) sums.add(cs, nc, parts, 1, nc, nc, db + v0, 0);
     if (dh) {
       // the first piece decides how many slabs there are; later ones add to them
       MmArgs m{{d, (int64_t)nc_pad * PL, a->N, 0}, {w.p + v0 * w.ld, w.ld, nc, q.h_pad * PL}, a->N, a->H, nc_pad / kstep, 0,
                via ? (void*)acc : dh, via ? ldf : a->H, via ? (int64_t)a->N * ldf : 0, !via && bf, v0 > 0,
                via || (a->H % 4 == 0 && aligned16(dh))};
-      const int used = product<PL, tg::KC, tg::KM>(m, v0 == 0 ? q.h_splits : h_used, st);
+      const int used = product<PL, tg::KC, tg::KM>(m, q.h_cut.shape, v0 == 0 ? q.h_cut.splits : h_used, st);
       if (used < 0) return used;
       if (v0 == 0) h_used = used;
+      if (via && v0 + nc == a->V) sums.add(acc, (int64_t)a->N * ldf, h_used, a->N, a->H, ldf, dh, bf);
     }
     if (dw) {
-      const bool slabs = q.w_splits > 1;
+      const bool slabs = q.w_cut.splits > 1;
       void* out = (char*)dw + v0 * a->H * esz;
       MmArgs m{{d, (int64_t)nc_pad * PL, (int)q.rows_pad, nc_pad * PL}, {hp, (int64_t)q.h_pad * PL, (int)q.rows_pad, q.h_pad * PL}, nc, a->H, (int)(q.rows_pad / kstep), 0,
                slabs ? (void*)wacc : out, slabs ? ldf : a->H, slabs ? (int64_t)nc * ldf : 0, !slabs && bf, 0,
                slabs || (a->H % 4 == 0 && aligned16(out))};
-      const int used = product<PL, tg::KM, tg::KM>(m, q.w_splits, st);
+      if (q.turned) m.b = tg::Operand{ht, q.rows_pad, q.h_pad, 0};
+      const int used = q.turned ? product<PL, tg::KM, tg::KC>(m, q.w_cut.shape, q.w_cut.splits, st) : product<PL, tg::KM, tg::KM>(m, q.w_cut.shape, q.w_cut.splits, st);
       if (used < 0) return used;
-      if (slabs) hipLaunchKernelGGL(sum_kernel, dim3(blocks_for((int64_t)nc * a->H)), dim3(256), 0, st, wacc, (int64_t)nc * ldf, used, nc, a->H, ldf, out, bf ? 1 : 0);
+      if (slabs) sums.add(wacc, (int64_t)nc * ldf, used, nc, a->H, ldf, out, bf);
     }
+    sums.run(st);
   }
-  if (dh && via) hipLaunchKernelGGL(sum_kernel, dim3(blocks_for((int64_t)a->N * a->H)), dim3(256), 0, st, acc, (int64_t)a->N * ldf, h_used, a->N, a->H, ldf, dh, bf ? 1 : 0);
   SGPO_CHECK_HIP(hipGetLastError());
   return SGPO_OK;
 }
@@ -585,9 +937,9 @@ extern "C" int sgpo_linear_ce_forward(const sgpo_linear_ce_args* a, float* nll, 
     SGPO_CHECK_HIP(hipGetLastError());
     return SGPO_OK;
   }
-  SGPO_REQUIRE(a->hidden && a->weight && a->targets && nll && lse && workspace, "linear_ce_forward: null argument");
+  SGPO_REQUIRE(a->hidden && a->weight && a->targets && nll && lse, "linear_ce_forward: null argument");
   const Plan q = make_plan(a, false);
-  if (workspace_bytes < q.bytes) { sgpo_set_error("linear_ce_forward: workspace %zu < %zu", workspace_bytes, q.bytes); return SGPO_ERR_WORKSPACE; }
+  if (q.bytes && (!workspace || workspace_bytes < q.bytes)) { sgpo_set_error("linear_ce_forward: workspace %zu < %zu", workspace_bytes, q.bytes); return SGPO_ERR_WORKSPACE; }
   return q.PL == 1 ? forward<1>(a, q, nll, lse, loss, inv_count, (char*)workspace, st) : forward<3>(a, q, nll, lse, loss, inv_count, (char*)workspace, st);
 }
 
@@ -601,7 +953,7 @@ extern "C" int sgpo_linear_ce_backward(const sgpo_linear_ce_args* a, const float
     if (dweight) {
       if (words) hipLaunchKernelGGL(fill_kernel, dim3(blocks_for(words)), dim3(256), 0, st, (float*)dweight, words, 0.f);
       if (a->dtype == SGPO_DTYPE_BF16 && odd)
-        hipLaunchKernelGGL(sum_kernel, dim3(1), dim3(256), 0, st, (const float*)nullptr, (int64_t)0, 0, 1, 1, (int64_t)1, (bf16_t*)dweight + words * 2, 1);
+        { Sums one; one.add(nullptr, 0, 0, 1, 1, 1, (bf16_t*)dweight + words * 2, 1); one.run(st); }
     }
     if (dbias) hipLaunchKernelGGL(fill_kernel, dim3(blocks_for(a->V)), dim3(256), 0, st, dbias, (int64_t)a->V, 0.f);
     SGPO_CHECK_HIP(hipGetLastError());
