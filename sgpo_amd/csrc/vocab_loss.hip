@@ -10,8 +10,9 @@
 // that read it -- d as rows (dhidden) and d as columns (dweight) come from the same buffer (tile_gemm.h, KC and KM).
 // 2 N V H operations forward and 6 backward; everything but the operands and gradients stays in caches or registers.
 //
-// bf16 operands: one plane; d is rounded to bf16 once (relative error 2^-8 at most per term, of the size of the outputs' own
-// rounding), sums in fp32.  fp32 operands: three planes, i.e. products and d with 24 bits.
+// bf16 operands: one plane; d is rounded to bf16 once (2^-8 of a term at most, of the size of the outputs' own rounding), sums in
+// fp32.  A factor common to all tokens (mean, sum) is left out of d and applied to the products' sums: rounded into d it would be off
+// by the same up to 2^-8 everywhere, while p - 1 of an unlikely target is -1 almost exactly.  fp32 operands: three planes, i.e. products and d with 24 bits.
 // Sums over tokens and classes run in a fixed order: the same inputs give the same bits.
 #include "../../include/sgpo_hip.h"
 #include "tile_gemm.h"
@@ -223,10 +224,16 @@ __global__ __launch_bounds__(1024) void total_kernel(const float* nll, const int
 }
 
 // ----------------------------------------------------------------------------------------------------------- backward
-// d of a piece of the vocabulary into d [rows_pad][cols_pad] planes (zero beyond the tokens and classes); column sums per row tile
+// The factor common to all tokens' gradients; 1 where each has its own.
+struct Factor {
+  const float *g, *inv;   // null: 1
+  __device__ __forceinline__ float get() const { return g ? g[0] * (inv ? inv[0] : 1.f) : 1.f; }
+};
+
+// d (without the common factor) of a piece of the vocabulary into d [rows_pad][cols_pad] planes (zero beyond the tokens and classes); column sums per row tile
 template <class S>
 __global__ __launch_bounds__(S::THREADS, 2) void grad_kernel(LossArgs p, int tm, int tn, const float* lse, const float* g,
-                                                               int g_rows, const float* inv, bf16_t* d, int rows_pad, int cols_pad,
+                                                               int g_rows, bf16_t* d, int rows_pad, int cols_pad,
                                                                float* col_sums) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int im, in;
@@ -236,7 +243,6 @@ __global__ __launch_bounds__(S::THREADS, 2) void grad_kernel(LossArgs p, int tm,
   logits<S>(p, m0, n0, smem, acc);
   const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
   const int wave = (int)threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-  const float f = inv ? inv[0] : 1.f;
   float cs[S::NT][4];
 #pragma unroll
   for (int y = 0; y < S::NT; ++y)
@@ -259,7 +265,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void grad_kernel(LossArgs p, int tm,
       const bool keep = in_rows && t != p.ignore;
       const bool bad = keep && (t < 0 || t >= (int64_t)p.w.rows + p.v0);
       const float l = keep ? lse[m] : 0.f;
-      const float gm = keep ? (bad ? __builtin_nanf("") : g[g_rows ? m : 0] * f) : 0.f;
+      const float gm = keep ? (bad ? __builtin_nanf("") : g_rows ? g[m] : 1.f) : 0.f;
       const int64_t tw = t - p.v0 - nb - 4 * l4;
       const int tq = tw >= 0 && tw < S::NT * 16 ? (int)tw : -1;   // 16 y + q, if the class lies with this lane
 #pragma unroll
@@ -329,7 +335,7 @@ struct HeadArgs {
   int64_t ignore;
   int N, H, V, vec;          // vec: rows may be read 16 bytes at a time
   float *nll, *lse;          // forward's outputs; GRAD reads lse
-  const float *g, *inv;
+  const float* g;            // [N], or not read (g_rows 0)
   int g_rows, rows_pad, h_pad;
   bf16_t *d, *hp;            // [rows_pad][64], [rows_pad][h_pad] planes
   float* col_sums;           // [workgroup][V], or null
@@ -461,7 +467,7 @@ __global__ __launch_bounds__(256) void head_kernel(HeadArgs p) {
     if (l4 == 0 && m < p.N) store_loss(top + logf(sum), at, t, p.ignore, p.V, p.nll + m, p.lse + m);
   } else {
     const float l = keep ? p.lse[m] : 0.f;
-    const float gm = keep ? (cls ? p.g[p.g_rows ? m : 0] * (p.inv ? p.inv[0] : 1.f) : __builtin_nanf("")) : 0.f;
+    const float gm = keep ? (cls ? (p.g_rows ? p.g[m] : 1.f) : __builtin_nanf("")) : 0.f;
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const int n = y * 16 + 4 * l4;
@@ -501,6 +507,7 @@ struct MmArgs {
   int M, N, nk, nk_split;
   void* out;
   int64_t ldo, slab;
+  Factor factor;            // on the sums
   int out_bf16, add, vec;   // vec: rows start 16-B (fp32) / 8-B (bf16) aligned
 };
 
@@ -516,6 +523,7 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void mm_kernel(MmArgs p, int tm, 
   tg::run<S, KA, KB>(p.a, p.b, m0, n0, k0, nk, smem, acc);
   const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
   const int wm = S::wave() / S::WN, wn = S::wave() % S::WN;
+  const float factor = p.factor.get();
 #pragma unroll
   for (int x = 0; x < S::MT; ++x) {
     const int m = m0 + (wm * S::MT + x) * 16 + l16;
@@ -524,7 +532,7 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void mm_kernel(MmArgs p, int tm, 
     for (int y = 0; y < S::NT; ++y) {
       if (!S::owns(x, y)) continue;
       const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4;
-      f32x4 v = acc[x][y];
+      f32x4 v = acc[x][y] * factor;
       if (p.out_bf16) {
         bf16_t* o = reinterpret_cast<bf16_t*>(p.out) + m * p.ldo + n;
         if (p.vec && n + 4 <= p.N) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
@@ -551,6 +559,7 @@ struct SumJob {
   void* out;
   int64_t slab, ld, total;   // ld: src's row pitch; total = rows * cols
   int n_slabs, cols, out_bf16, spread, blocks;
+  Factor factor;
 };
 struct SumJobs { SumJob j[3]; };
 __global__ __launch_bounds__(256) void sum_kernel(SumJobs jobs) {
@@ -575,6 +584,7 @@ __global__ __launch_bounds__(256) void sum_kernel(SumJobs jobs) {
         for (int q = 1; q < p.spread; ++q) s += share[q * per + o];
     }
     if (g == 0 && i < p.total) {
+      s *= p.factor.get();
       if (p.out_bf16) reinterpret_cast<bf16_t*>(p.out)[i] = f2bf(s);
       else reinterpret_cast<float*>(p.out)[i] = s;
     }
@@ -831,11 +841,11 @@ int product(MmArgs p, int shape, int splits, hipStream_t st) {
 struct Sums {
   SumJobs jobs = {};
   int n = 0;
-  void add(const float* src, int64_t slab, int n_slabs, int64_t rows, int cols, int64_t ld, void* out, int out_bf16) {
+  void add(const float* src, int64_t slab, int n_slabs, int64_t rows, int cols, int64_t ld, void* out, int out_bf16, Factor factor = Factor{nullptr, nullptr}) {
     const int64_t total = rows * cols;
     const int spread = total >= 65536 || n_slabs < 8 ? 1 : n_slabs < 64 ? 8 : 32;
     const int64_t blocks = (total * spread + 255) / 256;
-    jobs.j[n++] = SumJob{src, out, slab, ld, total, n_slabs, cols, out_bf16, spread, (int)(blocks < 8192 ? blocks : 8192)};
+    jobs.j[n++] = SumJob{src, out, slab, ld, total, n_slabs, cols, out_bf16, spread, (int)(blocks < 8192 ? blocks : 8192), factor};
   }
   void run(hipStream_t st) {
     int blocks = 0;
@@ -871,13 +881,14 @@ int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, cons
   const bool via = q.h_cut.splits > 1 || q.n_pieces > 1;
   int h_used = 1;
   Sums sums;
+  const Factor factor = a->reduction == SGPO_REDUCE_NONE ? Factor{nullptr, nullptr} : Factor{g, inv};
   for (int64_t v0 = 0; v0 < a->V; v0 += q.piece) {
     const int nc = (int)(a->V - v0 < q.piece ? a->V - v0 : q.piece);
     const int nc_pad = (int)round_up(nc, 64);
     int parts = 0;
     if (q.head) {
       HeadArgs p = head_args(a, q);
-      p.lse = const_cast<float*>(lse); p.g = g; p.g_rows = a->reduction == SGPO_REDUCE_NONE; p.inv = inv;
+      p.lse = const_cast<float*>(lse); p.g = g; p.g_rows = a->reduction == SGPO_REDUCE_NONE;
       p.rows_pad = (int)q.rows_pad; p.h_pad = q.h_pad; p.d = d; p.hp = dw ? hp : nullptr; p.col_sums = db ? cs : nullptr;
       if ((rc = PL == 1 ? head<bf16_t, true>(p, st) : head<float, true>(p, st))) return rc;
       parts = (int)(a->N <= 8192 ? (a->N + 15) / 16 : (a->N + 63) / 64);
@@ -887,15 +898,15 @@ int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, cons
         parts = (a->N + S::BM - 1) / S::BM;
         const int tn = (nc + S::BN - 1) / S::BN;
         ALLOW((grad_kernel<S>), S::LDS);
-        hipLaunchKernelGGL((grad_kernel<S>), dim3((unsigned)parts * tn), dim3(S::THREADS), S::LDS, st, p, parts, tn, lse, g, a->reduction == SGPO_REDUCE_NONE, inv, d,
+        hipLaunchKernelGGL((grad_kernel<S>), dim3((unsigned)parts * tn), dim3(S::THREADS), S::LDS, st, p, parts, tn, lse, g, a->reduction == SGPO_REDUCE_NONE, d,
                            (int)q.rows_pad, nc_pad, db ? cs : nullptr);
       })
     }
-    if (db) sums.add(cs, nc, parts, 1, nc, nc, db + v0, 0);
+    if (db) sums.add(cs, nc, parts, 1, nc, nc, db + v0, 0, factor);
     if (dh) {
       // the first piece decides how many slabs there are; later ones add to them
       MmArgs m{{d, (int64_t)nc_pad * PL, a->N, 0}, {w.p + v0 * w.ld, w.ld, nc, q.h_pad * PL}, a->N, a->H, nc_pad / kstep, 0,
-               via ? (void*)acc : dh, via ? ldf : a->H, via ? (int64_t)a->N * ldf : 0, !via && bf, v0 > 0,
+               via ? (void*)acc : dh, via ? ldf : a->H, via ? (int64_t)a->N * ldf : 0, factor, !via && bf, v0 > 0,
                via || (a->H % 4 == 0 && aligned16(dh))};
       const int used = product<PL, tg::KC, tg::KM>(m, q.h_cut.shape, v0 == 0 ? q.h_cut.splits : h_used, st);
       if (used < 0) return used;
@@ -906,7 +917,7 @@ int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, cons
       const bool slabs = q.w_cut.splits > 1;
       void* out = (char*)dw + v0 * a->H * esz;
       MmArgs m{{d, (int64_t)nc_pad * PL, (int)q.rows_pad, nc_pad * PL}, {hp, (int64_t)q.h_pad * PL, (int)q.rows_pad, q.h_pad * PL}, nc, a->H, (int)(q.rows_pad / kstep), 0,
-               slabs ? (void*)wacc : out, slabs ? ldf : a->H, slabs ? (int64_t)nc * ldf : 0, !slabs && bf, 0,
+               slabs ? (void*)wacc : out, slabs ? ldf : a->H, slabs ? (int64_t)nc * ldf : 0, factor, !slabs && bf, 0,
                slabs || (a->H % 4 == 0 && aligned16(out))};
       if (q.turned) m.b = tg::Operand{ht, q.rows_pad, q.h_pad, 0};
       const int used = q.turned ? product<PL, tg::KM, tg::KC>(m, q.w_cut.shape, q.w_cut.splits, st) : product<PL, tg::KM, tg::KM>(m, q.w_cut.shape, q.w_cut.splits, st);
