@@ -30,7 +30,7 @@ struct Source {
   float momentum;
   int nesterov;
   int64_t stride_b, ld;    // of grad; buf is contiguous
-  int rows, cols;
+  int rows, cols, vec;     // vec: grad contiguous and, like buf, readable four elements at a time
 };
 
 template <typename T>
@@ -41,20 +41,48 @@ __device__ __forceinline__ float update_at(const Source& s, int b, int r, int c)
   return s.nesterov ? fmaf(s.momentum, m, g) : m;
 }
 
-// momentum buffer, and partial sums of the update's squares
+// four consecutive elements of a contiguous gradient
+template <typename T> __device__ __forceinline__ void grad4(const T* p, float (&g)[4]);
+template <> __device__ __forceinline__ void grad4<float>(const float* p, float (&g)[4]) {
+  const f32x4 v = *reinterpret_cast<const f32x4*>(p);
+  g[0] = v[0]; g[1] = v[1]; g[2] = v[2]; g[3] = v[3];
+}
+template <> __device__ __forceinline__ void grad4<bf16_t>(const bf16_t* p, float (&g)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  g[0] = bf2f(v.x & 0xffff); g[1] = bf2f(v.x >> 16); g[2] = bf2f(v.y & 0xffff); g[3] = bf2f(v.y >> 16);
+}
+
+// momentum buffer, and partial sums of the update's squares; s.vec: four elements at a time
 template <typename T>
 __global__ __launch_bounds__(256) void square_kernel(Source s, double* part) {
   const int b = blockIdx.y;
-  const int64_t total = (int64_t)s.rows * s.cols;
+  const uint32_t total = (uint32_t)s.rows * (uint32_t)s.cols;
+  const T* grad = reinterpret_cast<const T*>(s.grad) + b * s.stride_b;
+  float* buf = s.buf ? s.buf + (int64_t)b * total : nullptr;
   double sum = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int r = (int)((uint32_t)i / (uint32_t)s.cols), c = (int)((uint32_t)i - (uint32_t)r * (uint32_t)s.cols);
-    if (s.buf) {
-      float* m = s.buf + (int64_t)b * total + i;
-      *m = fmaf(s.momentum, *m, up<T>(reinterpret_cast<const T*>(s.grad)[b * s.stride_b + r * s.ld + c]));
+  if (s.vec) {
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total / 4; i += gridDim.x * 256) {
+      float g[4];
+      grad4<T>(grad + (size_t)i * 4, g);
+      if (buf) {
+        f32x4 m = *reinterpret_cast<const f32x4*>(buf + (size_t)i * 4);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          m[q] = fmaf(s.momentum, m[q], g[q]);
+          g[q] = s.nesterov ? fmaf(s.momentum, m[q], g[q]) : m[q];
+        }
+        *reinterpret_cast<f32x4*>(buf + (size_t)i * 4) = m;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sum += (double)g[q] * g[q];
     }
-    const double u = (double)update_at<T>(s, b, r, c);
-    sum += u * u;
+  } else {
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
+      const uint32_t r = i / (uint32_t)s.cols, c = i - r * (uint32_t)s.cols;
+      if (buf) buf[i] = fmaf(s.momentum, buf[i], up<T>(grad[r * s.ld + c]));
+      const double u = (double)update_at<T>(s, b, r, c);
+      sum += u * u;
+    }
   }
   __shared__ double share[4];
 #pragma unroll
@@ -82,7 +110,21 @@ __global__ __launch_bounds__(256) void load_kernel(Source s, const double* part,
     const int r = (int)(i / quads), c = (int)(i - (uint32_t)r * quads) * 4;
     float v[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = c + q < s.cols ? inv * update_at<T>(s, b, r, c + q) : 0.f;
+    for (int q = 0; q < 4; ++q) v[q] = 0.f;
+    if (s.vec && c < s.cols) {
+      const int64_t at = (int64_t)r * s.cols + c;
+      grad4<T>(reinterpret_cast<const T*>(s.grad) + b * s.stride_b + at, v);
+      if (s.buf) {
+        const f32x4 m = *reinterpret_cast<const f32x4*>(s.buf + (int64_t)b * s.rows * s.cols + at);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = s.nesterov ? fmaf(s.momentum, m[q], v[q]) : m[q];
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) if (c + q < s.cols) v[q] = update_at<T>(s, b, r, c + q);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] *= inv;
     tg::store4<2>(X + b * bstride + r * ldx, c, v);
   }
 }
@@ -110,7 +152,8 @@ __device__ __forceinline__ void triangle(int t, int tiles, int& i, int& j) {
 
 enum { WIDE = 0, TALL = 1, POLY = 2 };   // G = X X^T;  G = X^T X;  P = a I + b G + c G G
 
-// one triangle of tiles, each also written transposed
+// One triangle of tiles, each also written transposed (element by element: taking the transposed tile through LDS and out in whole lines
+// measured the same, 60 us either way for 512 x 1536 in 192 x 192 tiles)
 template <class S, int MODE>
 __global__ __launch_bounds__(S::WG_THREADS, 2) void symmetric_kernel(Mats q, int tiles, float ca, float cb, float cc) {
   static_assert(S::BM == S::BN && S::PL == 2, "square tiles of two planes");
@@ -365,23 +408,35 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void apply_kernel(Mats q, int tm,
   const bf16_t *X = q.X + b * q.sx, *P = q.P + b * q.sg;
   f32x4 acc[S::MT][S::NT];
   tg::clear<S>(acc);
-  if constexpr (TALLX) tg::run<S, tg::KC, tg::KC>(tg::Operand{X, q.ldx, q.rows, 0}, tg::Operand{P, q.ldg, q.d, 0}, m0, n0, 0, (int)(q.ldg / 64), smem, acc);   // P is symmetric
-  else tg::run<S, tg::KC, tg::KM>(tg::Operand{P, q.ldg, q.d, 0}, tg::Operand{X, q.ldx, q.d, (int)q.ldx}, m0, n0, 0, (int)(q.ldg / 64), smem, acc);
+  if constexpr (TALLX) tg::run<S, tg::KC, tg::KC, !LAST>(tg::Operand{X, q.ldx, q.rows, 0}, tg::Operand{P, q.ldg, q.d, 0}, m0, n0, 0, (int)(q.ldg / 64), smem, acc);   // P is symmetric
+  else tg::run<S, tg::KC, tg::KM, !LAST>(tg::Operand{P, q.ldg, q.d, 0}, tg::Operand{X, q.ldx, q.d, (int)q.ldx}, m0, n0, 0, (int)(q.ldg / 64), smem, acc);
   const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4, wm = S::wave() / S::WN, wn = S::wave() % S::WN;
+  const int pad = (int)(q.ldx / 2);
 #pragma unroll
   for (int x = 0; x < S::MT; ++x) {
     const int m = m0 + (wm * S::MT + x) * 16 + l16;
-    if (m >= q.rows) continue;
+    const bool row = m < q.rows;
+    float w[S::NT][4];
 #pragma unroll
     for (int y = 0; y < S::NT; ++y) {
-      if (!S::owns(x, y)) continue;
+      if (!S::template owns<!LAST>(x, y)) continue;
       const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4;
-      if (n >= q.ldx / 2) continue;
-      float v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = n + e < q.cols ? acc[x][y][e] : 0.f;
-      if constexpr (LAST) store_result(res, b, m, n, v);
-      else tg::store4<2>(q.Y + b * q.sx + m * q.ldx, n, v);
+      for (int e = 0; e < 4; ++e) w[y][e] = n + e < q.cols ? acc[x][y][e] : 0.f;
+      if (LAST && row && n < q.cols) store_result(res, b, m, n, w[y]);
+    }
+    if constexpr (!LAST) {
+      bf16_t* at = q.Y + b * q.sx + m * q.ldx;
+#pragma unroll
+      for (int y = 0; y < S::NT; y += 2) {
+        if (!S::template owns<!LAST>(x, y)) continue;
+        const int e = n0 + (wn * S::NT + y) * 16;
+        if (y + 1 < S::NT && e % 32 == 0) tg::store_pair<2>(at, e, w[y], w[y + 1 < S::NT ? y + 1 : y], l4, row && e < pad);
+        else {
+          if (row && e < pad) tg::store4<2>(at, e + 4 * l4, w[y]);
+          if (y + 1 < S::NT && row && e + 16 < pad) tg::store4<2>(at, e + 16 + 4 * l4, w[y + 1 < S::NT ? y + 1 : y]);
+        }
+      }
     }
   }
 }
@@ -415,8 +470,8 @@ int apply(const Mats& q, int batch, const Result& r, hipStream_t st) {
 // Tile shapes, and what one tile costs (us): `symmetric` and `apply` + `step` per 32 k, one workgroup on a CU, measured at 1 x 1536 x 512 and
 // 8 x 512 x 2048.  Small tiles spread a small product over the CUs and read more bytes for it; large ones the other way round.
 struct Kind { int side, per_cu; double symmetric, apply, step; };
-constexpr Kind KINDS[] = {{256, 1, 30., 18., 1.40}, {192, 1, 17., 11., 0.90}, {129, 1, 11., 8.2, 0.46}, {128, 2, 11., 5.3, 0.575},
-                          {96, 1, 8.5, 7.0, 0.276}, {64, 2, 4.5, 4.2, 0.21}, {32, 2, 3.6, 3.6, 0.08}};
+constexpr Kind KINDS[] = {{256, 1, 30., 11., 1.40}, {192, 1, 17., 9.7, 0.90}, {129, 1, 11., 6.4, 0.46}, {128, 2, 11., 3.5, 0.575},
+                          {96, 1, 8.5, 6.8, 0.276}, {64, 2, 4.5, 3.6, 0.21}, {32, 2, 3.6, 3.3, 0.08}};
 typedef tg::Shape<256, 256, 2, 4, 2, 2> Shape256;
 typedef tg::Shape<192, 192, 2, 4, 2, 2> Shape192;
 typedef tg::Shape<128, 128, 2, 2, 2, 2, 2> Shape129;   // 128 x 128 with two groups over K: one workgroup fills a CU
@@ -487,7 +542,7 @@ int orthogonalise_small(const Source& src, int batch, const float* coef, int ste
 }
 
 template <typename T>
-int orthogonalise(const Source& src, int batch, const float* coef, int steps, double eps, Result res, char* ws, hipStream_t st) {
+int orthogonalise(Source src, int batch, const float* coef, int steps, double eps, Result res, char* ws, hipStream_t st) {
   const Sizes z = sizes(batch, src.rows, src.cols);
   res.rows = src.rows; res.cols = src.cols;
   res.vec = src.cols % 4 == 0 && (uintptr_t)res.out % (res.out_bf16 ? 8 : 16) == 0;
@@ -496,8 +551,9 @@ int orthogonalise(const Source& src, int batch, const float* coef, int steps, do
   double* part = reinterpret_cast<double*>(ws);
   Mats q{(bf16_t*)(ws + z.off_x), (bf16_t*)(ws + z.off_y), (bf16_t*)(ws + z.off_g), (bf16_t*)(ws + z.off_p), z.ldx, z.ldg, (int64_t)z.x, (int64_t)z.g, src.rows, src.cols, z.d};
   const bool tall = src.rows > src.cols;
-  // about 16 elements a thread
-  const int64_t want = ((int64_t)src.rows * src.cols + 4095) / 4096;
+  src.vec = src.cols % 4 == 0 && src.ld == src.cols && src.stride_b % 4 == 0 && (uintptr_t)src.grad % (4 * sizeof(T)) == 0 && (uintptr_t)src.buf % 16 == 0;
+  // about four elements a thread
+  const int64_t want = ((int64_t)src.rows * src.cols + 1023) / 1024;
   const int parts = want < PARTS ? (int)want : PARTS;
   hipLaunchKernelGGL((square_kernel<T>), dim3(parts, batch), dim3(256), 0, st, src, part);
   const int64_t blocks = ((int64_t)src.rows * (z.ldx / 8) + 255) / 256;
@@ -545,7 +601,7 @@ extern "C" int sgpo_newton_schulz(const void* update, int dtype, int batch, int 
   SGPO_REQUIRE(ld >= cols || rows == 1, "newton_schulz: row pitch %lld below %d columns", (long long)ld, cols);
   const size_t need = sgpo_newton_schulz_workspace_bytes(batch, rows, cols);
   if (need && (!workspace || workspace_bytes < need)) { sgpo_set_error("newton_schulz: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
-  const Source s{update, nullptr, 0.f, 0, stride_b, ld, rows, cols};
+  const Source s{update, nullptr, 0.f, 0, stride_b, ld, rows, cols, 0};
   const Result r{out, 1, 0, 0, 0, 0, 0.f, 0.f};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return dtype == SGPO_DTYPE_BF16 ? orthogonalise<bf16_t>(s, batch, coefficients, steps, eps, r, (char*)workspace, st)
@@ -563,7 +619,7 @@ extern "C" int sgpo_muon_step(void* weight, int weight_dtype, const void* grad, 
   SGPO_REQUIRE(weight && grad && momentum_buffer, "muon_step: null argument");
   const size_t need = sgpo_newton_schulz_workspace_bytes(batch, rows, cols);
   if (need && (!workspace || workspace_bytes < need)) { sgpo_set_error("muon_step: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
-  const Source s{grad, momentum_buffer, momentum, nesterov != 0, (int64_t)rows * cols, cols, rows, cols};
+  const Source s{grad, momentum_buffer, momentum, nesterov != 0, (int64_t)rows * cols, cols, rows, cols, 0};
   const double ratio = rows > cols ? (double)rows / cols : 1.0;
   const Result r{weight, weight_dtype == SGPO_DTYPE_BF16, 0, 0, 1, 0, (float)(1.0 - (double)lr * weight_decay), (float)(lr * sqrt(ratio))};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

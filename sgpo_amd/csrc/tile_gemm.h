@@ -62,8 +62,9 @@ struct Shape {
   __device__ static __forceinline__ int tid() { return KG == 1 ? (int)threadIdx.x : (int)threadIdx.x % THREADS; }
   __device__ static __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) % (WM * WN); }
   __device__ static __forceinline__ int group() { return KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) / (WM * WN); }
-  // whether this wave holds the finished 16x16 product (x, y) of its part of the tile
-  __device__ static __forceinline__ bool owns(int x, int y) { return KG == 1 || (x * NT + y) % KG == group(); }
+  // whether this wave holds the finished 16x16 product (x, y) of its part of the tile; PAIRS: products 2j and 2j + 1 of a row block have one owner
+  template <bool PAIRS = false>
+  __device__ static __forceinline__ bool owns(int x, int y) { return KG == 1 || (PAIRS ? x * ((NT + 1) / 2) + y / 2 : x * NT + y) % KG == group(); }
 };
 
 // chunk permutation of a KM row: the 16 rows that one transposed read touches ({0..3} + 8 l4) go to different banks
@@ -302,10 +303,8 @@ __device__ __forceinline__ void run_phased(Stager<S, S::BM, KA>& sa, Stager<S, S
   }
 }
 
-// acc[mt][nt][q] += C[m = m0 + (wm MT + mt) 16 + l16][n = n0 + (wn NT + nt) 16 + 4 l4 + q], k steps [kt0, kt0 + nk), nk >= 1; with several
-// groups, in the products that the wave owns.  Every thread of the workgroup calls it; smem is free again when it returns.
 template <class S, int KA, int KB>
-__device__ __forceinline__ void run(const Operand& a, const Operand& b, int m0, int n0, int kt0, int nk, char* smem, f32x4 (&acc)[S::MT][S::NT]) {
+__device__ __forceinline__ void run_groups(const Operand& a, const Operand& b, int m0, int n0, int kt0, int nk, char* smem, f32x4 (&acc)[S::MT][S::NT]) {
   Stager<S, S::BM, KA> sa;
   Stager<S, S::BN, KB> sb;
   const int each = (nk + S::KG - 1) / S::KG, g = S::group(), own = min(each, nk - g * each);
@@ -315,8 +314,15 @@ __device__ __forceinline__ void run(const Operand& a, const Operand& b, int m0, 
   if constexpr (S::NST == 2) run_phased<S, KA, KB>(sa, sb, each, slots, acc);
   else run_ring<S, KA, KB>(sa, sb, each, slots, acc);
   __syncthreads();
+}
+
+// acc[mt][nt][q] += C[m = m0 + (wm MT + mt) 16 + l16][n = n0 + (wn NT + nt) 16 + 4 l4 + q], k steps [kt0, kt0 + nk), nk >= 1; with several
+// groups, in the products that the wave owns.  Every thread of the workgroup calls it; smem is free again when it returns.
+template <class S, int KA, int KB, bool PAIRS = false>
+__device__ __forceinline__ void run(const Operand& a, const Operand& b, int m0, int n0, int kt0, int nk, char* smem, f32x4 (&acc)[S::MT][S::NT]) {
+  run_groups<S, KA, KB>(a, b, m0, n0, kt0, nk, smem, acc);
   if constexpr (S::KG > 1) {
-    f32x4* mine = reinterpret_cast<f32x4*>(slots);   // [wave][product][lane]
+    f32x4* mine = reinterpret_cast<f32x4*>(smem + S::group() * S::SLOTS);   // [wave][product][lane]
     const int at = S::wave() * S::MT * S::NT * 64 + (threadIdx.x & 63);
 #pragma unroll
     for (int x = 0; x < S::MT; ++x)
@@ -327,7 +333,7 @@ __device__ __forceinline__ void run(const Operand& a, const Operand& b, int m0, 
     for (int x = 0; x < S::MT; ++x)
 #pragma unroll
       for (int y = 0; y < S::NT; ++y) {
-        if (!S::owns(x, y)) continue;
+        if (!S::template owns<PAIRS>(x, y)) continue;
         f32x4 v = *reinterpret_cast<const f32x4*>(smem + (at + (x * S::NT + y) * 64) * 16);
 #pragma unroll
         for (int k = 1; k < S::KG; ++k) v += *reinterpret_cast<const f32x4*>(smem + k * S::SLOTS + (at + (x * S::NT + y) * 64) * 16);
@@ -393,6 +399,25 @@ __device__ __forceinline__ void load4(const bf16_t* row, int64_t e, float (&v)[4
     const uint2 w = *reinterpret_cast<const uint2*>(at + p * 32);
     v[0] += bf2f(w.x & 0xffff); v[1] += bf2f(w.x >> 16);
     v[2] += bf2f(w.y & 0xffff); v[3] += bf2f(w.y >> 16);
+  }
+}
+
+// Eight consecutive elements of a row as one 16-B store per plane: the products y and y + 1 of a row block hold, per lane, four elements of each
+// (v0, v1); neighbouring rows of lanes swap so that a lane has eight of one.  e: the first element of product y in the row (a
+// multiple of 16); a row's two products (32 elements) then go out as 64 contiguous bytes per plane instead of four pieces of 8 bytes twice.
+// Every lane of the wave calls it; `live` lanes' rows are written.
+template <int PL>
+__device__ __forceinline__ void store_pair(bf16_t* row, int64_t e, const float (&v0)[4], const float (&v1)[4], int l4, bool live) {
+  float p0[4][PL], p1[4][PL];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) { split<PL>(v0[q], p0[q]); split<PL>(v1[q], p1[q]); }
+  const int64_t at = e + (l4 & 1) * 16 + (l4 >> 1) * 8;
+  bf16_t* dst = row + (at >> 5) * (32 * PL) + (at & 31);
+#pragma unroll
+  for (int p = 0; p < PL; ++p) {
+    const auto a = __builtin_amdgcn_permlane16_swap(pack_bf16x2(p0[0][p], p0[1][p]), pack_bf16x2(p1[0][p], p1[1][p]), false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(pack_bf16x2(p0[2][p], p0[3][p]), pack_bf16x2(p1[2][p], p1[3][p]), false, false);
+    if (live) *reinterpret_cast<uint4*>(dst + p * 32) = make_uint4(a[0], b[0], a[1], b[1]);
   }
 }
 
