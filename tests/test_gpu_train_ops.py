@@ -554,3 +554,53 @@ def test_a_training_step_of_a_small_denoiser():
         x, _ = _schulz64(v.grad * 1.95, [T.NS_COEFFICIENTS] * 5, 1e-7)
         rate = 0.02 * max(1.0, v.shape[0] / v.shape[1]) ** 0.5
         assert float((new.double() - (par[k].double() - rate * x)).norm()) <= rate * 2.0 ** -9 * float(x.norm()) + 4 * U32 * float(par[k].norm())
+
+
+def test_second_derivatives():
+    """The rotation is linear: its gradient can be differentiated again.  The loss's cannot, and says so only where it is used."""
+    from sgpo_amd import train_ops as T
+    g = _gen(61)
+    q, k = (torch.randn(2, 5, 3, 16, generator=g, device='cuda', requires_grad=True) for _ in range(2))
+    u = torch.randn(2, 5, 3, 16, generator=g, device='cuda', requires_grad=True)
+    freq, _ = T.rotary_frequencies(8)
+    out, _ = T.rotary_positions(q, k, freq)
+    dq, = torch.autograd.grad(out, q, u, create_graph=True)
+    ddu, = torch.autograd.grad((dq * q.detach()).sum(), u)
+    # d/du <R^T u, q> = R q
+    assert torch.equal(ddu, out.detach())
+    h = torch.randn(6, 16, generator=g, device='cuda', requires_grad=True)
+    w = torch.randn(9, 16, generator=g, device='cuda', requires_grad=True)
+    t = torch.arange(6, device='cuda')
+    first = torch.autograd.grad(T.linear_cross_entropy(h, w, t), (h, w))
+    again = torch.autograd.grad(T.linear_cross_entropy(h, w, t), (h, w), create_graph=True)
+    assert all(torch.equal(a, b.detach()) for a, b in zip(first, again))
+    with pytest.raises(RuntimeError, match='differentiated once'):
+        torch.autograd.grad(again[0].sum(), h)
+    # only what is asked for is computed, and in any combination
+    for needs in ((True, False), (False, True)):
+        hh, ww = h.detach().requires_grad_(needs[0]), w.detach().requires_grad_(needs[1])
+        got, = torch.autograd.grad(T.linear_cross_entropy(hh, ww, t), [x for x, n in zip((hh, ww), needs) if n])
+        assert torch.equal(got, first[0] if needs[0] else first[1])
+    bias = torch.zeros(9, device='cuda', requires_grad=True)
+    got, = torch.autograd.grad(T.linear_cross_entropy(h.detach(), w.detach(), t, bias), bias)
+    assert got.shape == (9,) and float(got.sum().abs()) <= 20 * U32
+
+
+def test_versions_tell_autograd_of_writes_in_place():
+    from sgpo_amd import train_ops as T
+    freq, _ = T.rotary_frequencies(8)
+    w = torch.randn(8, 8, device='cuda')
+    x = torch.randn(8, 8, device='cuda', requires_grad=True)
+    y = x @ w
+    T.muon_step(w, torch.randn(8, 8, device='cuda'), torch.zeros(8, 8, device='cuda'), 0.1)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+    q = torch.randn(1, 4, 2, 8, device='cuda')
+    y = (x[:1, :4].reshape(1, 4, 1, 1) * q).sum()
+    T.rotary_positions_(q, None, freq)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward()
+    with torch.inference_mode():
+        q = torch.randn(1, 4, 2, 8, device='cuda')
+        T.rotary_positions_(q, None, freq)
+        T.muon_step(torch.zeros(8, 8, device='cuda'), q.new_ones(8, 8), torch.zeros(8, 8, device='cuda'), 0.1)
