@@ -10,7 +10,8 @@
 // each written twice).  X, G and P are held as two bf16 planes, about 17 bits (tile_gemm.h): in one plane the rounding of X
 // pollutes the directions of small singular values, which the polynomial then multiplies by up to a^5 = 485 (relative error of
 // the result 2e-2 on Gaussian updates, against 3e-5 with two planes; the result is rounded to bf16, 2e-3).
-// The squared norm is summed in 64 bits: it neither overflows nor depends on how the update is cut.
+// The squared norm is summed in 64 bits: it neither overflows nor depends on how the update is cut.  An infinity or NaN in an update
+// makes its whole result NaN.
 #include "../../include/sgpo_hip.h"
 #include "tile_gemm.h"
 
@@ -125,7 +126,7 @@ __global__ __launch_bounds__(256) void load_kernel(Source s, const double* part,
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) v[q] *= inv;
-    tg::store4<2>(X + b * bstride + r * ldx, c, v);
+    tg::store4<2, true>(X + b * bstride + r * ldx, c, v);
   }
 }
 
@@ -191,14 +192,14 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void symmetric_kernel(Mats q, int
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) if (n + e >= q.d) v[e] = 0.f;
-        tg::store4<2>(dst + m * q.ldg, n, v);
+        tg::store4<2, true>(dst + m * q.ldg, n, v);
       }
       if (i != j && m < q.ldg / 2) {   // the mirror image: row n + e, column m
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (n + e < q.d) {
             float pl[2];
-            tg::split<2>(m < q.d ? v[e] : 0.f, pl);
+            tg::split<2, true>(m < q.d ? v[e] : 0.f, pl);
             bf16_t* at = dst + (n + e) * q.ldg + (m >> 5) * 64 + (m & 31);
             at[0] = f2bf(pl[0]);
             at[32] = f2bf(pl[1]);
@@ -250,9 +251,9 @@ __device__ __forceinline__ void store_result(const Result& r, int b, int m, int 
 // keeps both kinds of read off each other's banks.  Bound by the chain of 3 dependent products per triple, each a few LDS round trips.
 template <int E>
 struct Small {
-  static constexpr int WAVES_M = 2, WAVES_N = E == 128 ? 4 : 2, THREADS = 64 * WAVES_M * WAVES_N;
+  static constexpr int WAVES_M = 4, WAVES_N = 4, THREADS = 64 * WAVES_M * WAVES_N;
   static constexpr int MT = E / WAVES_M / 16, NT = E / WAVES_N / 16;
-  static constexpr int ROWB = E * 4, IMAGE = E * ROWB, LDS = 2 * IMAGE;
+  static constexpr int ROWB = E * 4, IMAGE = E * ROWB, IMAGES = 4 * IMAGE <= 163840 ? 4 : 2, LDS = IMAGES * IMAGE;
   typedef f32x4 Acc[MT][NT];
   __device__ static __forceinline__ int swz(int row) { return ((row & 1) << 1) | ((row & 2) << 1) | ((row & 8)) | ((row >> 2) & 1); }
   // byte of element (row, e) of plane 0; its 16-B chunk holds e .. e + 7 of one plane, plane 1 is 4 chunks on
@@ -274,7 +275,9 @@ struct Small {
     for (int x = 0; x < MT; ++x)
 #pragma unroll
       for (int y = 0; y < NT; ++y) r[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < slices; ++s) {
+#pragma unroll
+    for (int s = 0; s < E / 32; ++s) {   // unrolled: the fragments' addresses are then formed once for all triples
+      if (s >= slices) break;
       bf16x8 a[2][MT], b[2][NT];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -299,7 +302,7 @@ struct Small {
         const int row = (wm * MT + x) * 16 + l16, e = (wn * NT + y) * 16 + 4 * l4;
         float pl[4][2];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tg::split<2>(v[x][y][q], pl[q]);
+        for (int q = 0; q < 4; ++q) tg::split<2, true>(v[x][y][q], pl[q]);
 #pragma unroll
         for (int p = 0; p < 2; ++p)
           *reinterpret_cast<uint2*>(img + at(row, e, p)) = make_uint2(pack_bf16x2(pl[0][p], pl[1][p]), pack_bf16x2(pl[2][p], pl[3][p]));
@@ -314,7 +317,6 @@ __global__ __launch_bounds__(Small<E>::THREADS, 1) void small_kernel(Source s, i
   typedef Small<E> K;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ double share[K::THREADS / 64];
-  char *X = smem, *G = smem + K::IMAGE;
   const int b = blockIdx.x, lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave / K::WAVES_N, wn = wave % K::WAVES_N;
   typename K::Acc x, g, h;
@@ -351,10 +353,13 @@ __global__ __launch_bounds__(Small<E>::THREADS, 1) void small_kernel(Source s, i
 #pragma unroll
     for (int j = 0; j < K::NT; ++j) x[i][j] *= inv;
   const int sm = (m + 31) >> 5, sn = (n + 31) >> 5;   // k slices
+  // Four images (X and the next X, G, P) need one barrier per product; where only two fit, what overwrites an image waits for its readers.
+  constexpr bool ROOM = K::IMAGES == 4;
+  char *X = smem, *G = smem + K::IMAGE, *P = ROOM ? smem + 2 * K::IMAGE : G, *next = ROOM ? smem + 3 * K::IMAGE : X;
+  K::put(X, x, wm, wn, l16, l4);
+  __syncthreads();
   for (int k = 0; k < steps; ++k) {
     const float ca = coef.v[3 * k], cb = coef.v[3 * k + 1], cc = coef.v[3 * k + 2];
-    K::put(X, x, wm, wn, l16, l4);
-    __syncthreads();
     K::template product<false>(X, X, sn, g, wm, wn, l16, l4);
     K::put(G, g, wm, wn, l16, l4);
     __syncthreads();
@@ -365,17 +370,21 @@ __global__ __launch_bounds__(Small<E>::THREADS, 1) void small_kernel(Source s, i
       for (int j = 0; j < K::NT; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) h[i][j][q] = fmaf(cb, g[i][j][q], cc * h[i][j][q]);
+    if (!ROOM) __syncthreads();
+    K::put(P, h, wm, wn, l16, l4);
     __syncthreads();
-    K::put(G, h, wm, wn, l16, l4);
-    __syncthreads();
-    K::template product<true>(G, X, sm, g, wm, wn, l16, l4);
+    K::template product<true>(P, X, sm, g, wm, wn, l16, l4);
 #pragma unroll
     for (int i = 0; i < K::MT; ++i)
 #pragma unroll
       for (int j = 0; j < K::NT; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) x[i][j][q] = fmaf(ca, x[i][j][q], g[i][j][q]);
+    if (k + 1 == steps) break;
+    if (!ROOM) __syncthreads();
+    K::put(next, x, wm, wn, l16, l4);
     __syncthreads();
+    char* t = X; X = next; next = t;
   }
 #pragma unroll
   for (int i = 0; i < K::MT; ++i)
@@ -431,10 +440,10 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void apply_kernel(Mats q, int tm,
       for (int y = 0; y < S::NT; y += 2) {
         if (!S::template owns<!LAST>(x, y)) continue;
         const int e = n0 + (wn * S::NT + y) * 16;
-        if (y + 1 < S::NT && e % 32 == 0) tg::store_pair<2>(at, e, w[y], w[y + 1 < S::NT ? y + 1 : y], l4, row && e < pad);
+        if (y + 1 < S::NT && e % 32 == 0) tg::store_pair<2, true>(at, e, w[y], w[y + 1 < S::NT ? y + 1 : y], l4, row && e < pad);
         else {
-          if (row && e < pad) tg::store4<2>(at, e + 4 * l4, w[y]);
-          if (y + 1 < S::NT && row && e + 16 < pad) tg::store4<2>(at, e + 16 + 4 * l4, w[y + 1 < S::NT ? y + 1 : y]);
+          if (row && e < pad) tg::store4<2, true>(at, e + 4 * l4, w[y]);
+          if (y + 1 < S::NT && row && e + 16 < pad) tg::store4<2, true>(at, e + 16 + 4 * l4, w[y + 1 < S::NT ? y + 1 : y]);
         }
       }
     }

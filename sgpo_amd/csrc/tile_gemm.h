@@ -361,29 +361,23 @@ __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& im, int& in
   in = in_band / h;
 }
 
-// x as PL bf16 planes
-template <int PL>
+// x as PL bf16 planes; an infinity has no rest (inf - inf) -- unless FINITE, where it becomes NaN
+template <int PL, bool FINITE = false>
 __device__ __forceinline__ void split(float x, float (&pl)[PL]) {
+  pl[0] = bf2f(f2bf(x));
 #pragma unroll
-  for (int p = 0; p < PL; ++p) {
+  for (int p = 1; p < PL; ++p) {
+    x = !FINITE && __builtin_isinf(pl[0]) ? 0.f : x - pl[p - 1];
     pl[p] = bf2f(f2bf(x));
-    if (p + 1 < PL) x -= pl[p];
-  }
-  // an infinity minus itself is no rest
-  if constexpr (PL > 1) {
-    if (__builtin_isinf(pl[0])) {
-#pragma unroll
-      for (int p = 1; p < PL; ++p) pl[p] = 0.f;
-    }
   }
 }
 
 // four consecutive elements (e % 4 == 0) of a row, as planes
-template <int PL>
+template <int PL, bool FINITE = false>
 __device__ __forceinline__ void store4(bf16_t* row, int64_t e, const float (&v)[4]) {
   float pl[4][PL];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) split<PL>(v[q], pl[q]);
+  for (int q = 0; q < 4; ++q) split<PL, FINITE>(v[q], pl[q]);
   bf16_t* at = row + (e >> 5) * (32 * PL) + (e & 31);
 #pragma unroll
   for (int p = 0; p < PL; ++p)
@@ -406,11 +400,11 @@ __device__ __forceinline__ void load4(const bf16_t* row, int64_t e, float (&v)[4
 // (v0, v1); neighbouring rows of lanes swap so that a lane has eight of one.  e: the first element of product y in the row (a
 // multiple of 16); a row's two products (32 elements) then go out as 64 contiguous bytes per plane instead of four pieces of 8 bytes twice.
 // Every lane of the wave calls it; `live` lanes' rows are written.
-template <int PL>
+template <int PL, bool FINITE = false>
 __device__ __forceinline__ void store_pair(bf16_t* row, int64_t e, const float (&v0)[4], const float (&v1)[4], int l4, bool live) {
   float p0[4][PL], p1[4][PL];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) { split<PL>(v0[q], p0[q]); split<PL>(v1[q], p1[q]); }
+  for (int q = 0; q < 4; ++q) { split<PL, FINITE>(v0[q], p0[q]); split<PL, FINITE>(v1[q], p1[q]); }
   const int64_t at = e + (l4 & 1) * 16 + (l4 >> 1) * 8;
   bf16_t* dst = row + (at >> 5) * (32 * PL) + (at & 31);
 #pragma unroll

@@ -665,7 +665,7 @@ Plan make_plan(const sgpo_linear_ce_args* a, bool backward) {
   const bool bf = a->dtype == SGPO_DTYPE_BF16;
   q.PL = bf ? 1 : 3;
   const int kstep = bf ? 64 : 32;
-  q.h_pad = (int)round_up(a->H, 64);
+  q.h_pad = (int)round_up(a->H, kstep);
   q.n_kstep = q.h_pad / kstep;
   const bool whole = bf && a->H % 64 == 0;
   q.head = a->V <= 64;
