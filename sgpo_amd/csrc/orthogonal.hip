@@ -151,12 +151,18 @@ __device__ __forceinline__ void triangle(int t, int tiles, int& i, int& j) {
   j = i + t;
 }
 
+// K cut over gridDim.y: fp32 sums [cut][matrix][d][pitch], in the tiles of the triangle
+struct Slabs {
+  float* out;        // null: not cut
+  int steps, pitch;  // K steps per cut
+};
+
 enum { WIDE = 0, TALL = 1, POLY = 2 };   // G = X X^T;  G = X^T X;  P = a I + b G + c G G
 
 // One triangle of tiles, each also written transposed (element by element: taking the transposed tile through LDS and out in whole lines
 // measured the same, 60 us either way for 512 x 1536 in 192 x 192 tiles)
 template <class S, int MODE>
-__global__ __launch_bounds__(S::WG_THREADS, 2) void symmetric_kernel(Mats q, int tiles, float ca, float cb, float cc) {
+__global__ __launch_bounds__(S::WG_THREADS, 2) void symmetric_kernel(Mats q, int tiles, float ca, float cb, float cc, Slabs slabs) {
   static_assert(S::BM == S::BN && S::PL == 2, "square tiles of two planes");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int i, j, b, t;
@@ -168,10 +174,12 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void symmetric_kernel(Mats q, int
   tg::clear<S>(acc);
   if constexpr (MODE == TALL) {
     const tg::Operand o{q.X + b * q.sx, q.ldx, q.rows, (int)q.ldx};
-    tg::run<S, tg::KM, tg::KM>(o, o, m0, n0, 0, (q.rows + 31) / 32, smem, acc);
+    const int nk = (q.rows + 31) / 32, k0 = slabs.out ? blockIdx.y * slabs.steps : 0;
+    tg::run<S, tg::KM, tg::KM>(o, o, m0, n0, k0, slabs.out ? min(slabs.steps, nk - k0) : nk, smem, acc);
   } else {
     const tg::Operand o{MODE == POLY ? G : q.X + b * q.sx, MODE == POLY ? q.ldg : q.ldx, q.d, 0};
-    tg::run<S, tg::KC, tg::KC>(o, o, m0, n0, 0, (int)(o.ld / 64), smem, acc);
+    const int nk = (int)(o.ld / 64), k0 = MODE != POLY && slabs.out ? blockIdx.y * slabs.steps : 0;
+    tg::run<S, tg::KC, tg::KC>(o, o, m0, n0, k0, MODE != POLY && slabs.out ? min(slabs.steps, nk - k0) : nk, smem, acc);
   }
   bf16_t* dst = (MODE == POLY ? q.P : q.G) + b * q.sg;
   const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4, wm = S::wave() / S::WN, wn = S::wave() % S::WN;
@@ -182,6 +190,10 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void symmetric_kernel(Mats q, int
     for (int y = 0; y < S::NT; ++y) {
       if (!S::owns(x, y)) continue;
       const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4;
+      if (MODE != POLY && slabs.out) {
+        if (m < q.d && n < slabs.pitch) *reinterpret_cast<f32x4*>(slabs.out + (((int64_t)blockIdx.y * (gridDim.x / (tiles * (tiles + 1) / 2)) + b) * q.d + m) * slabs.pitch + n) = acc[x][y];
+        continue;
+      }
       float v[4] = {acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]};
       if (m < q.d && n < q.ldg / 2) {
         if constexpr (MODE == POLY) {
@@ -206,6 +218,24 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void symmetric_kernel(Mats q, int
           }
       }
     }
+  }
+}
+
+// G from the cuts' sums; side: of the triangle's tiles
+__global__ __launch_bounds__(256) void join_kernel(Mats q, Slabs slabs, int cuts, int side) {
+  const int b = blockIdx.y, quads = (int)(q.ldg / 8);
+  const int64_t stride = (int64_t)gridDim.y * q.d * slabs.pitch;
+  const float* src = slabs.out + (int64_t)b * q.d * slabs.pitch;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < q.d * quads; i += gridDim.x * 256) {
+    const int r = i / quads, c = (i - r * quads) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool upper = c / side >= r / side;
+    for (int k = 0; k < cuts; ++k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < q.d) v[e] += src[k * stride + (upper ? (int64_t)r * slabs.pitch + c + e : (int64_t)(c + e) * slabs.pitch + r)];
+    }
+    tg::store4<2, true>(q.G + b * q.sg + r * q.ldg, c, v);
   }
 }
 
@@ -462,10 +492,14 @@ int allow_lds(K kernel, int bytes) {
   } while (0)
 
 template <class S, int MODE>
-int symmetric(const Mats& q, int batch, const float* coef, hipStream_t st) {
+int symmetric(const Mats& q, int batch, const float* coef, const Slabs& slabs, int cuts, hipStream_t st) {
   const int t = (q.d + S::BM - 1) / S::BM;
   ALLOW((symmetric_kernel<S, MODE>), S::LDS);
-  hipLaunchKernelGGL((symmetric_kernel<S, MODE>), dim3((unsigned)(t * (t + 1) / 2) * batch), dim3(S::WG_THREADS), S::LDS, st, q, t, coef[0], coef[1], coef[2]);
+  hipLaunchKernelGGL((symmetric_kernel<S, MODE>), dim3((unsigned)(t * (t + 1) / 2) * batch, cuts), dim3(S::WG_THREADS), S::LDS, st, q, t, coef[0], coef[1], coef[2], slabs);
+  if (slabs.out) {
+    const int blocks = (int)((q.d * (q.ldg / 8) + 255) / 256);
+    hipLaunchKernelGGL(join_kernel, dim3(blocks, batch), dim3(256), 0, st, q, slabs, cuts, S::BM);
+  }
   return SGPO_OK;
 }
 template <class S, bool TALLX, bool LAST>
@@ -489,16 +523,21 @@ typedef tg::Shape<96, 96, 2, 2, 2, 2, 3> Shape96;
 typedef tg::Shape<64, 64, 2, 2, 2, 2, 2> Shape64;
 typedef tg::Shape<32, 32, 1, 1, 2, 2, 4> Shape32;
 
-// the kind with the least rounds of the 256 CUs x cost of a tile; count(side) tiles of `steps` K steps
+// The kind with the least rounds of the 256 CUs x cost of a tile; count(side) tiles of `steps` K steps.  A symmetric product with few tiles and a
+// long K may also be cut along K (at most `cuts` times), which costs the joining launch and its bytes (64 x 7616, ten of them: 45 -> 13 us).
+struct Pick { int kind, cuts; };
 template <typename F>
-int pick(F count, int64_t steps, bool sym) {
-  int best = 0;
+Pick pick(F count, int64_t steps, bool sym, int most_cuts = 1, double joined_bytes = 0.) {
+  Pick best = {0, 1};
   double least = 1e300;
-  for (const Kind& k : KINDS) {
-    const int64_t n = count(k.side == 129 ? 128 : k.side);
-    const double rounds = k.per_cu == 1 ? (double)((n + 255) / 256) : n <= 256 ? 1. : (n + 127) / 128 * 0.5;
-    const double t = rounds * ((sym ? k.symmetric : k.apply) + steps * k.step);
-    if (t < least) { least = t; best = k.side; }
+  for (int s = 1; s <= most_cuts; s *= 2) {
+    if (s > 1 && steps / s < 8) break;
+    for (const Kind& k : KINDS) {
+      const int64_t n = count(k.side == 129 ? 128 : k.side) * s;
+      const double rounds = k.per_cu == 1 ? (double)((n + 255) / 256) : n <= 256 ? 1. : (n + 127) / 128 * 0.5;
+      const double t = rounds * ((sym ? k.symmetric : k.apply) + (double)((steps + s - 1) / s) * k.step) + (s > 1 ? 5. + s * joined_bytes * 2. / 4e6 : 0.);
+      if (t < least) { least = t; best = {k.side, s}; }
+    }
   }
   return best;
 }
@@ -513,15 +552,16 @@ int pick(F count, int64_t steps, bool sym) {
     default: { typedef Shape32 S; return CALL; }                       \
   }
 template <int MODE>
-int symmetric_any(int kind, const Mats& q, int batch, const float* coef, hipStream_t st) {
-  FOR_KIND(kind, (symmetric<S, MODE>(q, batch, coef, st)))
+int symmetric_any(int kind, const Mats& q, int batch, const float* coef, const Slabs& slabs, int cuts, hipStream_t st) {
+  FOR_KIND(kind, (symmetric<S, MODE>(q, batch, coef, slabs, cuts, st)))
 }
 template <bool TALLX, bool LAST>
 int apply_any(int kind, const Mats& q, int batch, const Result& r, hipStream_t st) {
   FOR_KIND(kind, (apply<S, TALLX, LAST>(q, batch, r, st)))
 }
 
-struct Sizes { int d, longer; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, bytes; };
+constexpr int CUTS = 32;
+struct Sizes { int d, longer; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, off_s, bytes; Pick gram, poly, full; };
 Sizes sizes(int batch, int rows, int cols) {
   Sizes s = {};
   s.d = rows < cols ? rows : cols;
@@ -535,6 +575,13 @@ Sizes sizes(int batch, int rows, int cols) {
   take((size_t)batch * PARTS * 8);
   s.off_x = take(batch * s.x * 2); s.off_y = take(batch * s.x * 2);
   s.off_g = take(batch * s.g * 2); s.off_p = take(batch * s.g * 2);
+  auto up = [](int64_t n, int64_t m) { return (n + m - 1) / m; };
+  auto triangles = [&](int side) { return batch * up(s.d, side) * (up(s.d, side) + 1) / 2; };
+  const double sums = (double)batch * s.d * round_up(s.d, 4) * 4;
+  s.gram = pick(triangles, up(s.longer, 32), true, CUTS, sums);
+  s.poly = pick(triangles, up(s.d, 32), true);
+  s.full = pick([&](int side) { return batch * up(rows, side) * up(cols, side); }, up(s.d, 32), false);
+  s.off_s = take(s.gram.cuts > 1 ? (size_t)(s.gram.cuts * sums) : 0);
   s.bytes = at;
   return s;
 }
@@ -567,13 +614,17 @@ int orthogonalise(Source src, int batch, const float* coef, int steps, double ep
   hipLaunchKernelGGL((square_kernel<T>), dim3(parts, batch), dim3(256), 0, st, src, part);
   const int64_t blocks = ((int64_t)src.rows * (z.ldx / 8) + 255) / 256;
   hipLaunchKernelGGL((load_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), batch), dim3(256), 0, st, src, part, parts, eps, q.X, z.ldx, (int64_t)z.x);
-  auto up = [](int64_t n, int64_t s) { return (n + s - 1) / s; };
-  auto triangles = [&](int s) { return batch * up(z.d, s) * (up(z.d, s) + 1) / 2; };
-  const int kg = pick(triangles, up(z.longer, 32), true), kp = pick(triangles, up(z.d, 32), true);
-  const int ka = pick([&](int s) { return batch * up(src.rows, s) * up(src.cols, s); }, up(z.d, 32), false);
+  Slabs slabs = {nullptr, 0, 0};
+  int cuts = 1;
+  if (z.gram.cuts > 1) {
+    const int steps_k = (z.longer + 31) / 32, per = (steps_k + z.gram.cuts - 1) / z.gram.cuts;
+    cuts = (steps_k + per - 1) / per;
+    slabs = Slabs{(float*)(ws + z.off_s), per, (int)round_up(z.d, 4)};
+  }
+  const int kg = z.gram.kind, kp = z.poly.kind, ka = z.full.kind;
   for (int k = 0; k < steps; ++k) {
-    int rc = tall ? symmetric_any<TALL>(kg, q, batch, coef + 3 * k, st) : symmetric_any<WIDE>(kg, q, batch, coef + 3 * k, st);
-    if (!rc) rc = symmetric_any<POLY>(kp, q, batch, coef + 3 * k, st);
+    int rc = tall ? symmetric_any<TALL>(kg, q, batch, coef + 3 * k, slabs, cuts, st) : symmetric_any<WIDE>(kg, q, batch, coef + 3 * k, slabs, cuts, st);
+    if (!rc) rc = symmetric_any<POLY>(kp, q, batch, coef + 3 * k, Slabs{nullptr, 0, 0}, 1, st);
     if (!rc) {
       if (k + 1 < steps) rc = tall ? apply_any<true, false>(ka, q, batch, res, st) : apply_any<false, false>(ka, q, batch, res, st);
       else rc = tall ? apply_any<true, true>(ka, q, batch, res, st) : apply_any<false, true>(ka, q, batch, res, st);

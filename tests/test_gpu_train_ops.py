@@ -360,7 +360,7 @@ def _schulz64(u, coefficients, eps):
 
 
 ORTHO = [((8, 8), F32), ((1, 1), F32), ((1, 40), BF), ((40, 1), F32), ((64, 64), F32), ((33, 65), BF), ((100, 70), F32), ((200, 130), BF), ((130, 517), F32),
-         ((513, 129), BF), ((512, 2048), BF), ((1536, 512), F32), ((3, 64, 48), F32), ((2, 2, 150, 40), BF)]
+         ((513, 129), BF), ((512, 2048), BF), ((1536, 512), F32), ((3, 64, 48), F32), ((2, 2, 150, 40), BF), ((3, 64, 4000), F32), ((5000, 70), BF), ((2, 150, 9000), BF)]
 
 
 @pytest.mark.parametrize('shape,dtype', ORTHO)
