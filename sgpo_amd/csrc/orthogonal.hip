@@ -613,7 +613,9 @@ int orthogonalise(Source src, int batch, const float* coef, int steps, double ep
   const int parts = want < PARTS ? (int)want : PARTS;
   hipLaunchKernelGGL((square_kernel<T>), dim3(parts, batch), dim3(256), 0, st, src, part);
   const int64_t blocks = ((int64_t)src.rows * (z.ldx / 8) + 255) / 256;
-  hipLaunchKernelGGL((load_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), batch), dim3(256), 0, st, src, part, parts, eps, q.X, z.ldx, (int64_t)z.x);
+  // Each workgroup adds up the norm's parts first, so the device is filled once and not more (six 384 x 1536 bf16: 22.3 us with up to 4096 a matrix, 16.1 so).
+  const int64_t most = batch < 32 ? 2048 / batch : 64;
+  hipLaunchKernelGGL((load_kernel<T>), dim3((unsigned)(blocks < most ? blocks : most), batch), dim3(256), 0, st, src, part, parts, eps, q.X, z.ldx, (int64_t)z.x);
   Slabs slabs = {nullptr, 0, 0};
   int cuts = 1;
   if (z.gram.cuts > 1) {
