@@ -375,7 +375,8 @@ int sgpo_daps_mh(sgpo_mlp* m, const int64_t* x0hat, int N, int L, int S, const i
 /* Rotation of query and key heads by their positions.  Pair j < rot / 2 of a head -- elements (j, j + rot / 2), or (2j, 2j + 1)
  * if interleaved -- turns by position * frequencies[j] (formed in 64 bits) and is multiplied by scale; elements from rot on are
  * copied.  inverse: the transposed rotation, i.e. the gradient.  Strides in elements: batch, token, head; a head's elements
- * are contiguous.  q_out may be q and k_out may be k (in place); otherwise outputs must not overlap inputs.  heads_k 0: no keys.
+ * are contiguous.  q_out may be q and k_out may be k (in place); any other overlap of an output with itself, the other one or an input is
+ * refused (views of different strides count as overlapping where their address ranges meet).  heads_k 0: no keys.
  * positions NULL: the token's index 0 .. L-1.  positions and frequencies are device memory. */
 typedef struct {
   const void* q; void* q_out;
@@ -395,7 +396,7 @@ int sgpo_rotary(const sgpo_rotary_args* args, void* stream);
  *   target outside [0, V) gives NaN.
  * forward: nll [N], lse [N] fp32; loss [1] and inv_count [1] unless reduction is NONE (the mean over no token is 0).
  * backward: grad_out is [1] ([N] for NONE); lse and inv_count are the forward's; dhidden [N][H], dweight [V][H] of `dtype` and dbias fp32
- *   [V], contiguous; any of them may be NULL.
+ *   [V], contiguous, overlapping neither the inputs nor one another; any of them may be NULL.
  * The workspace is scratch: forward and backward each ask for their own. */
 #define SGPO_REDUCE_NONE 0
 #define SGPO_REDUCE_MEAN 1
@@ -417,7 +418,8 @@ int sgpo_linear_ce_backward(const sgpo_linear_ce_args* args, const float* lse, c
 /* Orthogonalised updates: X = U / (|U|_F + eps), then X <- a X + (b X X^T + c (X X^T)^2) X for each triple of `coefficients` (HOST,
  * 3 * steps floats).  newton_schulz: update [batch][rows][cols] of `dtype`, matrices stride_b and rows ld elements apart; out bf16,
  * contiguous.  muon_step, everything contiguous: buffer = momentum buffer + grad; U = grad + momentum buffer if nesterov, else
- * buffer; weight = (1 - lr weight_decay) weight - lr sqrt(max(1, rows / cols)) X. */
+ * buffer; weight = (1 - lr weight_decay) weight - lr sqrt(max(1, rows / cols)) X.  Outputs and what is updated overlap nothing else; at most 65535
+ * matrices of at most 2^22 rows and columns. */
 size_t sgpo_newton_schulz_workspace_bytes(int batch, int rows, int cols);
 int sgpo_newton_schulz(const void* update, int dtype, int batch, int rows, int cols, int64_t stride_b, int64_t ld,
                        const float* coefficients, int steps, float eps, void* out, void* workspace,

@@ -638,10 +638,15 @@ int orthogonalise(Source src, int batch, const float* coef, int steps, double ep
   return SGPO_OK;
 }
 
+constexpr int MOST = 1 << 22;
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) { return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; }   // bytes
+
 int check_sizes(int batch, int rows, int cols, int steps, const float* coef) {
   SGPO_REQUIRE(batch >= 0 && rows >= 0 && cols >= 0, "newton_schulz: negative size");
   SGPO_REQUIRE(batch <= 65535 && (int64_t)rows * cols <= 0x7fffffff && (int64_t)batch * rows * cols <= ((int64_t)1 << 40), "newton_schulz: %d matrices of %d x %d over the supported range",
                batch, rows, cols);
+  // 256 rows of X, two planes each, lie within the 32-bit offsets of the tiles' loads
+  SGPO_REQUIRE(rows <= MOST && cols <= MOST, "newton_schulz: %d x %d: at most %d rows or columns", rows, cols, MOST);
   SGPO_REQUIRE(steps >= 1 && steps <= 64 && coef, "newton_schulz: 1 to 64 coefficient triples are needed, got %d", steps);
   return SGPO_OK;
 }
@@ -663,6 +668,8 @@ extern "C" int sgpo_newton_schulz(const void* update, int dtype, int batch, int 
   SGPO_REQUIRE(ld >= cols || rows == 1, "newton_schulz: row pitch %lld below %d columns", (long long)ld, cols);
   const size_t need = sgpo_newton_schulz_workspace_bytes(batch, rows, cols);
   if (need && (!workspace || workspace_bytes < need)) { sgpo_set_error("newton_schulz: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
+  const int esz = dtype == SGPO_DTYPE_BF16 ? 2 : 4;
+  SGPO_REQUIRE(stride_b >= 0 && !overlap(update, ((batch - 1) * stride_b + (rows - 1) * ld + cols) * esz, out, (int64_t)batch * rows * cols * 2), "newton_schulz: out overlaps update");
   const Source s{update, nullptr, 0.f, 0, stride_b, ld, rows, cols, 0};
   const Result r{out, 1, 0, 0, 0, 0, 0.f, 0.f};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -681,6 +688,9 @@ extern "C" int sgpo_muon_step(void* weight, int weight_dtype, const void* grad, 
   SGPO_REQUIRE(weight && grad && momentum_buffer, "muon_step: null argument");
   const size_t need = sgpo_newton_schulz_workspace_bytes(batch, rows, cols);
   if (need && (!workspace || workspace_bytes < need)) { sgpo_set_error("muon_step: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
+  const int64_t n = (int64_t)batch * rows * cols, wb = n * (weight_dtype == SGPO_DTYPE_BF16 ? 2 : 4), gb = n * (grad_dtype == SGPO_DTYPE_BF16 ? 2 : 4);
+  SGPO_REQUIRE(!overlap(weight, wb, grad, gb) && !overlap(weight, wb, momentum_buffer, n * 4) && !overlap(grad, gb, momentum_buffer, n * 4),
+               "muon_step: weight, grad and momentum_buffer overlap");
   const Source s{grad, momentum_buffer, momentum, nesterov != 0, (int64_t)rows * cols, cols, rows, cols, 0};
   const double ratio = rows > cols ? (double)rows / cols : 1.0;
   const Result r{weight, weight_dtype == SGPO_DTYPE_BF16, 0, 0, 1, 0, (float)(1.0 - (double)lr * weight_decay), (float)(lr * sqrt(ratio))};

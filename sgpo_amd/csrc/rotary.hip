@@ -7,6 +7,8 @@
 // Bound by memory: every element is read and written once (q and k in one launch).  The angles of a token are formed once for
 // all of its heads, in 64 bits -- at position 2^22 an fp32 product is off by a quarter radian -- reduced to one turn in 64 bits and only then
 // rounded to fp32 for sin / cos.
+#include <algorithm>
+
 #include "../../include/sgpo_hip.h"
 #include "common.h"
 
@@ -176,10 +178,7 @@ int run(const sgpo_rotary_args* a, hipStream_t st) {
       const int dim = i == 0 ? a->B : i == 1 ? a->L : heads[w];
       if (heads[w] && dim > 1) off |= (uint64_t)p.is[w][i] | (uint64_t)p.os[w][i];
     }
-    if (heads[w]) {
-      SGPO_REQUIRE(p.in[w] && p.out[w] && (uintptr_t)p.in[w] % sizeof(T) == 0 && (uintptr_t)p.out[w] % sizeof(T) == 0, "rotary: null or misaligned heads");
-      off |= (uintptr_t)p.in[w] / sizeof(T) | (uintptr_t)p.out[w] / sizeof(T);
-    }
+    if (heads[w]) off |= (uintptr_t)p.in[w] / sizeof(T) | (uintptr_t)p.out[w] / sizeof(T);
   }
   int vec = most;
   while (vec > 1 && off % vec) vec >>= 1;
@@ -196,6 +195,86 @@ int run(const sgpo_rotary_args* a, hipStream_t st) {
   return launch<T, 1, false>(p, h, st);
 }
 
+// Heads in memory: four dimensions, the last one contiguous.  Host side of the in-place call: what a workgroup writes must be nothing that
+// another one reads.
+struct View {
+  uintptr_t at;
+  int64_t n[4], s[4];   // elements; a dimension of one element has no stride
+  int64_t extent() const {
+    int64_t e = 1;
+    for (int i = 0; i < 4; ++i) e += (n[i] - 1) * (s[i] < 0 ? -s[i] : s[i]);
+    return e;
+  }
+};
+View view_of(const void* p, const int64_t* stride, int B, int L, int heads, int D) {
+  return View{(uintptr_t)p, {B, L, heads, D}, {stride[0], stride[1], stride[2], 1}};
+}
+// is r = sum of delta_i * s_i with -(nb_i - 1) <= delta_i <= na_i - 1, over the dimensions from i on (strides descending)?
+bool reachable(int64_t r, const int64_t (&s)[4], const int64_t (&na)[4], const int64_t (&nb)[4], int i) {
+  if (i == 4) return r == 0;
+  int64_t up = 0, down = 0;   // what the dimensions behind this one can add
+  for (int j = i + 1; j < 4; ++j) { up += (na[j] - 1) * s[j]; down += (nb[j] - 1) * s[j]; }
+  if (s[i] == 0) return reachable(r, s, na, nb, i + 1);
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  int64_t lo = -floor_div(up - r, s[i]), hi = floor_div(r + down, s[i]);   // r - delta s within [-down, up]
+  if (lo < -(nb[i] - 1)) lo = -(nb[i] - 1);
+  if (hi > na[i] - 1) hi = na[i] - 1;
+  for (int64_t d = lo; d <= hi; ++d)
+    if (reachable(r - d * s[i], s, na, nb, i + 1)) return true;
+  return false;
+}
+// no two elements at one place: each stride reaches over all that the smaller ones span
+bool apart(const View& v) {
+  int order[4] = {0, 1, 2, 3};
+  std::sort(order, order + 4, [&](int a, int b) { return v.s[a] < v.s[b]; });
+  int64_t span = 1;
+  for (int i : order) {
+    if (v.n[i] <= 1) continue;
+    if (v.s[i] < span) return false;
+    span += (v.n[i] - 1) * v.s[i];
+  }
+  return true;
+}
+// may a and b share memory?  Exact for views of one packed tensor (the same strides); any others whose address ranges meet count as sharing.
+bool share(const View& a, const View& b, size_t esz) {
+  for (int i = 0; i < 3; ++i) if (a.s[i] < 0 || b.s[i] < 0) return true;
+  if (a.at + a.extent() * esz <= b.at || b.at + b.extent() * esz <= a.at) return false;
+  const int64_t bytes = (int64_t)(a.at - b.at);
+  if (bytes % (int64_t)esz) return true;
+  int order[4] = {0, 1, 2, 3};
+  int64_t s[4];
+  for (int i = 0; i < 4; ++i) {
+    if (a.n[i] > 1 && b.n[i] > 1 && a.s[i] != b.s[i]) return true;
+    s[i] = a.n[i] > 1 ? a.s[i] : b.n[i] > 1 ? b.s[i] : 0;
+  }
+  std::sort(order, order + 4, [&](int x, int y) { return s[x] > s[y]; });
+  int64_t so[4], na[4], nb[4];
+  for (int i = 0; i < 4; ++i) { so[i] = s[order[i]]; na[i] = a.n[order[i]]; nb[i] = b.n[order[i]]; }
+  return reachable(-bytes / (int64_t)esz, so, na, nb, 0);   // a.at + delta s = b.at
+}
+
+int check_memory(const sgpo_rotary_args* a) {
+  const size_t esz = a->dtype == SGPO_DTYPE_BF16 ? 2 : 4;
+  View in[2], out[2];
+  const int heads[2] = {a->heads_q, a->heads_k};
+  for (int w = 0; w < 2; ++w) {
+    if (!heads[w]) continue;
+    in[w] = view_of(w ? a->k : a->q, w ? a->k_stride : a->q_stride, a->B, a->L, heads[w], a->head_dim);
+    out[w] = view_of(w ? a->k_out : a->q_out, w ? a->k_out_stride : a->q_out_stride, a->B, a->L, heads[w], a->head_dim);
+    SGPO_REQUIRE(in[w].at && out[w].at && in[w].at % esz == 0 && out[w].at % esz == 0, "rotary: null or misaligned heads");
+    SGPO_REQUIRE(apart(out[w]), "rotary: elements of the output overlap");
+  }
+  for (int w = 0; w < 2; ++w)
+    for (int u = 0; u < 2; ++u) {
+      if (!heads[w] || !heads[u]) continue;
+      bool same = w == u && in[u].at == out[w].at;
+      for (int i = 0; i < 3; ++i) same = same && (in[u].n[i] <= 1 || in[u].s[i] == out[w].s[i]);
+      SGPO_REQUIRE(same || !share(out[w], in[u], esz), "rotary: an output overlaps %s", w == u ? "its input without being it" : "the other input");
+    }
+  SGPO_REQUIRE(!heads[0] || !heads[1] || !share(out[0], out[1], esz), "rotary: q_out and k_out overlap");
+  return SGPO_OK;
+}
+
 }  // namespace
 
 extern "C" int sgpo_rotary(const sgpo_rotary_args* a, void* stream) {
@@ -206,6 +285,7 @@ extern "C" int sgpo_rotary(const sgpo_rotary_args* a, void* stream) {
   SGPO_REQUIRE(a->dtype == SGPO_DTYPE_F32 || a->dtype == SGPO_DTYPE_BF16, "rotary: unknown dtype %d", a->dtype);
   if ((int64_t)a->B * a->L == 0 || a->heads_q + a->heads_k == 0) return SGPO_OK;
   SGPO_REQUIRE((int64_t)a->B * a->L < 0x7fffffff, "rotary: B * L = %lld tokens in one call", (long long)a->B * a->L);
+  if (const int rc = check_memory(a)) return rc;
   SGPO_REQUIRE(a->rot == 0 || a->frequencies, "rotary: null frequencies");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return a->dtype == SGPO_DTYPE_BF16 ? run<bf16_t>(a, st) : run<float>(a, st);

@@ -83,6 +83,7 @@ struct Call {
 const Tensor* opt(const OptTensor& t) { return t && t->defined() ? &*t : nullptr; }
 
 int dtype_of(const Tensor& t, const char* what) {
+  REQUIRE(!t.is_neg(), what, " is a lazily negated view: resolve_neg() it first");
   if (t.scalar_type() == at::kFloat) return SGPO_DTYPE_F32;
   REQUIRE(t.scalar_type() == at::kBFloat16, what, " must be float32 or bfloat16, got ", t.dtype());
   return SGPO_DTYPE_BF16;
@@ -131,7 +132,6 @@ variable_list rotate(Tensor q, Tensor k, const Tensor& freq, const Tensor& pos, 
     if (!x.defined()) continue;
     if (in_place) {
       REQUIRE(D <= 1 || x.stride(3) == 1, "in place, the elements of a head must be contiguous");
-      for (int i = 0; i < 4; ++i) REQUIRE(x.stride(i) != 0 || x.size(i) <= 1, "in place, heads must not be broadcast");
       out[w] = x;
     } else {
       if (D > 1 && x.stride(3) != 1) x = x.contiguous();
@@ -175,6 +175,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 };
 
 std::pair<Tensor, OptTensor> rotary_positions(const Tensor& q, const OptTensor& k, const Tensor& freq, const OptTensor& pos, bool interleaved, double scale) {
+  REQUIRE(!records({&freq}), "rotary_positions has no gradient for the frequencies: detach them");
   variable_list out;
   if (records({&q, opt(k)})) {
     out = Rotary::apply(q, k, freq, pos, interleaved, scale, false);
@@ -185,6 +186,7 @@ std::pair<Tensor, OptTensor> rotary_positions(const Tensor& q, const OptTensor& 
 }
 
 void rotary_positions_(const Tensor& q, const OptTensor& k, const Tensor& freq, const OptTensor& pos, bool interleaved, double scale) {
+  REQUIRE(!records({&freq}), "rotary_positions has no gradient for the frequencies: detach them");
   REQUIRE(!records({&q, opt(k)}), "rotary_positions_ has no gradient: use rotary_positions");
   rotate(q, k.value_or(Tensor()), freq, pos.value_or(Tensor()), interleaved, scale, false, true);
   // what autograd saved of them is stale now
@@ -193,8 +195,8 @@ void rotary_positions_(const Tensor& q, const OptTensor& k, const Tensor& freq, 
 }
 
 // ----------------------------------------------------------------------------------------------------------------- loss
-Tensor rows(const Tensor& t) {   // contiguous rows that do not overlap
-  return t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) ? t : t.contiguous();
+Tensor rows(const Tensor& t) {   // contiguous rows that do not overlap, of a pitch that the library takes
+  return t.stride(1) == 1 && (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) < 1 << 22)) ? t : t.contiguous();
 }
 
 sgpo_linear_ce_args ce_args(const Tensor& h, const Tensor& w, const Tensor& t, const Tensor& b, int64_t ignore, int64_t reduction) {
@@ -299,6 +301,7 @@ void check_table(const std::vector<float>& c, int64_t steps) {
 }
 
 Tensor newton_schulz(const Tensor& update, int64_t steps, const std::vector<float>& table, double eps) {
+  REQUIRE(!records({&update}), "newton_schulz has no gradient: detach the update, or call it under torch.no_grad()");
   const Call call({&update});
   const int dt = dtype_of(update, "update");
   REQUIRE(update.dim() >= 2, "an update is a matrix or a batch of them, got ", update.sizes());
@@ -320,13 +323,14 @@ Tensor newton_schulz(const Tensor& update, int64_t steps, const std::vector<floa
 
 void muon_step(const Tensor& weight, const Tensor& grad, const Tensor& buffer, double lr, double momentum, bool nesterov, double weight_decay, int64_t steps,
                const std::vector<float>& table, double eps) {
+  for (const Tensor* t : {&weight, &buffer})
+    REQUIRE(!records({t}) || t->is_leaf(), "weight or momentum_buffer is part of a graph: a step updates leaves");
   const Call call({&weight, &grad, &buffer});
   const int wd = dtype_of(weight, "weight"), gd = dtype_of(grad, "grad");
   REQUIRE(weight.dim() >= 2 && weight.sizes() == grad.sizes() && weight.sizes() == buffer.sizes(), "weight ", weight.sizes(), ", grad ", grad.sizes(), " and buffer ", buffer.sizes(),
           " must agree");
   REQUIRE(buffer.scalar_type() == at::kFloat, "momentum_buffer must be float32");
   REQUIRE(weight.is_contiguous() && buffer.is_contiguous(), "weight and momentum_buffer are updated in place and must be contiguous");
-  REQUIRE(!(at::GradMode::is_enabled() && weight.requires_grad() && !weight.is_leaf()), "weight is part of a graph: a step updates leaves");
   check_table(table, steps);
   if (!weight.numel()) return;
   at::AutoGradMode off(false);

@@ -669,7 +669,9 @@ Plan make_plan(const sgpo_linear_ce_args* a, bool backward) {
   q.n_kstep = q.h_pad / kstep;
   const bool whole = bf && a->H % 64 == 0;
   q.head = a->V <= 64;
-  q.turned = backward && bf && !q.head;      // both operands of dweight read by rows of k would be 1110 TFLOP/s, one of them 1440
+  // both operands of dweight read by rows of k would be 1110 TFLOP/s, one of them 1440; a row of the transposed features is a token long,
+  // and 256 of them have to lie within the 32-bit offsets of a tile's loads
+  q.turned = backward && bf && !q.head && a->N <= 1 << 22;
   q.w_direct = whole && a->ld_weight % 8 == 0 && aligned16(a->weight);
   // a product that reads the features by k (dweight's) needs zeros for ignored tokens: a packed copy, unless the transposed one has them
   q.h_direct = (!backward || q.turned) && whole && a->ld_hidden % 8 == 0 && aligned16(a->hidden);
@@ -724,6 +726,10 @@ int check_args(const sgpo_linear_ce_args* a) {
   SGPO_REQUIRE(a->ld_hidden >= a->H && a->ld_weight >= a->H && a->ld_hidden < (1 << 22) && a->ld_weight < (1 << 22), "linear_ce: bad row pitch %lld / %lld for H=%d",
                (long long)a->ld_hidden, (long long)a->ld_weight, a->H);
   return SGPO_OK;
+}
+
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {   // bytes; a null output overlaps nothing
+  return a && b && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
 
 int blocks_for(int64_t items) {
@@ -972,6 +978,10 @@ extern "C" int sgpo_linear_ce_backward(const sgpo_linear_ce_args* a, const float
   }
   SGPO_REQUIRE(a->hidden && a->weight && a->targets && lse && grad_out && workspace, "linear_ce_backward: null argument");
   SGPO_REQUIRE(a->reduction == SGPO_REDUCE_NONE || inv_count, "linear_ce_backward: null inv_count");
+  const int64_t esz = a->dtype == SGPO_DTYPE_BF16 ? 2 : 4, hb = (int64_t)a->N * a->H * esz, wb = (int64_t)a->V * a->H * esz;
+  const int64_t hin = ((a->N - 1) * a->ld_hidden + a->H) * esz, win = ((a->V - 1) * a->ld_weight + a->H) * esz;
+  SGPO_REQUIRE(!(overlap(dhidden, hb, a->hidden, hin) || overlap(dhidden, hb, a->weight, win) || overlap(dweight, wb, a->hidden, hin) || overlap(dweight, wb, a->weight, win) ||
+                 overlap(dhidden, hb, dweight, wb)), "linear_ce_backward: a gradient overlaps hidden, weight or the other gradient");
   const Plan q = make_plan(a, true);
   if (workspace_bytes < q.bytes) { sgpo_set_error("linear_ce_backward: workspace %zu < %zu", workspace_bytes, q.bytes); return SGPO_ERR_WORKSPACE; }
   const float* inv = a->reduction == SGPO_REDUCE_NONE ? nullptr : inv_count;

@@ -152,7 +152,8 @@ def test_rotation_of_nothing_and_refusals():
                 lambda: T.rotary_positions(q[..., :4], None, freq), lambda: T.rotary_positions(q, q[:1], freq),
                 lambda: T.rotary_positions(q, None, freq, torch.zeros(5, dtype=torch.int64)),
                 lambda: T.rotary_positions_(q[..., ::2], None, freq[:2]), lambda: T.rotary_positions_(q[:1].expand(2, 5, 2, 8), None, freq),
-                lambda: T.rotary_positions_(q.clone().requires_grad_(), None, freq)):
+                lambda: T.rotary_positions_(q.clone().requires_grad_(), None, freq), lambda: T.rotary_positions_(q, q, freq),
+                lambda: T.rotary_positions_(q[:, :4], q[:, 1:], freq), lambda: T.rotary_positions(torch._neg_view(q), None, freq)):
         with pytest.raises(L.SgpoError):
             bad()
 
@@ -264,6 +265,42 @@ def test_loss_in_several_pieces_and_tile_sizes():
     # 40000 tokens: pieces of 3355 -> 3328 classes, so 3 of 8000; the largest tiles
     _check_loss(40000, 64, 8000, BF, True, True, 0.4, 'mean', seed=9)
     _check_loss(9000, 96, 20000, F32, True, False, 0.4, 'mean', seed=10)
+
+
+def test_loss_of_more_tokens_than_a_tile_of_transposed_features_reaches():
+    # 256 rows of 8421600 bf16 tokens are over 2^32 bytes.  All but a few tokens are ignored, so that the sums stay short; those few are everywhere.
+    from sgpo_amd import train_ops as T
+    g = _gen(13)
+    N, H, V = 8421600, 64, 70
+    h = torch.randn(N, H, generator=g, device='cuda').to(BF).requires_grad_()
+    w = (torch.randn(V, H, generator=g, device='cuda') * H ** -0.5).to(BF).requires_grad_()
+    at = torch.cat([torch.randint(0, N, (500,), generator=g, device='cuda'), torch.tensor([0, N - 1], device='cuda')]).unique()
+    t = torch.full((N,), -100, device='cuda')
+    t[at] = torch.randint(0, V, (len(at),), generator=g, device='cuda')
+    out = T.linear_cross_entropy(h, w, t)
+    dh, dw = torch.autograd.grad(out, (h, w))
+    few = h.detach()[at].requires_grad_()
+    want = T.linear_cross_entropy(few, w, t[at])              # checked above against 64 bits
+    fh, fw = torch.autograd.grad(want, (few, w))
+    _within(out.detach(), want.detach(), 2 * U32 * want.detach().double(), 'loss')      # the same losses, summed in 64 bits
+    # the same d; its products' sums in another order, and each side's own rounding to bf16
+    z = few.detach().double() @ w.detach().double().T
+    d = (torch.softmax(z, 1) + torch.nn.functional.one_hot(t[at], V)) / len(at) * (1 + 2 ** -6)
+    _within(dh[at], fh, 2 * V * U32 * (d @ w.detach().double().abs()) + 2.01 * UBF * fh.double().abs(), 'dhidden')
+    _within(dw, fw, 2 * (len(at) + 70) * U32 * (d.T @ few.detach().double().abs()) + 2.01 * UBF * fw.double().abs(), 'dweight')
+    dh[at] = 0
+    assert int(dh.count_nonzero()) == 0
+    del h, dh
+    torch.cuda.empty_cache()
+
+
+def test_loss_of_rows_far_apart():
+    from sgpo_amd import train_ops as T
+    g = _gen(14)
+    far = torch.randn(3, 1 << 22, generator=g, device='cuda')
+    h, w = far[:, 5:69], torch.randn(40, 64, generator=g, device='cuda')
+    t = torch.tensor([1, 2, 39], device='cuda')
+    assert torch.equal(T.linear_cross_entropy(h, w, t), T.linear_cross_entropy(h.clone(), w, t))
 
 
 def test_loss_gradient_against_differences():
