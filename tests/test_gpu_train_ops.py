@@ -415,6 +415,29 @@ def test_newton_schulz(shape, dtype):
     assert torch.equal(got, T.newton_schulz(u))
 
 
+@pytest.mark.parametrize('tall', [False, True])
+def test_newton_schulz_of_the_longest_updates(tall):
+    # 200 x 2^22, zero but for some columns everywhere: the others' updates are those of the small matrix that is left
+    from sgpo_amd import train_ops as T
+    g = _gen(22)
+    n = 1 << 22
+    at = torch.cat([torch.randint(0, n, (300,), generator=g, device='cuda'), torch.tensor([0, n - 1], device='cuda')]).unique()
+    few = torch.randn(200, len(at), generator=g, device='cuda').to(BF)
+    u = torch.zeros((n, 200) if tall else (200, n), dtype=BF, device='cuda')
+    if tall:
+        u[at] = few.T
+    else:
+        u[:, at] = few
+    got = T.newton_schulz(u)
+    got = got.T if tall else got
+    want, err = _schulz64(few, [T.NS_COEFFICIENTS] * 5, 1e-7)
+    off = float((got[:, at].double() - want).norm())
+    assert off <= err + UBF * float(want.norm()) and off <= (UBF + 2.0 ** -9) * float(want.norm())
+    assert int(got.count_nonzero()) == int(got[:, at].count_nonzero())
+    del u, got
+    torch.cuda.empty_cache()
+
+
 def test_newton_schulz_properties():
     from sgpo_amd import _lib as L
     from sgpo_amd import train_ops as T
