@@ -228,14 +228,27 @@ __global__ __launch_bounds__(256) void join_kernel(Mats q, Slabs slabs, int cuts
   const float* src = slabs.out + (int64_t)b * q.d * slabs.pitch;
   for (int i = blockIdx.x * 256 + threadIdx.x; i < q.d * quads; i += gridDim.x * 256) {
     const int r = i / quads, c = (i - r * quads) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool upper = c / side >= r / side;
-    for (int k = 0; k < cuts; ++k) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < q.d) v[e] += src[k * stride + (upper ? (int64_t)r * slabs.pitch + c + e : (int64_t)(c + e) * slabs.pitch + r)];
+    if (c / side < r / side) continue;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (c < slabs.pitch) {
+      const float* at = src + (int64_t)r * slabs.pitch + c;
+#pragma unroll 8
+      for (int k = 0; k < cuts; ++k) v += *reinterpret_cast<const f32x4*>(at + k * stride);
     }
-    tg::store4<2, true>(q.G + b * q.sg + r * q.ldg, c, v);
+    const float w[4] = {c < q.d ? v[0] : 0.f, c + 1 < q.d ? v[1] : 0.f, c + 2 < q.d ? v[2] : 0.f, c + 3 < q.d ? v[3] : 0.f};
+    bf16_t* g = q.G + b * q.sg;
+    tg::store4<2, true>(g + r * q.ldg, c, w);
+    if (c / side > r / side) {   // the tile below the diagonal: 2-byte stores, where reading the sums transposed took 13 us (100 x 100, 32 cuts)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (c + e >= q.d) break;
+        float pl[2];
+        tg::split<2, true>(w[e], pl);
+        bf16_t* to = g + (c + e) * q.ldg + (r >> 5) * 64 + (r & 31);
+        to[0] = f2bf(pl[0]);
+        to[32] = f2bf(pl[1]);
+      }
+    }
   }
 }
 

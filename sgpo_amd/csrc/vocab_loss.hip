@@ -201,26 +201,51 @@ __global__ __launch_bounds__(256) void finish_kernel(const float2* part, int n_r
   }
 }
 
-// loss[0] = sum of nll (reduction 2) or its mean over the tokens with a loss (1; 0 if there are none); inv[0] = the factor on every token's gradient
-__global__ __launch_bounds__(1024) void total_kernel(const float* nll, const int64_t* targets, int64_t ignore, int N, int mean, float* loss, float* inv) {
+// loss[0] = sum of nll (reduction 2) or its mean over the tokens with a loss (1; 0 if there are none); inv[0] = the factor on every token's gradient.
+// Over TOTAL_ROWS tokens a workgroup to as many writes its part and one more adds the parts up (65536 tokens: 8.3 us; by one workgroup 20.6).
+constexpr int TOTAL_ROWS = 8192;
+struct Part { double sum; int64_t count; };
+__device__ __forceinline__ Part block_total(double s, int64_t c) {   // valid in thread 0
   __shared__ double ssum[16];
-  __shared__ int scnt[16];
-  double s = 0.0;
-  int c = 0;
-  for (int i = threadIdx.x; i < N; i += 1024) {
-    s += (double)nll[i];
-    c += targets[i] != ignore;
-  }
+  __shared__ int64_t scnt[16];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o); c += __shfl_xor(c, o); }
   if ((threadIdx.x & 63) == 0) { ssum[threadIdx.x >> 6] = s; scnt[threadIdx.x >> 6] = c; }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0)
     for (int i = 1; i < 16; ++i) { s += ssum[i]; c += scnt[i]; }
-    const int n = mean ? (c > 0 ? c : 1) : 1;
-    loss[0] = (float)(s / n);
-    inv[0] = 1.f / (float)n;
+  return Part{s, c};
+}
+__device__ __forceinline__ Part rows_total(const float* nll, const int64_t* targets, int64_t ignore, int64_t first, int n) {
+  double s = 0.0;
+  int64_t c = 0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    s += (double)nll[first + i];
+    c += targets[first + i] != ignore;
   }
+  return block_total(s, c);
+}
+__device__ __forceinline__ void store_total(const Part& p, int mean, float* loss, float* inv) {
+  const double n = mean ? (double)(p.count > 0 ? p.count : 1) : 1.0;
+  loss[0] = (float)(p.sum / n);
+  inv[0] = (float)(1.0 / n);
+}
+__global__ __launch_bounds__(1024) void total_kernel(const float* nll, const int64_t* targets, int64_t ignore, int N, int mean, float* loss, float* inv) {
+  const Part p = rows_total(nll, targets, ignore, 0, N);
+  if (threadIdx.x == 0) store_total(p, mean, loss, inv);
+}
+__global__ __launch_bounds__(1024) void parts_kernel(const float* nll, const int64_t* targets, int64_t ignore, int N, Part* parts) {
+  const int64_t first = (int64_t)blockIdx.x * TOTAL_ROWS;
+  const Part p = rows_total(nll, targets, ignore, first, (int)min((int64_t)TOTAL_ROWS, N - first));
+  if (threadIdx.x == 0) parts[blockIdx.x] = p;
+}
+__global__ __launch_bounds__(1024) void join_total_kernel(const Part* parts, int n, int mean, float* loss, float* inv) {
+  double s = 0.0;
+  int64_t c = 0;
+  for (int i = threadIdx.x; i < n; i += 1024) { s += parts[i].sum; c += parts[i].count; }
+  const Part p = block_total(s, c);
+  if (threadIdx.x == 0) store_total(p, mean, loss, inv);
 }
 
 // ----------------------------------------------------------------------------------------------------------- backward
@@ -572,8 +597,9 @@ __global__ __launch_bounds__(256) void sum_kernel(SumJobs jobs) {
     const int64_t i = i0 + o;
     float s = 0.f;
     if (i < p.total) {
-      const int64_t r = i / p.cols;
+      const int64_t r = p.total >> 32 ? i / p.cols : (uint32_t)i / (uint32_t)p.cols;
       const float* src = p.src + r * p.ld + (i - r * p.cols);
+#pragma unroll 8
       for (int k2 = g; k2 < p.n_slabs; k2 += p.spread) s += src[k2 * p.slab];
     }
     if (p.spread > 1) {
@@ -622,19 +648,25 @@ int pick(int PL, int64_t M, int64_t N) {
   return 0;
 }
 
-// A product's tile shape and the slabs its K is cut into: the least of rounds of the 256 CUs x (fixed + steps x step), and the slabs' sum at
-// 4 TB/s.  Costs of one tile in us, measured at 8192 x 2048 x 8192 (one plane) and x 2048 (three).
+// A product's tile shape and the slabs its K is cut into: the least of the CUs' rounds x (fixed + steps x step), and the slabs' sum.  A step costs
+// a workgroup of the smaller shapes less than twice as much where two share a CU: alone, it waits for memory.  Costs of one tile in us,
+// fitted to 138 products of 16 .. 65536 rows, 64 .. 2048 columns and 16 .. 131072 k at every shape and cut (one plane; three: 75): the pick is 4 % (1 %)
+// slower than the best one on average and 28 % at worst.
 struct Cut { int shape, splits; };
+struct Cost { double fixed1, step1, fixed2, step2; };   // one workgroup on a CU, and two (0: only one fits)
 Cut cut_for(int PL, int64_t M, int64_t N, int64_t nk) {
-  static const double step[2][3] = {{0.15, 0.50, 1.45}, {0.55, 1.16, 2.1}}, fixed[3] = {3.5, 5., 10.};
+  static const Cost cost[2][3] = {{{1., .38, 1.1, .50}, {1., .72, .6, 1.06}, {2.2, 1.51, 0., 0.}}, {{2.8, .47, .9, 1.16}, {.85, 1.23, 0., 0.}, {.85, 2.26, 0., 0.}}};
   static const int cuts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
   Cut best = {0, 1};
   double least = 1e300;
   for (int c = 0; c < 3; ++c)
     for (int s : cuts) {
       if (s > 1 && nk / s < 2) break;
-      const int64_t n = tiles(M, N, config_bm(PL, c), config_bn(PL, c)) * s;
-      const double t = (double)((n + 255) / 256) * (fixed[c] + (double)((nk + s - 1) / s) * step[PL == 3][c]) + (s > 1 ? 3. + (double)s * M * N * 8. / 4e6 : 0.);
+      const Cost& k = cost[PL == 3][c];
+      const int64_t steps = (nk + s - 1) / s, used = (nk + steps - 1) / steps, n = tiles(M, N, config_bm(PL, c), config_bn(PL, c)) * used;
+      const int64_t slots = k.step2 > 0. ? 512 : 256, rest = n % slots;
+      const double one = k.fixed1 + steps * k.step1, two = k.fixed2 + steps * k.step2;
+      const double t = (double)(n / slots) * (slots == 512 ? two : one) + (rest > 256 ? two : rest ? one : 0.) + (s > 1 ? 4. + (double)used * M * N * 4. * .4e-6 : 0.);
       if (t < least) { least = t; best = {c, s}; }
     }
   return best;
@@ -655,7 +687,7 @@ struct Plan {
   int64_t piece, piece_pad, n_pieces;        // backward: classes
   Cut h_cut, w_cut;                          // the two products
   bool head, turned;                         // at most 64 classes; the features also transposed
-  size_t off_h, off_w, off_t, off_part, off_at, off_d, off_acc, off_wacc, off_cs, bytes;
+  size_t off_h, off_w, off_t, off_part, off_at, off_d, off_acc, off_wacc, off_cs, off_total, bytes;
 };
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -683,6 +715,8 @@ Plan make_plan(const sgpo_linear_ce_args* a, bool backward) {
   q.off_w = take(q.w_direct ? 0 : (size_t)a->V * q.h_pad * q.PL * 2);
   q.off_t = take(q.turned ? (size_t)q.rows_pad * q.h_pad * 2 : 0);
   if (!backward) {
+    q.off_total = take(a->reduction != SGPO_REDUCE_NONE && a->N > TOTAL_ROWS ? (size_t)((a->N + TOTAL_ROWS - 1) / TOTAL_ROWS) * sizeof(Part) : 0);
+    q.bytes = at;
     if (q.head) return q;
     const int64_t tn_max = (a->V + 63) / 64;
     q.chunk = ((int64_t)1 << 24) / tn_max & ~(int64_t)255;
@@ -783,6 +817,18 @@ HeadArgs head_args(const sgpo_linear_ce_args* a, const Plan& q) {
   return p;
 }
 
+void total(const sgpo_linear_ce_args* a, const float* nll, float* loss, float* inv, char* parts, hipStream_t st) {
+  if (a->reduction == SGPO_REDUCE_NONE) return;
+  const int mean = a->reduction == SGPO_REDUCE_MEAN;
+  if (a->N <= TOTAL_ROWS) {
+    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, nll, a->targets, a->ignore_index, a->N, mean, loss, inv);
+    return;
+  }
+  const int n = (a->N + TOTAL_ROWS - 1) / TOTAL_ROWS;
+  hipLaunchKernelGGL(parts_kernel, dim3(n), dim3(1024), 0, st, nll, a->targets, a->ignore_index, a->N, (Part*)parts);
+  hipLaunchKernelGGL(join_total_kernel, dim3(1), dim3(1024), 0, st, (const Part*)parts, n, mean, loss, inv);
+}
+
 template <int PL>
 int forward(const sgpo_linear_ce_args* a, const Plan& q, float* nll, float* lse, float* loss, float* inv, char* ws, hipStream_t st) {
   if (q.head) {
@@ -790,8 +836,7 @@ int forward(const sgpo_linear_ce_args* a, const Plan& q, float* nll, float* lse,
     p.nll = nll; p.lse = lse;
     const int rc = PL == 1 ? head<bf16_t, false>(p, st) : head<float, false>(p, st);
     if (rc) return rc;
-    if (a->reduction != SGPO_REDUCE_NONE)
-      hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, nll, a->targets, a->ignore_index, a->N, a->reduction == SGPO_REDUCE_MEAN, loss, inv);
+    total(a, nll, loss, inv, ws + q.off_total, st);
     SGPO_CHECK_HIP(hipGetLastError());
     return SGPO_OK;
   }
@@ -821,8 +866,7 @@ int forward(const sgpo_linear_ce_args* a, const Plan& q, float* nll, float* lse,
     })
     hipLaunchKernelGGL(finish_kernel, dim3((n + 15) / 16), dim3(256), 0, st, part, n, tn, at, a->targets + r0, a->ignore_index, a->V, nll + r0, lse + r0);
   }
-  if (a->reduction != SGPO_REDUCE_NONE)
-    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, nll, a->targets, a->ignore_index, a->N, a->reduction == SGPO_REDUCE_MEAN, loss, inv);
+  total(a, nll, loss, inv, ws + q.off_total, st);
   SGPO_CHECK_HIP(hipGetLastError());
   return SGPO_OK;
 }
@@ -849,7 +893,7 @@ struct Sums {
   int n = 0;
   void add(const float* src, int64_t slab, int n_slabs, int64_t rows, int cols, int64_t ld, void* out, int out_bf16, Factor factor = Factor{nullptr, nullptr}) {
     const int64_t total = rows * cols;
-    const int spread = total >= 65536 || n_slabs < 8 ? 1 : n_slabs < 64 ? 8 : 32;
+    const int spread = total >= 65536 || n_slabs <= 16 ? 1 : n_slabs <= 128 ? 8 : 32;
     const int64_t blocks = (total * spread + 255) / 256;
     jobs.j[n++] = SumJob{src, out, slab, ld, total, n_slabs, cols, out_bf16, spread, (int)(blocks < 8192 ? blocks : 8192), factor};
   }
@@ -950,7 +994,7 @@ extern "C" int sgpo_linear_ce_forward(const sgpo_linear_ce_args* a, float* nll, 
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   SGPO_REQUIRE(a->reduction == SGPO_REDUCE_NONE || (loss && inv_count), "linear_ce_forward: null loss / inv_count");
   if (a->N == 0) {   // no token: no loss
-    if (a->reduction != SGPO_REDUCE_NONE) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, nll, a->targets, a->ignore_index, 0, a->reduction == SGPO_REDUCE_MEAN, loss, inv_count);
+    total(a, nll, loss, inv_count, nullptr, st);
     SGPO_CHECK_HIP(hipGetLastError());
     return SGPO_OK;
   }
