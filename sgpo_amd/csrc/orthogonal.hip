@@ -493,6 +493,214 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void apply_kernel(Mats q, int tm,
   }
 }
 
+// ------------------------------------------------------------------------------------------------ long and narrow updates
+// d <= 64 rows (or columns), more than 128 of the other: the iteration runs on d x d matrices.  X_k = Q_k X_0 with Q a polynomial in G_0 = X_0 X_0^T, all
+// of them symmetric and commuting, so that
+//   P = a I + b G + c G G,   Q <- P Q,   G <- P G P
+// needs nothing of length n: X_0 is read for G_0 and again for the result Q X_0.  G's rounding grows by a^2 per triple in the directions of small
+// singular values (where P's is read off it), so G is formed afresh from Q X_0 before that reaches GROWTH; five triples of the default: after three.
+// Everything in fp32 on the fp32 matrix instructions, whose rate does not count at this size (relative error of the result 1e-6 on Gaussian updates, 1e-4
+// on nearly rank-one ones; formed afresh at every triple the same, never 1e-6 and 1e-3).  Six launches instead of 17 to 22.
+constexpr int NARROW = 64, NARROW_CHUNK = 64, NARROW_PITCH = NARROW_CHUNK + 4;
+constexpr double GROWTH = 200.;
+struct NarrowArgs {
+  Source src;
+  const double* part;    // of the squared norm
+  int parts;
+  double eps;
+  int d, n, tall;        // shorter and longer side
+  float* Q;              // [batch][D][D], symmetric
+  float* sums;           // [batch][cuts][D][D]
+  int chunks, per, cuts;
+};
+
+// a chunk of 64 of the n columns of X_0 into T [D][NARROW_PITCH], zero beyond d and n; 256 threads
+template <typename T, int D>
+__device__ __forceinline__ void narrow_load(const NarrowArgs& p, int b, int chunk, float inv, float* tile) {
+  const Source& s = p.src;
+  const int j0 = chunk * NARROW_CHUNK;
+  constexpr int PER_ROW = NARROW_CHUNK / 4, PER_COL = D / 4;
+#pragma unroll
+  for (int k = 0; k < D * NARROW_CHUNK / 4 / 256; ++k) {
+    const int e = k * 256 + threadIdx.x;
+    const int i = p.tall ? e % PER_COL * 4 : e / PER_ROW, j = p.tall ? e / PER_COL : e % PER_ROW * 4;   // the first of four along a row of the update
+    const int r = p.tall ? j0 + j : i, c = p.tall ? i : j0 + j;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r < s.rows && c < s.cols) {
+      if (s.vec) {
+        const int64_t at = (int64_t)r * s.cols + c;
+        grad4<T>(reinterpret_cast<const T*>(s.grad) + b * s.stride_b + at, v);
+        if (s.buf) {
+          const f32x4 m = *reinterpret_cast<const f32x4*>(s.buf + (int64_t)b * s.rows * s.cols + at);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = s.nesterov ? fmaf(s.momentum, m[q], v[q]) : m[q];
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) if (c + q < s.cols) v[q] = update_at<T>(s, b, r, c + q);
+      }
+    }
+    if (p.tall) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tile[(i + q) * NARROW_PITCH + j] = v[q] * inv;
+    } else {
+      *reinterpret_cast<f32x4*>(tile + i * NARROW_PITCH + j) = f32x4{v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+    }
+  }
+}
+// K elements of a row as a fragment: lane (l16, l4) holds k = l4 * K / 4 .., the same for both operands
+template <int K>
+__device__ __forceinline__ void narrow_row(const float* row, int l4, float (&f)[K / 4]) {
+#pragma unroll
+  for (int q = 0; q < K / 16; ++q) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(row + l4 * (K / 4) + 4 * q);
+    f[4 * q] = v[0]; f[4 * q + 1] = v[1]; f[4 * q + 2] = v[2]; f[4 * q + 3] = v[3];
+  }
+}
+// tile <- Q tile in place; wave w takes columns 16 w ..
+template <int D>
+__device__ __forceinline__ void narrow_turn(const float* Q, float* tile) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4, j = ((int)threadIdx.x >> 6) * 16 + l16;
+  float f[D / 4];
+#pragma unroll
+  for (int k = 0; k < D / 4; ++k) f[k] = tile[(l4 * (D / 4) + k) * NARROW_PITCH + j];
+  f32x4 acc[D / 16];
+#pragma unroll
+  for (int x = 0; x < D / 16; ++x) {
+    float a[D / 4];
+    narrow_row<D>(Q + (x * 16 + l16) * (D + 4), l4, a);
+    acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < D / 4; ++k) acc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], f[k], acc[x], 0, 0, 0);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) tile[(x * 16 + 4 * l4 + q) * NARROW_PITCH + j] = acc[x][q];
+  __syncthreads();
+}
+template <int D>
+__device__ __forceinline__ void narrow_fetch(const float* from, float* Q) {
+  for (int e = threadIdx.x; e < D * D / 4; e += 256)
+    *reinterpret_cast<f32x4*>(Q + e / (D / 4) * (D + 4) + e % (D / 4) * 4) = *reinterpret_cast<const f32x4*>(from + e * 4);
+}
+
+// sums[b][cut] = X X^T over the cut's chunks, X = X_0 or Q X_0
+template <typename T, int D, bool TURN>
+__global__ __launch_bounds__(256) void narrow_gram_kernel(NarrowArgs p) {
+  __shared__ __attribute__((aligned(16))) float tile[D * NARROW_PITCH];
+  __shared__ __attribute__((aligned(16))) float Q[TURN ? D * (D + 4) : 4];
+  constexpr int SIDE = D / 16, MINE = SIDE * SIDE / 4;   // 16 x 16 tiles of the result, and of a wave
+  const int b = blockIdx.y, lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4, wave = (int)threadIdx.x >> 6;
+  const float inv = inverse_norm(p.part + b * PARTS, p.parts, p.eps);
+  if constexpr (TURN) narrow_fetch<D>(p.Q + (int64_t)b * D * D, Q);
+  f32x4 acc[MINE];
+#pragma unroll
+  for (int t = 0; t < MINE; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int first = blockIdx.x * p.per, last = min(first + p.per, p.chunks);
+  const int x = wave * MINE / SIDE, y0 = wave * MINE % SIDE;
+  for (int c = first; c < last; ++c) {
+    __syncthreads();
+    narrow_load<T, D>(p, b, c, inv, tile);
+    __syncthreads();
+    if constexpr (TURN) narrow_turn<D>(Q, tile);
+    float a[NARROW_CHUNK / 4], f[MINE][NARROW_CHUNK / 4];
+    narrow_row<NARROW_CHUNK>(tile + (x * 16 + l16) * NARROW_PITCH, l4, a);
+#pragma unroll
+    for (int t = 0; t < MINE; ++t) narrow_row<NARROW_CHUNK>(tile + ((y0 + t) * 16 + l16) * NARROW_PITCH, l4, f[t]);
+#pragma unroll
+    for (int k = 0; k < NARROW_CHUNK / 4; ++k)
+#pragma unroll
+      for (int t = 0; t < MINE; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], f[t][k], acc[t], 0, 0, 0);
+  }
+  float* out = p.sums + ((int64_t)b * p.cuts + blockIdx.x) * D * D;
+#pragma unroll
+  for (int t = 0; t < MINE; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) out[(x * 16 + 4 * l4 + q) * D + (y0 + t) * 16 + l16] = acc[t][q];
+}
+
+// the triples [k0, k1): Q <- P Q, G <- P G P; one workgroup per matrix, one wave per 16 x 16 tile.  Images hold symmetric matrices: a lane's four rows go out as
+// four columns, and columns are read as rows.
+template <int D>
+__global__ __launch_bounds__(4 * D / 16 * D) void narrow_poly_kernel(NarrowArgs p, Table coef, int k0, int k1) {
+  constexpr int PITCH = D + 4, SIDE = D / 16;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float *G = reinterpret_cast<float*>(smem), *P = G + D * PITCH, *M = P + D * PITCH, *Q = M + D * PITCH;
+  const int b = blockIdx.x, lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4, wave = (int)threadIdx.x >> 6, x = wave / SIDE, y = wave % SIDE;
+  auto product = [&](const float* A, const float* B) {
+    float a[D / 4], f[D / 4];
+    narrow_row<D>(A + (x * 16 + l16) * PITCH, l4, a);
+    narrow_row<D>(B + (y * 16 + l16) * PITCH, l4, f);
+    f32x4 even = {0.f, 0.f, 0.f, 0.f}, odd = even;   // two chains
+#pragma unroll
+    for (int k = 0; k < D / 4; k += 2) {
+      even = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], f[k], even, 0, 0, 0);
+      odd = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k + 1], f[k + 1], odd, 0, 0, 0);
+    }
+    return even + odd;
+  };
+  auto put = [&](float* img, const f32x4& v) { *reinterpret_cast<f32x4*>(img + (y * 16 + l16) * PITCH + x * 16 + 4 * l4) = v; };
+  const int row = x * 16 + 4 * l4, col = y * 16 + l16;
+  f32x4 g = {0.f, 0.f, 0.f, 0.f}, q = g;
+  const float* from = p.sums + (int64_t)b * p.cuts * D * D + row * D + col;
+#pragma unroll 4
+  for (int c = 0; c < p.cuts; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) g[e] += from[(int64_t)c * D * D + e * D];
+  put(G, g);
+  if (k0 > 0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = p.Q[(int64_t)b * D * D + (row + e) * D + col];
+    put(Q, q);
+  }
+  __syncthreads();
+  for (int k = k0; k < k1; ++k) {
+    const float ca = coef.v[3 * k], cb = coef.v[3 * k + 1], cc = coef.v[3 * k + 2];
+    f32x4 h = product(G, G);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = fmaf(cb, g[e], cc * h[e]) + (row + e == col ? ca : 0.f);
+    put(P, h);
+    __syncthreads();
+    q = k > 0 ? product(P, Q) : h;
+    if (k + 1 == k1) break;
+    put(M, product(P, G));
+    __syncthreads();
+    g = product(P, M);
+    put(Q, q);
+    put(G, g);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) p.Q[(int64_t)b * D * D + (row + e) * D + col] = q[e];
+}
+
+// the result: Q X_0
+template <typename T, int D>
+__global__ __launch_bounds__(256) void narrow_apply_kernel(NarrowArgs p, Result res) {
+  __shared__ __attribute__((aligned(16))) float tile[D * NARROW_PITCH];
+  __shared__ __attribute__((aligned(16))) float Q[D * (D + 4)];
+  const int b = blockIdx.y, chunk = blockIdx.x, j0 = chunk * NARROW_CHUNK;
+  const float inv = inverse_norm(p.part + b * PARTS, p.parts, p.eps);
+  narrow_fetch<D>(p.Q + (int64_t)b * D * D, Q);
+  narrow_load<T, D>(p, b, chunk, inv, tile);
+  __syncthreads();
+  narrow_turn<D>(Q, tile);
+  constexpr int PER_ROW = NARROW_CHUNK / 4, PER_COL = D / 4;
+#pragma unroll
+  for (int k = 0; k < D * NARROW_CHUNK / 4 / 256; ++k) {
+    const int e = k * 256 + threadIdx.x;
+    const int i = p.tall ? e % PER_COL * 4 : e / PER_ROW, j = p.tall ? e / PER_COL : e % PER_ROW * 4;
+    const int r = p.tall ? j0 + j : i, c = p.tall ? i : j0 + j;
+    if (r >= res.rows || c >= res.cols) continue;
+    float v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = p.tall ? tile[(i + q) * NARROW_PITCH + j] : tile[i * NARROW_PITCH + j + q];
+    store_result(res, b, r, c, v);
+  }
+}
+
 template <typename K>
 int allow_lds(K kernel, int bytes) {
   SGPO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
@@ -574,12 +782,29 @@ int apply_any(int kind, const Mats& q, int batch, const Result& r, hipStream_t s
 }
 
 constexpr int CUTS = 32;
-struct Sizes { int d, longer; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, off_s, bytes; Pick gram, poly, full; };
+constexpr int NARROW_MOST = 1 << 15;
+struct Sizes { int d, longer, narrow, chunks, per, cuts; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, off_s, bytes; Pick gram, poly, full; };
 Sizes sizes(int batch, int rows, int cols) {
   Sizes s = {};
   s.d = rows < cols ? rows : cols;
   s.longer = rows < cols ? cols : rows;
   if (s.longer <= 128) return s;   // one launch, no scratch
+  if (s.d <= NARROW && s.longer <= NARROW_MOST) {
+    // a cut costs a workgroup its chunks one after the other (about 1 us each) and the one that adds the cuts up 16 KB of each (0.15 us)
+    s.narrow = s.d <= 32 ? 32 : 64;
+    s.chunks = (s.longer + NARROW_CHUNK - 1) / NARROW_CHUNK;
+    int64_t cuts = (int64_t)(sqrt(6. * s.chunks) + 1.);
+    if (cuts > 1024 / batch) cuts = 1024 / batch;
+    if (cuts > s.chunks) cuts = s.chunks;
+    if (cuts < 1) cuts = 1;
+    s.per = (int)((s.chunks + cuts - 1) / cuts);
+    s.cuts = (s.chunks + s.per - 1) / s.per;
+    const size_t one = (size_t)batch * s.narrow * s.narrow * 4;
+    s.off_g = (size_t)batch * PARTS * 8;
+    s.off_s = s.off_g + one;
+    s.bytes = s.off_s + one * s.cuts;
+    return s;
+  }
   s.ldx = round_up(cols, 32) * 2;
   s.ldg = round_up(s.d, 32) * 2;
   s.x = (size_t)rows * s.ldx; s.g = (size_t)s.d * s.ldg;
@@ -610,6 +835,28 @@ int orthogonalise_small(const Source& src, int batch, const float* coef, int ste
   return SGPO_OK;
 }
 
+template <typename T, int D>
+int orthogonalise_narrow(const NarrowArgs& p, int batch, const float* coef, int steps, const Result& res, hipStream_t st) {
+  Table t = {};
+  for (int i = 0; i < 3 * steps; ++i) t.v[i] = coef[i];
+  constexpr int LDS = 4 * D * (D + 4) * 4;
+  ALLOW((narrow_poly_kernel<D>), LDS);
+  for (int k0 = 0, k1; k0 < steps; k0 = k1) {
+    double grown = 1.;
+    for (k1 = k0 + 1; k1 < steps; ++k1) {
+      const double a = fabs(t.v[3 * k1 - 3]), top = fabs(t.v[3 * k1 - 3] + t.v[3 * k1 - 2] + t.v[3 * k1 - 1]);   // |P| at 0 and at 1
+      grown *= a > top ? a * a : top * top;
+      if (!(grown < GROWTH)) break;
+    }
+    if (k0 == 0) hipLaunchKernelGGL((narrow_gram_kernel<T, D, false>), dim3(p.cuts, batch), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((narrow_gram_kernel<T, D, true>), dim3(p.cuts, batch), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((narrow_poly_kernel<D>), dim3(batch), dim3(D / 16 * D * 4), LDS, st, p, t, k0, k1);
+  }
+  hipLaunchKernelGGL((narrow_apply_kernel<T, D>), dim3(p.chunks, batch), dim3(256), 0, st, p, res);
+  SGPO_CHECK_HIP(hipGetLastError());
+  return SGPO_OK;
+}
+
 template <typename T>
 int orthogonalise(Source src, int batch, const float* coef, int steps, double eps, Result res, char* ws, hipStream_t st) {
   const Sizes z = sizes(batch, src.rows, src.cols);
@@ -625,6 +872,10 @@ int orthogonalise(Source src, int batch, const float* coef, int steps, double ep
   const int64_t want = ((int64_t)src.rows * src.cols + 1023) / 1024;
   const int parts = want < PARTS ? (int)want : PARTS;
   hipLaunchKernelGGL((square_kernel<T>), dim3(parts, batch), dim3(256), 0, st, src, part);
+  if (z.narrow) {
+    const NarrowArgs p{src, part, parts, eps, z.d, z.longer, tall, (float*)(ws + z.off_g), (float*)(ws + z.off_s), z.chunks, z.per, z.cuts};
+    return z.narrow == 32 ? orthogonalise_narrow<T, 32>(p, batch, coef, steps, res, st) : orthogonalise_narrow<T, 64>(p, batch, coef, steps, res, st);
+  }
   const int64_t blocks = ((int64_t)src.rows * (z.ldx / 8) + 255) / 256;
   // Each workgroup adds up the norm's parts first, so the device is filled once and not more (six 384 x 1536 bf16: 22.3 us with up to 4096 a matrix, 16.1 so).
   const int64_t most = batch < 32 ? 2048 / batch : 64;

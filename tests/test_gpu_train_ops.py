@@ -397,7 +397,8 @@ def _schulz64(u, coefficients, eps):
 
 
 ORTHO = [((8, 8), F32), ((1, 1), F32), ((1, 40), BF), ((40, 1), F32), ((64, 64), F32), ((33, 65), BF), ((100, 70), F32), ((200, 130), BF), ((130, 517), F32),
-         ((513, 129), BF), ((512, 2048), BF), ((1536, 512), F32), ((3, 64, 48), F32), ((2, 2, 150, 40), BF), ((3, 64, 4000), F32), ((5000, 70), BF), ((2, 150, 9000), BF)]
+         ((513, 129), BF), ((512, 2048), BF), ((1536, 512), F32), ((3, 64, 48), F32), ((2, 2, 150, 40), BF), ((3, 64, 4000), F32), ((5000, 70), BF), ((2, 150, 9000), BF),
+         ((31, 512), F32), ((512, 31), BF), ((7, 200), F32), ((1, 129), BF), ((1003, 17), F32), ((3, 64, 129), BF), ((2, 33, 4100), F32), ((30000, 64), BF), ((3, 40000), F32)]
 
 
 @pytest.mark.parametrize('shape,dtype', ORTHO)
@@ -413,6 +414,24 @@ def test_newton_schulz(shape, dtype):
         # away from the bound, as sharp as the output's type: iterates are 2^-16 wide and random in sign
         assert off <= (UBF + 2.0 ** -9) * float(want.norm()), (off, float(want.norm()))
     assert torch.equal(got, T.newton_schulz(u))
+
+
+@pytest.mark.parametrize('shape', [(40, 60), (64, 300), (700, 20), (100, 900)])
+def test_newton_schulz_of_uneven_spectra_and_other_tables(shape):
+    # nearly one direction; singular values over six orders; and one to nine triples, whose products grow small ones by up to 5^2 each
+    from sgpo_amd import train_ops as T
+    g = _gen(23)
+    m, n = shape
+    d = min(shape)
+    noise = torch.randn(shape, generator=g, device='cuda')
+    a, b = torch.randn(m, 1, generator=g, device='cuda'), torch.randn(1, n, generator=g, device='cuda')
+    left, right = torch.linalg.qr(torch.randn(m, d, generator=g, device='cuda').double())[0], torch.linalg.qr(torch.randn(n, d, generator=g, device='cuda').double())[0]
+    spread = (left * torch.logspace(0, -6, d, dtype=torch.float64, device='cuda')) @ right.T
+    for u in (a @ b + 1e-3 * noise, spread.float()):
+        for table in ([T.NS_COEFFICIENTS], [T.NS_COEFFICIENTS] * 5, [(5.0, -9.0, 4.5)] * 4, [(15 / 8, -10 / 8, 3 / 8)] * 9):
+            want, err = _schulz64(u, table, 1e-7)
+            off = float((T.newton_schulz(u, steps=len(table), coefficients=table).double() - want).norm())
+            assert off <= err + UBF * float(want.norm()), (off, err, float(want.norm()))
 
 
 @pytest.mark.parametrize('tall', [False, True])
@@ -468,7 +487,8 @@ def test_newton_schulz_properties():
             bad()
 
 
-@pytest.mark.parametrize('wdt,gdt,shape,nesterov', [(F32, F32, (96, 64), True), (F32, BF, (64, 200), False), (BF, BF, (2, 130, 70), True), (BF, F32, (512, 512), True)])
+@pytest.mark.parametrize('wdt,gdt,shape,nesterov', [(F32, F32, (96, 64), True), (F32, BF, (64, 200), False), (BF, BF, (2, 130, 70), True), (BF, F32, (512, 512), True),
+                                                      (F32, F32, (31, 512), True), (BF, F32, (3, 400, 24), False), (F32, BF, (50, 333), True)])
 def test_muon_step(wdt, gdt, shape, nesterov):
     from sgpo_amd import train_ops as T
     g = _gen(31)
