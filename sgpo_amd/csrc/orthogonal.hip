@@ -494,7 +494,7 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void apply_kernel(Mats q, int tm,
 }
 
 // ------------------------------------------------------------------------------------------------ long and narrow updates
-// d <= 64 rows (or columns), more than 128 of the other: the iteration runs on d x d matrices.  X_k = Q_k X_0 with Q a polynomial in G_0 = X_0 X_0^T, all
+// At most 64 rows (or columns) and more of the other: the iteration runs on d x d matrices.  X_k = Q_k X_0 with Q a polynomial in G_0 = X_0 X_0^T, all
 // of them symmetric and commuting, so that
 //   P = a I + b G + c G G,   Q <- P Q,   G <- P G P
 // needs nothing of length n: X_0 is read for G_0 and again for the result Q X_0.  G's rounding grows by a^2 per triple in the directions of small
@@ -514,18 +514,26 @@ struct NarrowArgs {
   int chunks, per, cuts;
 };
 
-// a chunk of 64 of the n columns of X_0 into T [D][NARROW_PITCH], zero beyond d and n; 256 threads
+// a chunk of 64 of the n columns of X_0: four elements along a row of the update at a time, zero beyond it; 256 threads
+template <int D> struct Chunk { float v[D * NARROW_CHUNK / 4 / 256][4]; };
+template <int D>
+__device__ __forceinline__ void narrow_place(bool tall, int k, int& i, int& j) {   // the k-th quad's first element: short index, and long one within the chunk
+  const int e = k * 256 + threadIdx.x;
+  i = tall ? e % (D / 4) * 4 : e / (NARROW_CHUNK / 4);
+  j = tall ? e / (D / 4) : e % (NARROW_CHUNK / 4) * 4;
+}
 template <typename T, int D>
-__device__ __forceinline__ void narrow_load(const NarrowArgs& p, int b, int chunk, float inv, float* tile) {
+__device__ __forceinline__ void narrow_load(const NarrowArgs& p, int b, int chunk, Chunk<D>& to) {
   const Source& s = p.src;
   const int j0 = chunk * NARROW_CHUNK;
-  constexpr int PER_ROW = NARROW_CHUNK / 4, PER_COL = D / 4;
 #pragma unroll
   for (int k = 0; k < D * NARROW_CHUNK / 4 / 256; ++k) {
-    const int e = k * 256 + threadIdx.x;
-    const int i = p.tall ? e % PER_COL * 4 : e / PER_ROW, j = p.tall ? e / PER_COL : e % PER_ROW * 4;   // the first of four along a row of the update
+    int i, j;
+    narrow_place<D>(p.tall, k, i, j);
     const int r = p.tall ? j0 + j : i, c = p.tall ? i : j0 + j;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    float (&v)[4] = to.v[k];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = 0.f;
     if (r < s.rows && c < s.cols) {
       if (s.vec) {
         const int64_t at = (int64_t)r * s.cols + c;
@@ -540,6 +548,16 @@ __device__ __forceinline__ void narrow_load(const NarrowArgs& p, int b, int chun
         for (int q = 0; q < 4; ++q) if (c + q < s.cols) v[q] = update_at<T>(s, b, r, c + q);
       }
     }
+  }
+}
+// into tile [D][NARROW_PITCH]: short index, long index
+template <int D>
+__device__ __forceinline__ void narrow_put(const NarrowArgs& p, const Chunk<D>& from, float inv, float* tile) {
+#pragma unroll
+  for (int k = 0; k < D * NARROW_CHUNK / 4 / 256; ++k) {
+    int i, j;
+    narrow_place<D>(p.tall, k, i, j);
+    const float (&v)[4] = from.v[k];
     if (p.tall) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) tile[(i + q) * NARROW_PITCH + j] = v[q] * inv;
@@ -600,10 +618,13 @@ __global__ __launch_bounds__(256) void narrow_gram_kernel(NarrowArgs p) {
   for (int t = 0; t < MINE; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int first = blockIdx.x * p.per, last = min(first + p.per, p.chunks);
   const int x = wave * MINE / SIDE, y0 = wave * MINE % SIDE;
+  Chunk<D> next;
+  narrow_load<T, D>(p, b, first, next);
   for (int c = first; c < last; ++c) {
     __syncthreads();
-    narrow_load<T, D>(p, b, c, inv, tile);
+    narrow_put<D>(p, next, inv, tile);
     __syncthreads();
+    if (c + 1 < last) narrow_load<T, D>(p, b, c + 1, next);   // on its way while this one is multiplied
     if constexpr (TURN) narrow_turn<D>(Q, tile);
     float a[NARROW_CHUNK / 4], f[MINE][NARROW_CHUNK / 4];
     narrow_row<NARROW_CHUNK>(tile + (x * 16 + l16) * NARROW_PITCH, l4, a);
@@ -684,14 +705,15 @@ __global__ __launch_bounds__(256) void narrow_apply_kernel(NarrowArgs p, Result 
   const int b = blockIdx.y, chunk = blockIdx.x, j0 = chunk * NARROW_CHUNK;
   const float inv = inverse_norm(p.part + b * PARTS, p.parts, p.eps);
   narrow_fetch<D>(p.Q + (int64_t)b * D * D, Q);
-  narrow_load<T, D>(p, b, chunk, inv, tile);
+  Chunk<D> here;
+  narrow_load<T, D>(p, b, chunk, here);
+  narrow_put<D>(p, here, inv, tile);
   __syncthreads();
   narrow_turn<D>(Q, tile);
-  constexpr int PER_ROW = NARROW_CHUNK / 4, PER_COL = D / 4;
 #pragma unroll
   for (int k = 0; k < D * NARROW_CHUNK / 4 / 256; ++k) {
-    const int e = k * 256 + threadIdx.x;
-    const int i = p.tall ? e % PER_COL * 4 : e / PER_ROW, j = p.tall ? e / PER_COL : e % PER_ROW * 4;
+    int i, j;
+    narrow_place<D>(p.tall, k, i, j);
     const int r = p.tall ? j0 + j : i, c = p.tall ? i : j0 + j;
     if (r >= res.rows || c >= res.cols) continue;
     float v[4];
@@ -782,18 +804,21 @@ int apply_any(int kind, const Mats& q, int batch, const Result& r, hipStream_t s
 }
 
 constexpr int CUTS = 32;
+// Where the matrices of at most 64 x 64 take over (us, before and with): d <= 32 from 65 on (31 x 128: 31.6, 22.2), d <= 64 from 129 on (64 x 128 in
+// one launch 38.9, 42.3 this way) up to 32768 (64 x 32768: 124, 105; the one workgroup that adds up the cuts grows with the length's root).
 constexpr int NARROW_MOST = 1 << 15;
 struct Sizes { int d, longer, narrow, chunks, per, cuts; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, off_s, bytes; Pick gram, poly, full; };
 Sizes sizes(int batch, int rows, int cols) {
   Sizes s = {};
   s.d = rows < cols ? rows : cols;
   s.longer = rows < cols ? cols : rows;
-  if (s.longer <= 128) return s;   // one launch, no scratch
-  if (s.d <= NARROW && s.longer <= NARROW_MOST) {
-    // a cut costs a workgroup its chunks one after the other (about 1 us each) and the one that adds the cuts up 16 KB of each (0.15 us)
+  const bool narrow = s.d <= NARROW && s.longer > (s.d <= 32 ? 64 : 128) && s.longer <= NARROW_MOST;
+  if (s.longer <= 128 && !narrow) return s;   // one launch, no scratch
+  if (narrow) {
+    // a cut costs its workgroup a chunk after the other, and the one that adds the cuts up 16 KB of each (64 x 4096: 20 cuts 58.6 us, 32 58.7)
     s.narrow = s.d <= 32 ? 32 : 64;
     s.chunks = (s.longer + NARROW_CHUNK - 1) / NARROW_CHUNK;
-    int64_t cuts = (int64_t)(sqrt(6. * s.chunks) + 1.);
+    int64_t cuts = (int64_t)(sqrt(10. * s.chunks) + 1.);
     if (cuts > 1024 / batch) cuts = 1024 / batch;
     if (cuts > s.chunks) cuts = s.chunks;
     if (cuts < 1) cuts = 1;
@@ -863,7 +888,7 @@ int orthogonalise(Source src, int batch, const float* coef, int steps, double ep
   res.rows = src.rows; res.cols = src.cols;
   res.vec = src.cols % 4 == 0 && (uintptr_t)res.out % (res.out_bf16 ? 8 : 16) == 0;
   if (z.longer <= 64) return orthogonalise_small<T, 64>(src, batch, coef, steps, eps, res, st);
-  if (z.longer <= 128) return orthogonalise_small<T, 128>(src, batch, coef, steps, eps, res, st);
+  if (z.longer <= 128 && !z.narrow) return orthogonalise_small<T, 128>(src, batch, coef, steps, eps, res, st);
   double* part = reinterpret_cast<double*>(ws);
   Mats q{(bf16_t*)(ws + z.off_x), (bf16_t*)(ws + z.off_y), (bf16_t*)(ws + z.off_g), (bf16_t*)(ws + z.off_p), z.ldx, z.ldg, (int64_t)z.x, (int64_t)z.g, src.rows, src.cols, z.d};
   const bool tall = src.rows > src.cols;

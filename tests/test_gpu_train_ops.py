@@ -398,7 +398,7 @@ def _schulz64(u, coefficients, eps):
 
 ORTHO = [((8, 8), F32), ((1, 1), F32), ((1, 40), BF), ((40, 1), F32), ((64, 64), F32), ((33, 65), BF), ((100, 70), F32), ((200, 130), BF), ((130, 517), F32),
          ((513, 129), BF), ((512, 2048), BF), ((1536, 512), F32), ((3, 64, 48), F32), ((2, 2, 150, 40), BF), ((3, 64, 4000), F32), ((5000, 70), BF), ((2, 150, 9000), BF),
-         ((31, 512), F32), ((512, 31), BF), ((7, 200), F32), ((1, 129), BF), ((1003, 17), F32), ((3, 64, 129), BF), ((2, 33, 4100), F32), ((30000, 64), BF), ((3, 40000), F32)]
+         ((31, 512), F32), ((512, 31), BF), ((7, 200), F32), ((1, 129), BF), ((20, 65), BF), ((128, 32), F32), ((33, 128), F32), ((1003, 17), F32), ((3, 64, 129), BF), ((2, 33, 4100), F32), ((30000, 64), BF), ((3, 40000), F32)]
 
 
 @pytest.mark.parametrize('shape,dtype', ORTHO)
