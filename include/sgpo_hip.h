@@ -368,7 +368,8 @@ int sgpo_daps_mh(sgpo_mlp* m, const int64_t* x0hat, int N, int L, int S, const i
 
 /* ---- training operators of a denoiser ---------------------------------------------------------
  * The reference trains its denoisers through torch autograd (models/pretraining/trainer.py); these are the pieces of such a
- * step that torch would run as chains of memory-bound kernels or not in one piece at all.  Types: fp32 or bf16. */
+ * step that torch would run as chains of memory-bound kernels or not in one piece at all.  Types: fp32 or bf16.
+ * Workspaces are 256-byte aligned. */
 #define SGPO_DTYPE_F32 0
 #define SGPO_DTYPE_BF16 1
 

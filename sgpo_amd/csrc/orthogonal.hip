@@ -767,7 +767,7 @@ typedef tg::Shape<64, 64, 2, 2, 2, 2, 2> Shape64;
 typedef tg::Shape<32, 32, 1, 1, 2, 2, 4> Shape32;
 
 // The kind with the least rounds of the 256 CUs x cost of a tile; count(side) tiles of `steps` K steps.  A symmetric product with few tiles and a
-// long K may also be cut along K (at most `cuts` times), which costs the joining launch and its bytes (64 x 7616, ten of them: 45 -> 13 us).
+// long K may also be cut along K (at most `cuts` times), which costs the joining launch and its bytes (two of 150 x 9000, the whole call: 313 us whole, 158 cut).
 struct Pick { int kind, cuts; };
 template <typename F>
 Pick pick(F count, int64_t steps, bool sym, int most_cuts = 1, double joined_bytes = 0.) {
@@ -956,6 +956,7 @@ extern "C" int sgpo_newton_schulz(const void* update, int dtype, int batch, int 
   SGPO_REQUIRE(update && out, "newton_schulz: null argument");
   SGPO_REQUIRE(ld >= cols || rows == 1, "newton_schulz: row pitch %lld below %d columns", (long long)ld, cols);
   const size_t need = sgpo_newton_schulz_workspace_bytes(batch, rows, cols);
+  SGPO_REQUIRE((uintptr_t)workspace % 256 == 0, "newton_schulz: the workspace must be 256-byte aligned");
   if (need && (!workspace || workspace_bytes < need)) { sgpo_set_error("newton_schulz: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
   const int esz = dtype == SGPO_DTYPE_BF16 ? 2 : 4;
   SGPO_REQUIRE(stride_b >= 0 && !overlap(update, ((batch - 1) * stride_b + (rows - 1) * ld + cols) * esz, out, (int64_t)batch * rows * cols * 2), "newton_schulz: out overlaps update");
@@ -976,6 +977,7 @@ extern "C" int sgpo_muon_step(void* weight, int weight_dtype, const void* grad, 
   if (!batch || !rows || !cols) return SGPO_OK;
   SGPO_REQUIRE(weight && grad && momentum_buffer, "muon_step: null argument");
   const size_t need = sgpo_newton_schulz_workspace_bytes(batch, rows, cols);
+  SGPO_REQUIRE((uintptr_t)workspace % 256 == 0, "muon_step: the workspace must be 256-byte aligned");
   if (need && (!workspace || workspace_bytes < need)) { sgpo_set_error("muon_step: workspace %zu < %zu", workspace_bytes, need); return SGPO_ERR_WORKSPACE; }
   const int64_t n = (int64_t)batch * rows * cols, wb = n * (weight_dtype == SGPO_DTYPE_BF16 ? 2 : 4), gb = n * (grad_dtype == SGPO_DTYPE_BF16 ? 2 : 4);
   SGPO_REQUIRE(!overlap(weight, wb, grad, gb) && !overlap(weight, wb, momentum_buffer, n * 4) && !overlap(grad, gb, momentum_buffer, n * 4),

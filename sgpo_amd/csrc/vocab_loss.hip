@@ -274,7 +274,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void grad_kernel(LossArgs p, int tm,
 #pragma unroll
     for (int q = 0; q < 4; ++q) cs[y][q] = 0.f;
   // The planes of XG row blocks at a time pass through this wave's part of the LDS, so that they leave in whole lines: from the registers a
-  // row would go out in pieces of 32 bytes (a piece of 8192 x 16384: 610 us with those).
+  // row would go out in pieces of 32 bytes (a piece of 8192 x 16384: 610 us with those, 506 so).
   constexpr int RB = S::NT * 32 * S::PL, CH = RB / 16, MASK = CH % 8 == 0 ? 7 : 3;   // bytes and 16-B chunks of a wave's row
   constexpr int PART = S::LDS / (S::WM * S::WN), FIT = PART / (16 * RB), XG = FIT >= S::MT ? S::MT : FIT >= S::MT / 2 ? S::MT / 2 : 1;
   static_assert(XG * 16 * RB <= PART && S::MT % XG == 0, "a row block fits the wave's part");
@@ -1000,6 +1000,7 @@ extern "C" int sgpo_linear_ce_forward(const sgpo_linear_ce_args* a, float* nll, 
   }
   SGPO_REQUIRE(a->hidden && a->weight && a->targets && nll && lse, "linear_ce_forward: null argument");
   const Plan q = make_plan(a, false);
+  SGPO_REQUIRE((uintptr_t)workspace % 256 == 0, "linear_ce_forward: the workspace must be 256-byte aligned");
   if (q.bytes && (!workspace || workspace_bytes < q.bytes)) { sgpo_set_error("linear_ce_forward: workspace %zu < %zu", workspace_bytes, q.bytes); return SGPO_ERR_WORKSPACE; }
   return q.PL == 1 ? forward<1>(a, q, nll, lse, loss, inv_count, (char*)workspace, st) : forward<3>(a, q, nll, lse, loss, inv_count, (char*)workspace, st);
 }
@@ -1027,6 +1028,7 @@ extern "C" int sgpo_linear_ce_backward(const sgpo_linear_ce_args* a, const float
   SGPO_REQUIRE(!(overlap(dhidden, hb, a->hidden, hin) || overlap(dhidden, hb, a->weight, win) || overlap(dweight, wb, a->hidden, hin) || overlap(dweight, wb, a->weight, win) ||
                  overlap(dhidden, hb, dweight, wb)), "linear_ce_backward: a gradient overlaps hidden, weight or the other gradient");
   const Plan q = make_plan(a, true);
+  SGPO_REQUIRE((uintptr_t)workspace % 256 == 0, "linear_ce_backward: the workspace must be 256-byte aligned");
   if (workspace_bytes < q.bytes) { sgpo_set_error("linear_ce_backward: workspace %zu < %zu", workspace_bytes, q.bytes); return SGPO_ERR_WORKSPACE; }
   const float* inv = a->reduction == SGPO_REDUCE_NONE ? nullptr : inv_count;
   return q.PL == 1 ? backward<1>(a, q, lse, grad_out, inv, dhidden, dweight, dbias, (char*)workspace, st)

@@ -88,7 +88,13 @@ def test_library_refuses_bad_arguments_without_a_device():
     one = C.c_void_p(4096)                                       # never read: the workspace is refused first
     refused(lib.sgpo_linear_ce_forward(C.byref(L.LinearCeArgs(hidden=4096, weight=4096, targets=4096, N=4, H=8, V=500, ld_hidden=8, ld_weight=8)),
                                        one, one, one, one, one, 16, None), 'workspace')
+    odd = C.c_void_p(4096 + 128)
+    big = L.LinearCeArgs(hidden=1 << 30, weight=1 << 31, targets=4096, N=4, H=8, V=500, ld_hidden=8, ld_weight=8)
+    refused(lib.sgpo_linear_ce_forward(C.byref(big), one, one, one, one, odd, 1 << 40, None), 'aligned')
+    refused(lib.sgpo_linear_ce_backward(C.byref(big), one, one, one, None, None, one, odd, 1 << 40, None), 'aligned')
     coef = (C.c_float * 3)(1, 0, 0)
+    refused(lib.sgpo_newton_schulz(one, 0, 1, 400, 4, 1600, 4, coef, 1, 1e-7, one, odd, 1 << 30, None), 'aligned')
+    refused(lib.sgpo_muon_step(one, 0, one, 0, one, 1, 400, 4, 0.1, 0.9, 1, 0.0, coef, 1, 1e-7, odd, 1 << 30, None), 'aligned')
     refused(lib.sgpo_newton_schulz(one, 0, 1, 4, 4, 16, 4, coef, 0, 1e-7, one, one, 1 << 30, None), 'triples')
     refused(lib.sgpo_newton_schulz(one, 5, 1, 4, 4, 16, 4, coef, 1, 1e-7, one, one, 1 << 30, None), 'dtype')
     refused(lib.sgpo_newton_schulz(one, 0, 1, 4, 4, 16, 3, coef, 1, 1e-7, one, one, 1 << 30, None), 'pitch')
