@@ -587,6 +587,75 @@ def test_captured_graphs_replay_with_new_inputs():
             assert all(torch.equal(x, y) for x, y in zip(out, want)), r
 
 
+@pytest.mark.parametrize('V,shape', [(31, (31, 512)), (26, (3, 700, 40)), (100, (48, 48)), (70, (2, 96, 3000))])
+def test_captured_graphs_of_heads_many_tokens_and_narrow_updates(V, shape):
+    from sgpo_amd import train_ops as T
+    g = _gen(43)
+    N = 20011                               # the losses' total in parts
+    h = torch.randn(N, 64, generator=g, device='cuda').to(BF).requires_grad_()
+    w = torch.randn(V, 64, generator=g, device='cuda').to(BF).requires_grad_()
+    t = torch.randint(0, V, (N,), generator=g, device='cuda')
+    u = torch.randn(shape, generator=g, device='cuda')
+
+    def step():
+        loss = T.linear_cross_entropy(h, w, t)
+        return [loss.detach(), *torch.autograd.grad(loss, (h, w)), T.newton_schulz(u)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        with torch.no_grad():
+            h.normal_(generator=g)
+            u.normal_(generator=g)
+            t.random_(0, V, generator=g)
+            t[::5] = -100
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+def test_calls_of_two_threads_at_once():
+    import threading
+    from sgpo_amd import train_ops as T
+    g = _gen(44)
+    h, w = torch.randn(500, 96, generator=g, device='cuda'), torch.randn(700, 96, generator=g, device='cuda')
+    t = torch.randint(0, 700, (500,), generator=g, device='cuda')
+    freq, _ = T.rotary_frequencies(32)
+    q = torch.randn(2, 30, 4, 32, generator=g, device='cuda')
+
+    def calls():
+        hl = h.detach().requires_grad_()
+        loss = T.linear_cross_entropy(hl, w, t)
+        return [loss.detach(), torch.autograd.grad(loss, hl)[0], T.newton_schulz(w), T.newton_schulz(w[:64]), T.newton_schulz(w[:50, :60]), T.rotary_positions(q, None, freq)[0]]
+
+    want = calls()
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i].append(calls())
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    for out in got[0] + got[1]:
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+    assert len(got[0]) == len(got[1]) == 10
+
+
 def test_a_training_step_of_a_small_denoiser():
     """The operators together, as one training step uses them: rotated heads, attention, the head's loss with the mask class closed, gradients
     through all of it, orthogonalised updates of the matrices; against the same step in 64 bits."""
