@@ -12,6 +12,7 @@
 // the result 2e-2 on Gaussian updates, against 3e-5 with two planes; the result is rounded to bf16, 2e-3).
 // The squared norm is summed in 64 bits: it neither overflows nor depends on how the update is cut.  An infinity or NaN in an update
 // makes its whole result NaN.
+// Three ways: both sides small, one workgroup and launch per matrix; one side small, iteration on d x d matrices; tiles over the device.
 #include "../../include/sgpo_hip.h"
 #include "tile_gemm.h"
 
@@ -499,8 +500,9 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void apply_kernel(Mats q, int tm,
 //   P = a I + b G + c G G,   Q <- P Q,   G <- P G P
 // needs nothing of length n: X_0 is read for G_0 and again for the result Q X_0.  G's rounding grows by a^2 per triple in the directions of small
 // singular values (where P's is read off it), so G is formed afresh from Q X_0 before that reaches GROWTH; five triples of the default: after three.
-// Everything in fp32 on the fp32 matrix instructions, whose rate does not count at this size (relative error of the result 1e-6 on Gaussian updates, 1e-4
-// on nearly rank-one ones; formed afresh at every triple the same, never 1e-6 and 1e-3).  Six launches instead of 17 to 22.
+// Everything in fp32 on the fp32 matrix instructions (before the last rounding the result's relative error is 1e-6 on Gaussian updates and 1e-4 on nearly
+// rank-one ones, the same with G formed afresh at every triple; formed once, 1e-6 and 1e-3).  Six launches instead of 17 to 22.  Bound by the chain of
+// products in one workgroup, 0.9 us each at 64 x 64 and half of it the matrix instructions, and by the launches (64 x 4096: two times 11 us of 51).
 constexpr int NARROW = 64, NARROW_CHUNK = 64, NARROW_PITCH = NARROW_CHUNK + 4;
 constexpr double GROWTH = 200.;
 struct NarrowArgs {
@@ -604,20 +606,23 @@ __device__ __forceinline__ void narrow_fetch(const float* from, float* Q) {
     *reinterpret_cast<f32x4*>(Q + e / (D / 4) * (D + 4) + e % (D / 4) * 4) = *reinterpret_cast<const f32x4*>(from + e * 4);
 }
 
-// sums[b][cut] = X X^T over the cut's chunks, X = X_0 or Q X_0
+// sums[b][cut] = X X^T over the cut's chunks, X = X_0 or Q X_0: the tiles on and over the diagonal
 template <typename T, int D, bool TURN>
 __global__ __launch_bounds__(256) void narrow_gram_kernel(NarrowArgs p) {
   __shared__ __attribute__((aligned(16))) float tile[D * NARROW_PITCH];
   __shared__ __attribute__((aligned(16))) float Q[TURN ? D * (D + 4) : 4];
-  constexpr int SIDE = D / 16, MINE = SIDE * SIDE / 4;   // 16 x 16 tiles of the result, and of a wave
-  const int b = blockIdx.y, lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4, wave = (int)threadIdx.x >> 6;
+  constexpr int TILES = D / 16 * (D / 16 + 1) / 2, MINE = (TILES + 3) / 4;   // 16 x 16 tiles of the triangle, and of a wave
+  const int b = blockIdx.y, lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const float inv = inverse_norm(p.part + b * PARTS, p.parts, p.eps);
   if constexpr (TURN) narrow_fetch<D>(p.Q + (int64_t)b * D * D, Q);
   f32x4 acc[MINE];
 #pragma unroll
   for (int t = 0; t < MINE; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int first = blockIdx.x * p.per, last = min(first + p.per, p.chunks);
-  const int x = wave * MINE / SIDE, y0 = wave * MINE % SIDE;
+  int x[MINE], y[MINE];
+#pragma unroll
+  for (int t = 0; t < MINE; ++t) triangle(min(wave + 4 * t, TILES - 1), D / 16, x[t], y[t]);
   Chunk<D> next;
   narrow_load<T, D>(p, b, first, next);
   for (int c = first; c < last; ++c) {
@@ -626,30 +631,37 @@ __global__ __launch_bounds__(256) void narrow_gram_kernel(NarrowArgs p) {
     __syncthreads();
     if (c + 1 < last) narrow_load<T, D>(p, b, c + 1, next);   // on its way while this one is multiplied
     if constexpr (TURN) narrow_turn<D>(Q, tile);
-    float a[NARROW_CHUNK / 4], f[MINE][NARROW_CHUNK / 4];
-    narrow_row<NARROW_CHUNK>(tile + (x * 16 + l16) * NARROW_PITCH, l4, a);
 #pragma unroll
-    for (int t = 0; t < MINE; ++t) narrow_row<NARROW_CHUNK>(tile + ((y0 + t) * 16 + l16) * NARROW_PITCH, l4, f[t]);
+    for (int t = 0; t < MINE; ++t) {
+      if (wave + 4 * t >= TILES) break;
+      float a[NARROW_CHUNK / 4], f[NARROW_CHUNK / 4];
+      narrow_row<NARROW_CHUNK>(tile + (x[t] * 16 + l16) * NARROW_PITCH, l4, a);
+      narrow_row<NARROW_CHUNK>(tile + (y[t] * 16 + l16) * NARROW_PITCH, l4, f);
 #pragma unroll
-    for (int k = 0; k < NARROW_CHUNK / 4; ++k)
-#pragma unroll
-      for (int t = 0; t < MINE; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], f[t][k], acc[t], 0, 0, 0);
+      for (int k = 0; k < NARROW_CHUNK / 4; ++k) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], f[k], acc[t], 0, 0, 0);
+    }
   }
   float* out = p.sums + ((int64_t)b * p.cuts + blockIdx.x) * D * D;
 #pragma unroll
-  for (int t = 0; t < MINE; ++t)
+  for (int t = 0; t < MINE; ++t) {
+    if (wave + 4 * t >= TILES) break;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) out[(x * 16 + 4 * l4 + q) * D + (y0 + t) * 16 + l16] = acc[t][q];
+    for (int q = 0; q < 4; ++q) out[(x[t] * 16 + 4 * l4 + q) * D + y[t] * 16 + l16] = acc[t][q];
+  }
 }
 
-// the triples [k0, k1): Q <- P Q, G <- P G P; one workgroup per matrix, one wave per 16 x 16 tile.  Images hold symmetric matrices: a lane's four rows go out as
-// four columns, and columns are read as rows.
+// the triples [k0, k1): Q <- P Q, G <- P G P; one workgroup per matrix, one wave per 16 x 16 tile of the triangle (64 x 64: the ten of them take the matrix
+// instructions of three on a SIMD, all sixteen those of four).  The images hold whole symmetric matrices, whose columns are read as rows.
+template <int D> constexpr int POLY_THREADS = D / 16 * (D / 16 + 1) / 2 * 64;
 template <int D>
-__global__ __launch_bounds__(4 * D / 16 * D) void narrow_poly_kernel(NarrowArgs p, Table coef, int k0, int k1) {
-  constexpr int PITCH = D + 4, SIDE = D / 16;
+__global__ __launch_bounds__(POLY_THREADS<D>) void narrow_poly_kernel(NarrowArgs p, Table coef, int k0, int k1) {
+  constexpr int PITCH = D + 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float *G = reinterpret_cast<float*>(smem), *P = G + D * PITCH, *M = P + D * PITCH, *Q = M + D * PITCH;
-  const int b = blockIdx.x, lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4, wave = (int)threadIdx.x >> 6, x = wave / SIDE, y = wave % SIDE;
+  const int b = blockIdx.x, lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
+  int x, y;
+  triangle(__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), D / 16, x, y);
+  const int row = x * 16 + 4 * l4, col = y * 16 + l16;
   auto product = [&](const float* A, const float* B) {
     float a[D / 4], f[D / 4];
     narrow_row<D>(A + (x * 16 + l16) * PITCH, l4, a);
@@ -662,8 +674,12 @@ __global__ __launch_bounds__(4 * D / 16 * D) void narrow_poly_kernel(NarrowArgs 
     }
     return even + odd;
   };
-  auto put = [&](float* img, const f32x4& v) { *reinterpret_cast<f32x4*>(img + (y * 16 + l16) * PITCH + x * 16 + 4 * l4) = v; };
-  const int row = x * 16 + 4 * l4, col = y * 16 + l16;
+  auto put = [&](float* img, const f32x4& v) {
+    *reinterpret_cast<f32x4*>(img + col * PITCH + row) = v;
+    if (x == y) return;   // the tile itself is its mirror image
+#pragma unroll
+    for (int e = 0; e < 4; ++e) img[(row + e) * PITCH + col] = v[e];
+  };
   f32x4 g = {0.f, 0.f, 0.f, 0.f}, q = g;
   const float* from = p.sums + (int64_t)b * p.cuts * D * D + row * D + col;
 #pragma unroll 4
@@ -693,8 +709,11 @@ __global__ __launch_bounds__(4 * D / 16 * D) void narrow_poly_kernel(NarrowArgs 
     put(G, g);
     __syncthreads();
   }
+  float* out = p.Q + (int64_t)b * D * D;
+  *reinterpret_cast<f32x4*>(out + col * D + row) = q;
+  if (x == y) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) p.Q[(int64_t)b * D * D + (row + e) * D + col] = q[e];
+  for (int e = 0; e < 4; ++e) out[(row + e) * D + col] = q[e];
 }
 
 // the result: Q X_0
@@ -804,8 +823,8 @@ int apply_any(int kind, const Mats& q, int batch, const Result& r, hipStream_t s
 }
 
 constexpr int CUTS = 32;
-// Where the matrices of at most 64 x 64 take over (us, before and with): d <= 32 from 65 on (31 x 128: 31.6, 22.2), d <= 64 from 129 on (64 x 128 in
-// one launch 38.9, 42.3 this way) up to 32768 (64 x 32768: 124, 105; the one workgroup that adds up the cuts grows with the length's root).
+// Where this takes over from the one launch and from the tiles (us, theirs and this): d <= 32 from 65 on (31 x 128: 31.6, 21.4), d <= 64 from 129 on
+// (64 x 128: 39.2, and 64 x 129 39.3 this way), up to 32768 (64 x 32768: 124, 88; the workgroup that adds up the cuts grows with the length's root).
 constexpr int NARROW_MOST = 1 << 15;
 struct Sizes { int d, longer, narrow, chunks, per, cuts; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, off_s, bytes; Pick gram, poly, full; };
 Sizes sizes(int batch, int rows, int cols) {
@@ -815,7 +834,7 @@ Sizes sizes(int batch, int rows, int cols) {
   const bool narrow = s.d <= NARROW && s.longer > (s.d <= 32 ? 64 : 128) && s.longer <= NARROW_MOST;
   if (s.longer <= 128 && !narrow) return s;   // one launch, no scratch
   if (narrow) {
-    // a cut costs its workgroup a chunk after the other, and the one that adds the cuts up 16 KB of each (64 x 4096: 20 cuts 58.6 us, 32 58.7)
+    // a cut costs its workgroup a chunk after the other, and the one that adds the cuts up 16 KB of each (64 x 4096: 20 and 32 cuts take the same time)
     s.narrow = s.d <= 32 ? 32 : 64;
     s.chunks = (s.longer + NARROW_CHUNK - 1) / NARROW_CHUNK;
     int64_t cuts = (int64_t)(sqrt(10. * s.chunks) + 1.);
@@ -875,7 +894,7 @@ int orthogonalise_narrow(const NarrowArgs& p, int batch, const float* coef, int 
     }
     if (k0 == 0) hipLaunchKernelGGL((narrow_gram_kernel<T, D, false>), dim3(p.cuts, batch), dim3(256), 0, st, p);
     else hipLaunchKernelGGL((narrow_gram_kernel<T, D, true>), dim3(p.cuts, batch), dim3(256), 0, st, p);
-    hipLaunchKernelGGL((narrow_poly_kernel<D>), dim3(batch), dim3(D / 16 * D * 4), LDS, st, p, t, k0, k1);
+    hipLaunchKernelGGL((narrow_poly_kernel<D>), dim3(batch), dim3(POLY_THREADS<D>), LDS, st, p, t, k0, k1);
   }
   hipLaunchKernelGGL((narrow_apply_kernel<T, D>), dim3(p.chunks, batch), dim3(256), 0, st, p, res);
   SGPO_CHECK_HIP(hipGetLastError());
