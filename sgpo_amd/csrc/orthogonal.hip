@@ -772,17 +772,21 @@ int apply(const Mats& q, int batch, const Result& r, hipStream_t st) {
   return SGPO_OK;
 }
 
-// Tile shapes, and what one tile costs (us): `symmetric` and `apply` + `step` per 32 k, one workgroup on a CU, measured at 1 x 1536 x 512 and
-// 8 x 512 x 2048.  Small tiles spread a small product over the CUs and read more bytes for it; large ones the other way round.
-struct Kind { int side, per_cu; double symmetric, apply, step; };
-constexpr Kind KINDS[] = {{256, 1, 30., 11., 1.40}, {192, 1, 17., 9.7, 0.90}, {129, 1, 11., 6.4, 0.46}, {128, 2, 11., 3.5, 0.575},
-                          {96, 1, 8.5, 6.8, 0.276}, {64, 2, 4.5, 3.6, 0.21}, {32, 2, 3.6, 3.3, 0.08}};
+// Tile shapes, and what one tile costs (us): `symmetric` and `apply` + `step` per 32 k, `alone` where the tiles are no more than the CUs (of two workgroups
+// on a CU one multiplies while the other waits for memory).  Measured at 1 x 1536 x 512, 8 x 512 x 2048, 1024 x 1024, 3 x 400 x 1000 and 16 x 200 x 200.  Small
+// tiles spread a small product over the CUs and read more bytes for it; large ones the other way round.  side: odd for the second shape of a side.
+struct Kind { int side, per_cu; double symmetric, apply, step, alone; };
+constexpr Kind KINDS[] = {{256, 1, 30., 11., 1.40, 1.40}, {192, 1, 17., 9.7, 0.90, 0.90}, {129, 1, 11., 6.4, 0.46, 0.46}, {128, 2, 11., 3.5, 0.575, 0.575},
+                          {96, 1, 8.5, 6.8, 0.276, 0.276}, {65, 1, 5.3, 4.2, 0.25, 0.25}, {64, 2, 4.5, 3.6, 0.21, 0.33}, {33, 1, 4.0, 3.7, 0.106, 0.106},
+                          {32, 2, 3.6, 3.3, 0.08, 0.147}};
 typedef tg::Shape<256, 256, 2, 4, 2, 2> Shape256;
 typedef tg::Shape<192, 192, 2, 4, 2, 2> Shape192;
 typedef tg::Shape<128, 128, 2, 2, 2, 2, 2> Shape129;   // 128 x 128 with two groups over K: one workgroup fills a CU
 typedef tg::Shape<128, 128, 2, 2, 2, 2> Shape128;
 typedef tg::Shape<96, 96, 2, 2, 2, 2, 3> Shape96;
-typedef tg::Shape<64, 64, 2, 2, 2, 2, 2> Shape64;
+typedef tg::Shape<64, 64, 2, 2, 2, 4, 2> Shape65;      // four slots, of which a CU holds one workgroup's: three steps on their way instead of one
+typedef tg::Shape<64, 64, 2, 2, 2, 2, 2> Shape64;      // (1024 x 1024: 229 us without, 198 with; four of 768 x 768, more tiles than CUs: 250 without, 296 with)
+typedef tg::Shape<32, 32, 1, 1, 2, 4, 4> Shape33;
 typedef tg::Shape<32, 32, 1, 1, 2, 2, 4> Shape32;
 
 // The kind with the least rounds of the 256 CUs x cost of a tile; count(side) tiles of `steps` K steps.  A symmetric product with few tiles and a
@@ -795,9 +799,9 @@ Pick pick(F count, int64_t steps, bool sym, int most_cuts = 1, double joined_byt
   for (int s = 1; s <= most_cuts; s *= 2) {
     if (s > 1 && steps / s < 8) break;
     for (const Kind& k : KINDS) {
-      const int64_t n = count(k.side == 129 ? 128 : k.side) * s;
+      const int64_t n = count(k.side & ~1) * s;
       const double rounds = k.per_cu == 1 ? (double)((n + 255) / 256) : n <= 256 ? 1. : (n + 127) / 128 * 0.5;
-      const double t = rounds * ((sym ? k.symmetric : k.apply) + (double)((steps + s - 1) / s) * k.step) + (s > 1 ? 5. + s * joined_bytes * 2. / 4e6 : 0.);
+      const double t = rounds * ((sym ? k.symmetric : k.apply) + (double)((steps + s - 1) / s) * (n <= 256 ? k.alone : k.step)) + (s > 1 ? 5. + s * joined_bytes * 2. / 4e6 : 0.);
       if (t < least) { least = t; best = {k.side, s}; }
     }
   }
@@ -810,7 +814,9 @@ Pick pick(F count, int64_t steps, bool sym, int most_cuts = 1, double joined_byt
     case 129: { typedef Shape129 S; return CALL; }                     \
     case 128: { typedef Shape128 S; return CALL; }                     \
     case 96: { typedef Shape96 S; return CALL; }                       \
+    case 65: { typedef Shape65 S; return CALL; }                       \
     case 64: { typedef Shape64 S; return CALL; }                       \
+    case 33: { typedef Shape33 S; return CALL; }                       \
     default: { typedef Shape32 S; return CALL; }                       \
   }
 template <int MODE>
