@@ -108,6 +108,8 @@ _tables = {}     # coefficients -> one flat list
 
 
 def _coefficients(coefficients, steps):
+    if len(coefficients) == 0:
+        _refuse(f'{steps} steps need {steps} coefficient triples')
     key = (tuple(map(tuple, coefficients)) if isinstance(coefficients[0], (tuple, list)) else tuple(coefficients), steps)
     table = _tables.get(key)
     if table is None:

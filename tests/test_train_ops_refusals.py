@@ -26,7 +26,8 @@ def test_what_has_no_gradient_is_refused():
     q, b = torch.zeros(1, 2, 2, 8), torch.zeros(5, 8)
     for call, text in ((lambda: T.rotary_positions(q, q, f), 'frequencies'), (lambda: T.rotary_positions_(q, None, f), 'frequencies'),
                        (lambda: T.newton_schulz(w), 'no gradient'), (lambda: T.muon_step(w * 2, b, b, 0.1), 'graph'),
-                       (lambda: T.muon_step(b, b, w * 2, 0.1), 'graph')):
+                       (lambda: T.muon_step(b, b, w * 2, 0.1), 'graph'), (lambda: T.newton_schulz(b, coefficients=()), 'triples'),
+                       (lambda: T.newton_schulz(b, steps=0), 'triples'), (lambda: T.muon_step(b, b, b, 0.1, coefficients=[(1.0, 2.0)] * 5), 'triples')):
         with pytest.raises(L.SgpoError, match=text):
             call()
 
