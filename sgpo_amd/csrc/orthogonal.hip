@@ -495,8 +495,7 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void apply_kernel(Mats q, int tm,
 }
 
 // ------------------------------------------------------------------------------------------------ long and narrow updates
-// At most 64 rows (or columns) and more of the other: the iteration runs on d x d matrices.  X_k = Q_k X_0 with Q a polynomial in G_0 = X_0 X_0^T, all
-// of them symmetric and commuting, so that
+// At most 64 rows (or columns) and more of the other: the iteration runs on d x d matrices.  X_k = Q_k X_0 with Q a polynomial in G_0 = X_0 X_0^T, so that
 //   P = a I + b G + c G G,   Q <- P Q,   G <- P G P
 // needs nothing of length n: X_0 is read for G_0 and again for the result Q X_0.  G's rounding grows by a^2 per triple in the directions of small
 // singular values (where P's is read off it), so G is formed afresh from Q X_0 before that reaches GROWTH; five triples of the default: after three.
@@ -511,7 +510,7 @@ struct NarrowArgs {
   int parts;
   double eps;
   int d, n, tall;        // shorter and longer side
-  float* Q;              // [batch][D][D], symmetric
+  float* Q;              // [batch][D][D]
   float* sums;           // [batch][cuts][D][D]
   int chunks, per, cuts;
 };
@@ -651,7 +650,9 @@ __global__ __launch_bounds__(256) void narrow_gram_kernel(NarrowArgs p) {
 }
 
 // the triples [k0, k1): Q <- P Q, G <- P G P; one workgroup per matrix, one wave per 16 x 16 tile of the triangle (64 x 64: the ten of them take the matrix
-// instructions of three on a SIMD, all sixteen those of four).  The images hold whole symmetric matrices, whose columns are read as rows.
+// instructions of three on a SIMD, all sixteen those of four).  The images hold whole matrices.  G, P and P G are symmetric but for rounding, which the mirrored
+// triangle may decide; Q is not: P and Q of separate phases do not commute within what Q's large entries make of their rounding (on updates of low rank a
+// mirrored Q was off by 7e-4 to 2e-2, against 3e-5), so Q is multiplied whole, in order, and kept transposed for its columns to be read as rows.
 template <int D> constexpr int POLY_THREADS = D / 16 * (D / 16 + 1) / 2 * 64;
 template <int D>
 __global__ __launch_bounds__(POLY_THREADS<D>) void narrow_poly_kernel(NarrowArgs p, Table coef, int k0, int k1) {
@@ -662,10 +663,11 @@ __global__ __launch_bounds__(POLY_THREADS<D>) void narrow_poly_kernel(NarrowArgs
   int x, y;
   triangle(__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), D / 16, x, y);
   const int row = x * 16 + 4 * l4, col = y * 16 + l16;
-  auto product = [&](const float* A, const float* B) {
+  const int row2 = y * 16 + 4 * l4, col2 = x * 16 + l16;   // the same lane's four elements of the tile's mirror image
+  auto product = [&](const float* A, int i, const float* B, int j) {   // tile (i, j) of A B^T
     float a[D / 4], f[D / 4];
-    narrow_row<D>(A + (x * 16 + l16) * PITCH, l4, a);
-    narrow_row<D>(B + (y * 16 + l16) * PITCH, l4, f);
+    narrow_row<D>(A + (i * 16 + l16) * PITCH, l4, a);
+    narrow_row<D>(B + (j * 16 + l16) * PITCH, l4, f);
     f32x4 even = {0.f, 0.f, 0.f, 0.f}, odd = even;   // two chains
 #pragma unroll
     for (int k = 0; k < D / 4; k += 2) {
@@ -674,46 +676,57 @@ __global__ __launch_bounds__(POLY_THREADS<D>) void narrow_poly_kernel(NarrowArgs
     }
     return even + odd;
   };
-  auto put = [&](float* img, const f32x4& v) {
+  auto put = [&](float* img, const f32x4& v) {   // a symmetric matrix, both triangles
     *reinterpret_cast<f32x4*>(img + col * PITCH + row) = v;
     if (x == y) return;   // the tile itself is its mirror image
 #pragma unroll
     for (int e = 0; e < 4; ++e) img[(row + e) * PITCH + col] = v[e];
   };
-  f32x4 g = {0.f, 0.f, 0.f, 0.f}, q = g;
+  f32x4 g = {0.f, 0.f, 0.f, 0.f}, q = g, q2 = g;   // q2: Q's tile (y, x)
   const float* from = p.sums + (int64_t)b * p.cuts * D * D + row * D + col;
 #pragma unroll 4
   for (int c = 0; c < p.cuts; ++c)
 #pragma unroll
     for (int e = 0; e < 4; ++e) g[e] += from[(int64_t)c * D * D + e * D];
   put(G, g);
+  auto put_q = [&]() {   // transposed
+    *reinterpret_cast<f32x4*>(Q + col * PITCH + row) = q;
+    if (x != y) *reinterpret_cast<f32x4*>(Q + col2 * PITCH + row2) = q2;
+  };
+  float* out = p.Q + (int64_t)b * D * D;
   if (k0 > 0) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = p.Q[(int64_t)b * D * D + (row + e) * D + col];
-    put(Q, q);
+    for (int e = 0; e < 4; ++e) { q[e] = out[(row + e) * D + col]; q2[e] = out[(row2 + e) * D + col2]; }
+    put_q();
   }
   __syncthreads();
   for (int k = k0; k < k1; ++k) {
     const float ca = coef.v[3 * k], cb = coef.v[3 * k + 1], cc = coef.v[3 * k + 2];
-    f32x4 h = product(G, G);
+    f32x4 h = product(G, x, G, y);
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = fmaf(cb, g[e], cc * h[e]) + (row + e == col ? ca : 0.f);
     put(P, h);
     __syncthreads();
-    q = k > 0 ? product(P, Q) : h;
+    if (k > 0) {
+      q = product(P, x, Q, y);
+      if (x != y) q2 = product(P, y, Q, x);
+    } else {
+      q = h;
+      q2 = *reinterpret_cast<const f32x4*>(P + col2 * PITCH + row2);
+    }
     if (k + 1 == k1) break;
-    put(M, product(P, G));
+    put(M, product(P, x, G, y));
     __syncthreads();
-    g = product(P, M);
-    put(Q, q);
+    g = product(P, x, M, y);
+    put_q();
     put(G, g);
     __syncthreads();
   }
-  float* out = p.Q + (int64_t)b * D * D;
-  *reinterpret_cast<f32x4*>(out + col * D + row) = q;
-  if (x == y) return;
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[(row + e) * D + col] = q[e];
+  if (x == y) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[(row2 + e) * D + col2] = q2[e];
 }
 
 // the result: Q X_0

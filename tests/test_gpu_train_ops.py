@@ -434,6 +434,21 @@ def test_newton_schulz_of_uneven_spectra_and_other_tables(shape):
             assert off <= err + UBF * float(want.norm()), (off, err, float(want.norm()))
 
 
+@pytest.mark.parametrize('shape', [(31, 128), (64, 300), (20, 90), (500, 48), (150, 400), (60, 60)])
+def test_newton_schulz_of_low_rank_updates(shape):
+    # five directions, and rows of zeros: what rounding leaves in the other directions is multiplied by a^5 = 485.  X_0 of norm 1 is rounded by 2^-17, and
+    # X_k, whose norm is at most a^k, again before the remaining factors a^(5 - k): 5 x 485 x 2^-17 at most, and the output's own rounding
+    from sgpo_amd import train_ops as T
+    g = _gen(24)
+    m, n = shape
+    u = torch.randn(m, 5, generator=g, device='cuda') @ torch.randn(5, n, generator=g, device='cuda')
+    u[::7] = 0
+    for x in (u, u * torch.logspace(0, -3, m, device='cuda')[:, None], u.to(BF)):
+        want, _ = _schulz64(x, [T.NS_COEFFICIENTS] * 5, 1e-7)
+        off = float((T.newton_schulz(x).double() - want).norm())
+        assert off <= 5 * 485 * 2.0 ** -17 + UBF * float(want.norm()), (off, float(want.norm()))
+
+
 @pytest.mark.parametrize('tall', [False, True])
 def test_newton_schulz_of_the_longest_updates(tall):
     # 200 x 2^22, zero but for some columns everywhere: the others' updates are those of the small matrix that is left
