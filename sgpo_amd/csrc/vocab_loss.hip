@@ -358,7 +358,7 @@ struct HeadArgs {
   const float* bias;
   const int64_t* targets;
   int64_t ignore;
-  int N, H, V, vec;          // vec: rows may be read 16 bytes at a time
+  int N, H, V;
   float *nll, *lse;          // forward's outputs; GRAD reads lse
   const float* g;            // [N], or not read (g_rows 0)
   int g_rows, rows_pad, h_pad;
@@ -369,34 +369,25 @@ struct HeadArgs {
 template <typename T> struct PlanesOf { static constexpr int value = 1; };
 template <> struct PlanesOf<float> { static constexpr int value = 3; };
 
-// eight consecutive features of a row as fragments of each plane
+// eight consecutive features of a row as fragments of each plane, zero from `limit` on; rows need no more than their elements' alignment
 template <typename T, int PL>
-__device__ __forceinline__ void load8(const T* row, int e, int H, bool vec, bool live, bf16x8 (&f)[PL]) {
-  if constexpr (PL == 1) {
-    if (vec) {
-      f[0] = live ? *reinterpret_cast<const bf16x8*>(row + e) : bf16x8{};
-    } else {
-      tg::s16x8 v = {};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) if (live && e + i < H) v[i] = (short)row[e + i];
-      f[0] = *reinterpret_cast<const bf16x8*>(&v);
-    }
+__device__ __forceinline__ void load8(const T* row, int e, int limit, bool live, bf16x8 (&f)[PL]) {
+  alignas(16) T x[8];
+  if (e + 8 <= limit) {
+    __builtin_memcpy(x, row + e, sizeof(x));   // 16-byte loads, also of odd rows (56377 x 1143 bf16, 31 classes: 338 us element by element, 109 so)
   } else {
-    float x[8];
-    if (vec) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(row + e), b = *reinterpret_cast<const f32x4*>(row + e + 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { x[i] = live ? a[i] : 0.f; x[4 + i] = live ? b[i] : 0.f; }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = live && e + i < H ? row[e + i] : 0.f;
-    }
+    for (int i = 0; i < 8; ++i) x[i] = e + i < limit ? row[e + i] : T(0);
+  }
+  if constexpr (PL == 1) {
+    f[0] = live ? *reinterpret_cast<const bf16x8*>(x) : bf16x8{};
+  } else {
     uint32_t w[PL][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float p0[PL], p1[PL];
-      tg::split<PL>(x[2 * i], p0);
-      tg::split<PL>(x[2 * i + 1], p1);
+      tg::split<PL>(live ? x[2 * i] : 0.f, p0);
+      tg::split<PL>(live ? x[2 * i + 1] : 0.f, p1);
 #pragma unroll
       for (int p = 0; p < PL; ++p) w[p][i] = pack_bf16x2(p0[p], p1[p]);
     }
@@ -423,14 +414,12 @@ __global__ __launch_bounds__(256) void head_kernel(HeadArgs p) {
 #pragma unroll
   for (int y = 0; y < NB; ++y) acc[y] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int H = p.H, slices = (H + 31) >> 5;
-  const bool vec = p.vec;
-  auto slice = [&](int s, bool whole) {
+  auto slice = [&](int s, int limit) {   // limit: H, or no limit for whole slices
     const int e = s * 32 + l4 * 8;
     bf16x8 a[PL], b[NB][PL];
-    const bool in = whole || (vec ? e < H : true);   // with 16-byte rows H is a multiple of 8
-    load8<T, PL>(hr, in ? e : 0, H, vec, in && (GRAD ? keep : true), a);
+    load8<T, PL>(hr, e, limit, GRAD ? keep : true, a);
 #pragma unroll
-    for (int y = 0; y < NB; ++y) load8<T, PL>(wr[y], in ? e : 0, H, vec, in, b[y]);
+    for (int y = 0; y < NB; ++y) load8<T, PL>(wr[y], e, limit, true, b[y]);
     if constexpr (GRAD) {
       if (p.hp && m < p.rows_pad) {
 #pragma unroll
@@ -445,9 +434,8 @@ __global__ __launch_bounds__(256) void head_kernel(HeadArgs p) {
         for (int y = 0; y < NB; ++y) acc[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[y][j], a[i], acc[y], 0, 0, 0);
   };
   int s = ks;
-  if (vec)
-    for (; (s + 1) * 32 <= H; s += KS) slice(s, true);
-  for (; s < slices; s += KS) slice(s, false);
+  for (; (s + 1) * 32 <= H; s += KS) slice(s, INT_MAX);
+  for (; s < slices; s += KS) slice(s, H);
   if constexpr (GRAD) {   // the packed features' last padding
     const int ps = p.h_pad >> 5;
     for (; s < ps; s += KS)
@@ -533,7 +521,7 @@ struct MmArgs {
   void* out;
   int64_t ldo, slab;
   Factor factor;            // on the sums
-  int out_bf16, add, vec;   // vec: rows start 16-B (fp32) / 8-B (bf16) aligned
+  int out_bf16, add;
 };
 
 template <class S, int KA, int KB>
@@ -558,17 +546,23 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void mm_kernel(MmArgs p, int tm, 
       if (!S::owns(x, y)) continue;
       const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4;
       f32x4 v = acc[x][y] * factor;
+      // four at a time, whatever the row's alignment (dhidden of 56377 x 1143 bf16, 31 classes: 109 us element by element, 49 so)
       if (p.out_bf16) {
         bf16_t* o = reinterpret_cast<bf16_t*>(p.out) + m * p.ldo + n;
-        if (p.vec && n + 4 <= p.N) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        const uint32_t w[2] = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        if (n + 4 <= p.N) __builtin_memcpy(o, w, 8);
         else
 #pragma unroll
           for (int q = 0; q < 4; ++q) if (n + q < p.N) o[q] = f2bf(v[q]);
       } else {
         float* o = reinterpret_cast<float*>(p.out) + blockIdx.y * p.slab + m * p.ldo + n;
-        if (p.vec && n + 4 <= p.N) {
-          if (p.add) v += *reinterpret_cast<const f32x4*>(o);
-          *reinterpret_cast<f32x4*>(o) = v;
+        if (n + 4 <= p.N) {
+          if (p.add) {
+            f32x4 was;
+            __builtin_memcpy(&was, o, 16);
+            v += was;
+          }
+          __builtin_memcpy(o, &v, 16);
         } else
 #pragma unroll
           for (int q = 0; q < 4; ++q) if (n + q < p.N) o[q] = p.add ? o[q] + v[q] : v[q];
@@ -808,12 +802,10 @@ int head(const HeadArgs& p, hipStream_t st) {
   SGPO_CHECK_HIP(hipGetLastError());
   return SGPO_OK;
 }
-HeadArgs head_args(const sgpo_linear_ce_args* a, const Plan& q) {
+HeadArgs head_args(const sgpo_linear_ce_args* a) {
   HeadArgs p = {};
-  const int n = 16 / (q.PL == 1 ? 2 : 4);
   p.h = a->hidden; p.w = a->weight; p.ldh = a->ld_hidden; p.ldw = a->ld_weight; p.bias = a->bias; p.targets = a->targets; p.ignore = a->ignore_index;
   p.N = a->N; p.H = a->H; p.V = a->V;
-  p.vec = a->H % 8 == 0 && a->ld_hidden % n == 0 && a->ld_weight % n == 0 && aligned16(a->hidden) && aligned16(a->weight);
   return p;
 }
 
@@ -832,7 +824,7 @@ void total(const sgpo_linear_ce_args* a, const float* nll, float* loss, float* i
 template <int PL>
 int forward(const sgpo_linear_ce_args* a, const Plan& q, float* nll, float* lse, float* loss, float* inv, char* ws, hipStream_t st) {
   if (q.head) {
-    HeadArgs p = head_args(a, q);
+    HeadArgs p = head_args(a);
     p.nll = nll; p.lse = lse;
     const int rc = PL == 1 ? head<bf16_t, false>(p, st) : head<float, false>(p, st);
     if (rc) return rc;
@@ -937,7 +929,7 @@ int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, cons
     const int nc_pad = (int)round_up(nc, 64);
     int parts = 0;
     if (q.head) {
-      HeadArgs p = head_args(a, q);
+      HeadArgs p = head_args(a);
       p.lse = const_cast<float*>(lse); p.g = g; p.g_rows = a->reduction == SGPO_REDUCE_NONE;
       p.rows_pad = (int)q.rows_pad; p.h_pad = q.h_pad; p.d = d; p.hp = dw ? hp : nullptr; p.col_sums = db ? cs : nullptr;
       if ((rc = PL == 1 ? head<bf16_t, true>(p, st) : head<float, true>(p, st))) return rc;
@@ -956,8 +948,7 @@ int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, cons
     if (dh) {
       // the first piece decides how many slabs there are; later ones add to them
       MmArgs m{{d, (int64_t)nc_pad * PL, a->N, 0}, {w.p + v0 * w.ld, w.ld, nc, q.h_pad * PL}, a->N, a->H, nc_pad / kstep, 0,
-               via ? (void*)acc : dh, via ? ldf : a->H, via ? (int64_t)a->N * ldf : 0, factor, !via && bf, v0 > 0,
-               via || (a->H % 4 == 0 && aligned16(dh))};
+               via ? (void*)acc : dh, via ? ldf : a->H, via ? (int64_t)a->N * ldf : 0, factor, !via && bf, v0 > 0};
       const int used = product<PL, tg::KC, tg::KM>(m, q.h_cut.shape, v0 == 0 ? q.h_cut.splits : h_used, st);
       if (used < 0) return used;
       if (v0 == 0) h_used = used;
@@ -967,8 +958,7 @@ int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, cons
       const bool slabs = q.w_cut.splits > 1;
       void* out = (char*)dw + v0 * a->H * esz;
       MmArgs m{{d, (int64_t)nc_pad * PL, (int)q.rows_pad, nc_pad * PL}, {hp, (int64_t)q.h_pad * PL, (int)q.rows_pad, q.h_pad * PL}, nc, a->H, (int)(q.rows_pad / kstep), 0,
-               slabs ? (void*)wacc : out, slabs ? ldf : a->H, slabs ? (int64_t)nc * ldf : 0, factor, !slabs && bf, 0,
-               slabs || (a->H % 4 == 0 && aligned16(out))};
+               slabs ? (void*)wacc : out, slabs ? ldf : a->H, slabs ? (int64_t)nc * ldf : 0, factor, !slabs && bf, 0};
       if (q.turned) m.b = tg::Operand{ht, q.rows_pad, q.h_pad, 0};
       const int used = q.turned ? product<PL, tg::KM, tg::KC>(m, q.w_cut.shape, q.w_cut.splits, st) : product<PL, tg::KM, tg::KM>(m, q.w_cut.shape, q.w_cut.splits, st);
       if (used < 0) return used;

@@ -246,6 +246,9 @@ LOSS = [
     (1000, 128, 5000, True, False, 0.15, 'mean'),
     (3, 2048, 20011, False, False, 0.0, 'mean'),
     (2100, 33, 70, True, True, 0.5, 'sum'),
+    (300, 517, 31, True, True, 0.2, 'none'),
+    (9001, 75, 31, True, False, 0.3, 'mean'),
+    (70, 7, 64, False, False, 0.0, 'sum'),
 ]
 
 
