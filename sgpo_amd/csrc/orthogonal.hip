@@ -32,7 +32,7 @@ struct Source {
   float momentum;
   int nesterov;
   int64_t stride_b, ld;    // of grad; buf is contiguous
-  int rows, cols, vec;     // vec: grad contiguous and, like buf, readable four elements at a time
+  int rows, cols, flat;    // flat: a matrix of grad is contiguous
 };
 
 template <typename T>
@@ -43,18 +43,31 @@ __device__ __forceinline__ float update_at(const Source& s, int b, int r, int c)
   return s.nesterov ? fmaf(s.momentum, m, g) : m;
 }
 
-// four consecutive elements of a contiguous gradient
-template <typename T> __device__ __forceinline__ void grad4(const T* p, float (&g)[4]);
-template <> __device__ __forceinline__ void grad4<float>(const float* p, float (&g)[4]) {
-  const f32x4 v = *reinterpret_cast<const f32x4*>(p);
-  g[0] = v[0]; g[1] = v[1]; g[2] = v[2]; g[3] = v[3];
+// four consecutive elements of a gradient's row, of any alignment
+__device__ __forceinline__ void grad4(const float* p, float (&g)[4]) { __builtin_memcpy(g, p, 16); }
+__device__ __forceinline__ void grad4(const bf16_t* p, float (&g)[4]) {
+  uint32_t v[2];
+  __builtin_memcpy(v, p, 8);
+  g[0] = bf2f(v[0] & 0xffff); g[1] = bf2f(v[0] >> 16); g[2] = bf2f(v[1] & 0xffff); g[3] = bf2f(v[1] >> 16);
 }
-template <> __device__ __forceinline__ void grad4<bf16_t>(const bf16_t* p, float (&g)[4]) {
-  const uint2 v = *reinterpret_cast<const uint2*>(p);
-  g[0] = bf2f(v.x & 0xffff); g[1] = bf2f(v.x >> 16); g[2] = bf2f(v.y & 0xffff); g[3] = bf2f(v.y >> 16);
+// elements (r, c .. c + 3) of the update, those that exist; after the buffer's own update
+template <typename T>
+__device__ __forceinline__ void update4(const Source& s, int b, int r, int c, float (&v)[4]) {
+  if (c + 4 <= s.cols) {
+    grad4(reinterpret_cast<const T*>(s.grad) + b * s.stride_b + r * s.ld + c, v);
+    if (s.buf) {
+      f32x4 m;
+      __builtin_memcpy(&m, s.buf + ((int64_t)b * s.rows + r) * s.cols + c, 16);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = s.nesterov ? fmaf(s.momentum, m[q], v[q]) : m[q];
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = c + q < s.cols ? update_at<T>(s, b, r, c + q) : 0.f;
+  }
 }
 
-// momentum buffer, and partial sums of the update's squares; s.vec: four elements at a time
+// momentum buffer, and partial sums of the update's squares; four elements at a time where a matrix is contiguous
 template <typename T>
 __global__ __launch_bounds__(256) void square_kernel(Source s, double* part) {
   const int b = blockIdx.y;
@@ -62,29 +75,31 @@ __global__ __launch_bounds__(256) void square_kernel(Source s, double* part) {
   const T* grad = reinterpret_cast<const T*>(s.grad) + b * s.stride_b;
   float* buf = s.buf ? s.buf + (int64_t)b * total : nullptr;
   double sum = 0.0;
-  if (s.vec) {
+  uint32_t done = 0;
+  if (s.flat) {
+    done = total / 4 * 4;
     for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total / 4; i += gridDim.x * 256) {
       float g[4];
-      grad4<T>(grad + (size_t)i * 4, g);
+      grad4(grad + (size_t)i * 4, g);
       if (buf) {
-        f32x4 m = *reinterpret_cast<const f32x4*>(buf + (size_t)i * 4);
+        f32x4 m;
+        __builtin_memcpy(&m, buf + (size_t)i * 4, 16);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           m[q] = fmaf(s.momentum, m[q], g[q]);
           g[q] = s.nesterov ? fmaf(s.momentum, m[q], g[q]) : m[q];
         }
-        *reinterpret_cast<f32x4*>(buf + (size_t)i * 4) = m;
+        __builtin_memcpy(buf + (size_t)i * 4, &m, 16);
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) sum += (double)g[q] * g[q];
     }
-  } else {
-    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
-      const uint32_t r = i / (uint32_t)s.cols, c = i - r * (uint32_t)s.cols;
-      if (buf) buf[i] = fmaf(s.momentum, buf[i], up<T>(grad[r * s.ld + c]));
-      const double u = (double)update_at<T>(s, b, r, c);
-      sum += u * u;
-    }
+  }
+  for (uint32_t i = done + blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
+    const uint32_t r = i / (uint32_t)s.cols, c = i - r * (uint32_t)s.cols;
+    if (buf) buf[i] = fmaf(s.momentum, buf[i], up<T>(grad[r * s.ld + c]));
+    const double u = (double)update_at<T>(s, b, r, c);
+    sum += u * u;
   }
   __shared__ double share[4];
 #pragma unroll
@@ -111,20 +126,7 @@ __global__ __launch_bounds__(256) void load_kernel(Source s, const double* part,
   for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
     const int r = (int)(i / quads), c = (int)(i - (uint32_t)r * quads) * 4;
     float v[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = 0.f;
-    if (s.vec && c < s.cols) {
-      const int64_t at = (int64_t)r * s.cols + c;
-      grad4<T>(reinterpret_cast<const T*>(s.grad) + b * s.stride_b + at, v);
-      if (s.buf) {
-        const f32x4 m = *reinterpret_cast<const f32x4*>(s.buf + (int64_t)b * s.rows * s.cols + at);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = s.nesterov ? fmaf(s.momentum, m[q], v[q]) : m[q];
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) if (c + q < s.cols) v[q] = update_at<T>(s, b, r, c + q);
-    }
+    update4<T>(s, b, r, c, v);
 #pragma unroll
     for (int q = 0; q < 4; ++q) v[q] *= inv;
     tg::store4<2, true>(X + b * bstride + r * ldx, c, v);
@@ -258,7 +260,6 @@ struct Result {
   int out_bf16;
   int rows, cols;
   int step;                // 0: out = X;  1: out = keep * out - rate * X
-  int vec;                 // rows start aligned to four elements
   float keep, rate;
 };
 
@@ -268,20 +269,24 @@ __device__ __forceinline__ void store_result(const Result& r, int b, int m, int 
   const int64_t at = ((int64_t)b * r.rows + m) * r.cols + n;
   if (r.out_bf16) {
     bf16_t* o = reinterpret_cast<bf16_t*>(r.out) + at;
-    if (r.vec && n + 4 <= r.cols) {
-      uint2 w = make_uint2(0, 0);
-      if (r.step) w = *reinterpret_cast<const uint2*>(o);
-      *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(result(r, bf2f(w.x & 0xffff), v[0]), result(r, bf2f(w.x >> 16), v[1])),
-                                                pack_bf16x2(result(r, bf2f(w.y & 0xffff), v[2]), result(r, bf2f(w.y >> 16), v[3])));
+    if (n + 4 <= r.cols) {
+      uint32_t w[2] = {0, 0};
+      if (r.step) __builtin_memcpy(w, o, 8);
+      w[0] = pack_bf16x2(result(r, bf2f(w[0] & 0xffff), v[0]), result(r, bf2f(w[0] >> 16), v[1]));
+      w[1] = pack_bf16x2(result(r, bf2f(w[1] & 0xffff), v[2]), result(r, bf2f(w[1] >> 16), v[3]));
+      __builtin_memcpy(o, w, 8);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) if (n + e < r.cols) o[e] = f2bf(result(r, r.step ? bf2f(o[e]) : 0.f, v[e]));
     }
   } else {   // only a step writes fp32
     float* o = reinterpret_cast<float*>(r.out) + at;
-    if (r.vec && n + 4 <= r.cols) {
-      const f32x4 w = *reinterpret_cast<const f32x4*>(o);
-      *reinterpret_cast<f32x4*>(o) = f32x4{result(r, w[0], v[0]), result(r, w[1], v[1]), result(r, w[2], v[2]), result(r, w[3], v[3])};
+    if (n + 4 <= r.cols) {
+      f32x4 w;
+      __builtin_memcpy(&w, o, 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = result(r, w[e], v[e]);
+      __builtin_memcpy(o, &w, 16);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) if (n + e < r.cols) o[e] = result(r, o[e], v[e]);
@@ -501,7 +506,7 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void apply_kernel(Mats q, int tm,
 // singular values (where P's is read off it), so G is formed afresh from Q X_0 before that reaches GROWTH; five triples of the default: after three.
 // Everything in fp32 on the fp32 matrix instructions (before the last rounding the result's relative error is 1e-6 on Gaussian updates and 1e-4 on nearly
 // rank-one ones, the same with G formed afresh at every triple; formed once, 1e-6 and 1e-3).  Six launches instead of 17 to 22.  Bound by the chain of
-// products in one workgroup, 0.9 us each at 64 x 64 and half of it the matrix instructions, and by the launches (64 x 4096: two times 11 us of 51).
+// products in one workgroup, 0.9 us each at 64 x 64 and half of it the matrix instructions, and by the launches (64 x 4096: two times 11 us of 52).
 constexpr int NARROW = 64, NARROW_CHUNK = 64, NARROW_PITCH = NARROW_CHUNK + 4;
 constexpr double GROWTH = 200.;
 struct NarrowArgs {
@@ -535,20 +540,7 @@ __device__ __forceinline__ void narrow_load(const NarrowArgs& p, int b, int chun
     float (&v)[4] = to.v[k];
 #pragma unroll
     for (int q = 0; q < 4; ++q) v[q] = 0.f;
-    if (r < s.rows && c < s.cols) {
-      if (s.vec) {
-        const int64_t at = (int64_t)r * s.cols + c;
-        grad4<T>(reinterpret_cast<const T*>(s.grad) + b * s.stride_b + at, v);
-        if (s.buf) {
-          const f32x4 m = *reinterpret_cast<const f32x4*>(s.buf + (int64_t)b * s.rows * s.cols + at);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] = s.nesterov ? fmaf(s.momentum, m[q], v[q]) : m[q];
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) if (c + q < s.cols) v[q] = update_at<T>(s, b, r, c + q);
-      }
-    }
+    if (r < s.rows) update4<T>(s, b, r, c, v);
   }
 }
 // into tile [D][NARROW_PITCH]: short index, long index
@@ -842,8 +834,8 @@ int apply_any(int kind, const Mats& q, int batch, const Result& r, hipStream_t s
 }
 
 constexpr int CUTS = 32;
-// Where this takes over from the one launch and from the tiles (us, theirs and this): d <= 32 from 65 on (31 x 128: 31.6, 21.4), d <= 64 from 129 on
-// (64 x 128: 39.2, and 64 x 129 39.3 this way), up to 32768 (64 x 32768: 124, 88; the workgroup that adds up the cuts grows with the length's root).
+// Where this takes over from the one launch and from the tiles (us, theirs and this): d <= 32 from 65 on (31 x 128: 31.6, 22.6), d <= 64 from 129 on
+// (64 x 128: 39.1, and 64 x 129 41.1 this way), up to 32768 (64 x 32768: 124, 88; the workgroup that adds up the cuts grows with the length's root).
 constexpr int NARROW_MOST = 1 << 15;
 struct Sizes { int d, longer, narrow, chunks, per, cuts; int64_t ldx, ldg; size_t x, g, off_x, off_y, off_g, off_p, off_s, bytes; Pick gram, poly, full; };
 Sizes sizes(int batch, int rows, int cols) {
@@ -924,13 +916,12 @@ template <typename T>
 int orthogonalise(Source src, int batch, const float* coef, int steps, double eps, Result res, char* ws, hipStream_t st) {
   const Sizes z = sizes(batch, src.rows, src.cols);
   res.rows = src.rows; res.cols = src.cols;
-  res.vec = src.cols % 4 == 0 && (uintptr_t)res.out % (res.out_bf16 ? 8 : 16) == 0;
   if (z.longer <= 64) return orthogonalise_small<T, 64>(src, batch, coef, steps, eps, res, st);
   if (z.longer <= 128 && !z.narrow) return orthogonalise_small<T, 128>(src, batch, coef, steps, eps, res, st);
   double* part = reinterpret_cast<double*>(ws);
   Mats q{(bf16_t*)(ws + z.off_x), (bf16_t*)(ws + z.off_y), (bf16_t*)(ws + z.off_g), (bf16_t*)(ws + z.off_p), z.ldx, z.ldg, (int64_t)z.x, (int64_t)z.g, src.rows, src.cols, z.d};
   const bool tall = src.rows > src.cols;
-  src.vec = src.cols % 4 == 0 && src.ld == src.cols && src.stride_b % 4 == 0 && (uintptr_t)src.grad % (4 * sizeof(T)) == 0 && (uintptr_t)src.buf % 16 == 0;
+  src.flat = src.ld == src.cols;
   // about four elements a thread
   const int64_t want = ((int64_t)src.rows * src.cols + 1023) / 1024;
   const int parts = want < PARTS ? (int)want : PARTS;
@@ -999,7 +990,7 @@ extern "C" int sgpo_newton_schulz(const void* update, int dtype, int batch, int 
   const int esz = dtype == SGPO_DTYPE_BF16 ? 2 : 4;
   SGPO_REQUIRE(stride_b >= 0 && !overlap(update, ((batch - 1) * stride_b + (rows - 1) * ld + cols) * esz, out, (int64_t)batch * rows * cols * 2), "newton_schulz: out overlaps update");
   const Source s{update, nullptr, 0.f, 0, stride_b, ld, rows, cols, 0};
-  const Result r{out, 1, 0, 0, 0, 0, 0.f, 0.f};
+  const Result r{out, 1, 0, 0, 0, 0.f, 0.f};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return dtype == SGPO_DTYPE_BF16 ? orthogonalise<bf16_t>(s, batch, coefficients, steps, eps, r, (char*)workspace, st)
                                   : orthogonalise<float>(s, batch, coefficients, steps, eps, r, (char*)workspace, st);
@@ -1022,7 +1013,7 @@ extern "C" int sgpo_muon_step(void* weight, int weight_dtype, const void* grad, 
                "muon_step: weight, grad and momentum_buffer overlap");
   const Source s{grad, momentum_buffer, momentum, nesterov != 0, (int64_t)rows * cols, cols, rows, cols, 0};
   const double ratio = rows > cols ? (double)rows / cols : 1.0;
-  const Result r{weight, weight_dtype == SGPO_DTYPE_BF16, 0, 0, 1, 0, (float)(1.0 - (double)lr * weight_decay), (float)(lr * sqrt(ratio))};
+  const Result r{weight, weight_dtype == SGPO_DTYPE_BF16, 0, 0, 1, (float)(1.0 - (double)lr * weight_decay), (float)(lr * sqrt(ratio))};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return grad_dtype == SGPO_DTYPE_BF16 ? orthogonalise<bf16_t>(s, batch, coefficients, steps, eps, r, (char*)workspace, st)
                                        : orthogonalise<float>(s, batch, coefficients, steps, eps, r, (char*)workspace, st);
