@@ -66,6 +66,12 @@ ROTARY = [
     (5, 2000, 2, 2, 256, 256, F32, False, 'plain', 'huge'),
     (2, 9, 2, 2, 64, 0, BF, False, 'plain', None),
     (2, 9, 5, 0, 64, 16, BF, False, 'plain', None),
+    # the last run of a part shorter than the others: 31 pairs and 2 copied, 3 and 60, 13 and 7, odd heads
+    (2, 37, 3, 1, 64, 62, BF, False, 'plain', 'ragged'),
+    (2, 37, 3, 1, 66, 6, F32, False, 'heads_first', None),
+    (3, 50, 2, 2, 33, 26, BF, True, 'plain', 'ragged'),
+    (3, 50, 2, 2, 33, 26, F32, False, 'plain', 'row'),
+    (2, 119, 8, 8, 64, 62, BF, False, 'packed', None),
 ]
 
 
