@@ -365,6 +365,7 @@ struct HeadArgs {
   bf16_t *d, *hp;            // [rows_pad][64], [rows_pad][h_pad] planes
   float* col_sums;           // [workgroup][V], or null
 };
+inline int head_rows(int64_t N) { return N <= 8192 ? 16 : 64; }   // tokens of a workgroup; few tokens: four waves to 16 of them
 
 template <typename T> struct PlanesOf { static constexpr int value = 1; };
 template <> struct PlanesOf<float> { static constexpr int value = 3; };
@@ -738,8 +739,8 @@ Plan make_plan(const sgpo_linear_ce_args* a, bool backward) {
     q.off_wacc = take(q.w_cut.splits > 1 ? (size_t)q.w_cut.splits * piece * round_up(a->H, 4) * 4 : 0);
     int bm = config_bm(q.PL, pick(q.PL, a->N, piece));
     if (a->V % piece) { const int b2 = config_bm(q.PL, pick(q.PL, a->N, a->V % piece)); if (b2 < bm) bm = b2; }
-    if (q.head) bm = 16;
-    q.off_cs = take((size_t)((a->N + bm - 1) / bm) * piece * 4);
+    // a row for every workgroup of the launch: a head's runs over the padded tokens
+    q.off_cs = take((size_t)(q.head ? q.rows_pad / head_rows(a->N) : (a->N + bm - 1) / bm) * piece * 4);
   }
   q.bytes = at;
   return q;
@@ -788,9 +789,8 @@ int pack(const void* src, int64_t ld, int rows, int cols, bf16_t* dst, int64_t r
 
 template <typename T, bool GRAD>
 int head(const HeadArgs& p, hipStream_t st) {
-  // few tokens: four waves to 16 of them
-  const bool share = p.N <= 8192;
-  const int rows = share ? 16 : 64;
+  const int rows = head_rows(p.N);
+  const bool share = rows == 16;
   const dim3 grid((unsigned)(((GRAD ? (int64_t)p.rows_pad : (int64_t)p.N) + rows - 1) / rows));
 #define HEAD(NB)                                                                                                       \
   case NB:                                                                                                             \
@@ -933,7 +933,7 @@ int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, cons
       p.lse = const_cast<float*>(lse); p.g = g; p.g_rows = a->reduction == SGPO_REDUCE_NONE;
       p.rows_pad = (int)q.rows_pad; p.h_pad = q.h_pad; p.d = d; p.hp = dw ? hp : nullptr; p.col_sums = db ? cs : nullptr;
       if ((rc = PL == 1 ? head<bf16_t, true>(p, st) : head<float, true>(p, st))) return rc;
-      parts = (int)(a->N <= 8192 ? (a->N + 15) / 16 : (a->N + 63) / 64);
+      parts = (a->N + head_rows(a->N) - 1) / head_rows(a->N);   // further rows, of padding, hold zeros
     } else {
       LossArgs p{h, {w.p + v0 * w.ld, w.ld, (int)(a->V - v0), 0}, a->bias, a->targets, a->ignore_index, 0, a->N, (int)v0, nc, q.n_kstep};
       FOR_SHAPE(PL, pick(PL, a->N, nc), {

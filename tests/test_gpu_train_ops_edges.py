@@ -1,0 +1,90 @@
+"""GPU: the training operators at the edges of their arguments: workspaces of exactly the size asked for, tensors that are more than plain memory."""
+import ctypes as C
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+GUARD = 1 << 16
+
+
+def _gen(seed):
+    return torch.Generator(device='cuda').manual_seed(seed)
+
+
+def _lib():
+    from sgpo_amd import _lib as L
+    from sgpo_amd import train_ops as T
+    T.newton_schulz(torch.zeros(1, 1, device='cuda'))         # the first call binds the process to its GPU
+    return L, L.load()
+
+
+class Guarded:
+    """`need` bytes, 256-byte aligned, with a filled region behind them."""
+    def __init__(self, need):
+        self.need = need
+        self.buf = torch.full((need + GUARD + 256,), 0xA5, dtype=torch.uint8, device='cuda')
+        self.skip = -self.buf.data_ptr() % 256
+        self.ptr = C.c_void_p(self.buf.data_ptr() + self.skip)
+
+    def whole(self):
+        return bool((self.buf[:self.skip] == 0xA5).all()) and bool((self.buf[self.skip + self.need:] == 0xA5).all())
+
+
+def _stream():
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+# heads of every number of padded workgroups, the largest that share tokens among waves; then the tiles, cut and not, in one piece and in several
+SIZES = [(N, 64, V) for N in (1, 16, 17, 33, 48, 49, 64, 513, 1537, 8145, 8192, 8193) for V in (1, 31, 64)] + [
+    (1, 512, 31), (17, 512, 64), (300, 517, 31), (257, 517, 1003), (130, 72, 257), (3, 2048, 20011), (2100, 33, 70), (40000, 64, 8000)]
+
+
+@pytest.mark.parametrize('dtype', [F32, BF])
+def test_loss_leaves_what_lies_behind_its_workspace(dtype):
+    L, lib = _lib()
+    g = _gen(1)
+    for N, H, V in SIZES:
+        h, w = torch.randn(N, H, generator=g, device='cuda').to(dtype), torch.randn(V, H, generator=g, device='cuda').to(dtype)
+        b, t = torch.randn(V, generator=g, device='cuda'), torch.randint(0, V, (N,), generator=g, device='cuda')
+        a = L.LinearCeArgs(hidden=h.data_ptr(), weight=w.data_ptr(), bias=b.data_ptr(), targets=t.data_ptr(), ld_hidden=H, ld_weight=H, ignore_index=-100, N=N, H=H, V=V,
+                           dtype=int(dtype == BF), reduction=L.REDUCE_MEAN)
+        out = {k: Guarded(n * 4) for k, n in (('nll', N), ('lse', N), ('loss', 1), ('inv', 1), ('db', V))}
+        out.update(dh=Guarded(N * H * h.element_size()), dw=Guarded(V * H * h.element_size()))
+        up = torch.ones(1, device='cuda')
+        for backward in (0, 1):
+            need = lib.sgpo_linear_ce_workspace_bytes(C.byref(a), backward)
+            ws = Guarded(need)
+            if backward:
+                rc = lib.sgpo_linear_ce_backward(C.byref(a), out['lse'].ptr, C.c_void_p(up.data_ptr()), out['inv'].ptr, out['dh'].ptr, out['dw'].ptr, out['db'].ptr, ws.ptr, need, _stream())
+            else:
+                rc = lib.sgpo_linear_ce_forward(C.byref(a), out['nll'].ptr, out['lse'].ptr, out['loss'].ptr, out['inv'].ptr, ws.ptr, need, _stream())
+            assert rc == 0, lib.sgpo_last_error()
+            torch.cuda.synchronize()
+            assert ws.whole(), (N, H, V, backward)
+        assert all(o.whole() for o in out.values()), (N, H, V)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF])
+def test_updates_leave_what_lies_behind_their_workspace(dtype):
+    L, lib = _lib()
+    g = _gen(2)
+    coef = (C.c_float * 15)(*([3.4445, -4.7750, 2.0315] * 5))
+    for batch, m, n in [(1, 1, 1), (3, 64, 64), (2, 128, 100), (1, 31, 512), (3, 64, 4000), (2, 1003, 17), (1, 100, 900), (2, 150, 9000), (1, 513, 129), (3, 400, 1000),
+                        (1, 1000, 1001), (1, 40000, 3), (8, 70, 5000)]:
+        grad = torch.randn(batch, m, n, generator=g, device='cuda').to(dtype)
+        need = lib.sgpo_newton_schulz_workspace_bytes(batch, m, n)
+        x, weight, buf = Guarded(batch * m * n * 2), Guarded(batch * m * n * 4), Guarded(batch * m * n * 4)
+        for o in (weight, buf):
+            o.buf[o.skip:o.skip + o.need] = 0
+        for step in (0, 1):
+            ws = Guarded(need)
+            if step:
+                rc = lib.sgpo_muon_step(weight.ptr, 0, C.c_void_p(grad.data_ptr()), int(dtype == BF), buf.ptr, batch, m, n, 0.02, 0.9, 1, 0.0, coef, 5, 1e-7, ws.ptr, need, _stream())
+            else:
+                rc = lib.sgpo_newton_schulz(C.c_void_p(grad.data_ptr()), int(dtype == BF), batch, m, n, m * n, n, coef, 5, 1e-7, x.ptr, ws.ptr, need, _stream())
+            assert rc == 0, lib.sgpo_last_error()
+            torch.cuda.synchronize()
+            assert ws.whole() and x.whole() and weight.whole() and buf.whole(), (batch, m, n, step)
