@@ -105,6 +105,12 @@ bool records(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+void no_tangents(std::initializer_list<const Tensor*> ts, const char* what) {
+  for (const Tensor* t : ts)
+    if (t && t->defined()) REQUIRE(!has_tangent(*t), what, " has no forward-mode derivative: detach its inputs");
+}
+
 // ------------------------------------------------------------------------------------------------------------- rotation
 variable_list rotate(Tensor q, Tensor k, const Tensor& freq, const Tensor& pos, bool interleaved, double scale, bool inverse, bool in_place) {
   const Call call({&q, &k, &freq, &pos});
@@ -152,6 +158,9 @@ variable_list rotate(Tensor q, Tensor k, const Tensor& freq, const Tensor& pos, 
   return {out[0], out[1]};
 }
 
+// rotate, with the derivatives of both modes in q and k
+variable_list turn(const Tensor& q, const Tensor& k, const Tensor& freq, const Tensor& pos, bool interleaved, double scale, bool inverse);
+
 struct Rotary : torch::autograd::Function<Rotary> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const Tensor& freq, const OptTensor& pos, bool interleaved, double scale, bool inverse) {
     const Tensor none, kk = k.value_or(none), pp = pos.value_or(none);
@@ -166,28 +175,44 @@ struct Rotary : torch::autograd::Function<Rotary> {
     const auto saved = ctx->get_saved_variables();
     const int64_t how = ctx->saved_data["how"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
-    const OptTensor k = how & 4 ? OptTensor(g[1]) : std::nullopt, pos = saved[1].defined() ? OptTensor(saved[1]) : std::nullopt;
     // the transposed rotation, itself differentiable where a second derivative is asked for
-    variable_list d = records({&g[0], how & 4 ? &g[1] : nullptr}) ? Rotary::apply(g[0], k, saved[0], pos, (how & 1) != 0, scale, !(how & 2))
-                                                                 : rotate(g[0], k.value_or(Tensor()), saved[0], saved[1], how & 1, scale, !(how & 2), false);
-    return {d[0], how & 4 ? d[1] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const variable_list d = turn(g[0], how & 4 ? g[1] : Tensor(), saved[0], saved[1], how & 1, scale, !(how & 2));
+    return {d[0], d[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
+variable_list turn(const Tensor& q, const Tensor& k, const Tensor& freq, const Tensor& pos, bool interleaved, double scale, bool inverse) {
+  const bool dq = has_tangent(q), dk = k.defined() && has_tangent(k);
+  if (dq || dk) {   // linear: a tangent turns like its heads
+    Tensor value[2] = {q, k}, tangent[2];
+    for (int w = 0; w < 2; ++w) {
+      if (!(w ? dk : dq)) continue;
+      std::tie(value[w], tangent[w]) = at::_unpack_dual(value[w], 0);
+      if (tangent[w]._is_zerotensor()) tangent[w] = at::zeros(tangent[w].sizes(), value[w].options());   // a zero without memory
+    }
+    variable_list out = turn(value[0], value[1], freq, pos, interleaved, scale, inverse);
+    const variable_list t = turn(tangent[dq ? 0 : 1], dq ? tangent[1] : Tensor(), freq, pos, interleaved, scale, inverse);
+    if (dq) out[0] = at::_make_dual(out[0], t[0], 0);
+    if (dk) out[1] = at::_make_dual(out[1], t[dq ? 1 : 0], 0);
+    return out;
+  }
+  if (!records({&q, &k})) return rotate(q, k, freq, pos, interleaved, scale, inverse, false);
+  variable_list out = Rotary::apply(q, k.defined() ? OptTensor(k) : std::nullopt, freq, pos.defined() ? OptTensor(pos) : std::nullopt, interleaved, scale, inverse);
+  out.resize(2);
+  return out;
+}
+
 std::pair<Tensor, OptTensor> rotary_positions(const Tensor& q, const OptTensor& k, const Tensor& freq, const OptTensor& pos, bool interleaved, double scale) {
   REQUIRE(!records({&freq}), "rotary_positions has no gradient for the frequencies: detach them");
-  variable_list out;
-  if (records({&q, opt(k)})) {
-    out = Rotary::apply(q, k, freq, pos, interleaved, scale, false);
-  } else {
-    out = rotate(q, k.value_or(Tensor()), freq, pos.value_or(Tensor()), interleaved, scale, false, false);
-  }
+  REQUIRE(!has_tangent(freq), "rotary_positions has no derivative for the frequencies: detach them");
+  const variable_list out = turn(q, k.value_or(Tensor()), freq, pos.value_or(Tensor()), interleaved, scale, false);
   return {out[0], opt(k) ? OptTensor(out[1]) : std::nullopt};
 }
 
 void rotary_positions_(const Tensor& q, const OptTensor& k, const Tensor& freq, const OptTensor& pos, bool interleaved, double scale) {
   REQUIRE(!records({&freq}), "rotary_positions has no gradient for the frequencies: detach them");
   REQUIRE(!records({&q, opt(k)}), "rotary_positions_ has no gradient: use rotary_positions");
+  no_tangents({&q, opt(k), &freq}, "rotary_positions_");
   rotate(q, k.value_or(Tensor()), freq, pos.value_or(Tensor()), interleaved, scale, false, true);
   // what autograd saved of them is stale now
   if (!q.is_inference()) q.unsafeGetTensorImpl()->bump_version();
@@ -251,6 +276,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
       at::AutoGradMode off(false);
       const auto s = ctx->get_saved_variables();
       const int64_t how = ctx->saved_data["how"].toInt();
+      no_tangents({&grads[0]}, "the gradient of linear_cross_entropy");
       const Call call({&s[0]});
       const sgpo_linear_ce_args a = ce_args(s[0], s[1], s[2], s[3], ctx->saved_data["ignore"].toInt(), how & 3);
       const Tensor g = grads[0].contiguous();
@@ -279,6 +305,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
 };
 
 Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets, const OptTensor& bias, int64_t ignore, const std::string& reduction) {
+  no_tangents({&hidden, &weight, opt(bias)}, "linear_cross_entropy");
   Call::device_of({&hidden, &weight, &targets, opt(bias)});
   dtype_of(hidden, "hidden");
   REQUIRE(hidden.dim() >= 1 && weight.dim() == 2 && hidden.size(-1) == weight.size(1) && weight.numel() > 0, "hidden ", hidden.sizes(), " does not match weight ", weight.sizes());
@@ -302,6 +329,7 @@ void check_table(const std::vector<float>& c, int64_t steps) {
 
 Tensor newton_schulz(const Tensor& update, int64_t steps, const std::vector<float>& table, double eps) {
   REQUIRE(!records({&update}), "newton_schulz has no gradient: detach the update, or call it under torch.no_grad()");
+  no_tangents({&update}, "newton_schulz");
   const Call call({&update});
   const int dt = dtype_of(update, "update");
   REQUIRE(update.dim() >= 2, "an update is a matrix or a batch of them, got ", update.sizes());
@@ -325,6 +353,7 @@ void muon_step(const Tensor& weight, const Tensor& grad, const Tensor& buffer, d
                const std::vector<float>& table, double eps) {
   for (const Tensor* t : {&weight, &buffer})
     REQUIRE(!records({t}) || t->is_leaf(), "weight or momentum_buffer is part of a graph: a step updates leaves");
+  no_tangents({&weight, &grad, &buffer}, "muon_step");
   const Call call({&weight, &grad, &buffer});
   const int wd = dtype_of(weight, "weight"), gd = dtype_of(grad, "grad");
   REQUIRE(weight.dim() >= 2 && weight.sizes() == grad.sizes() && weight.sizes() == buffer.sizes(), "weight ", weight.sizes(), ", grad ", grad.sizes(), " and buffer ", buffer.sizes(),

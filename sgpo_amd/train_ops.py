@@ -5,7 +5,8 @@ The reference trains its denoisers through torch autograd (models/pretraining/tr
 torch kernels; here each is one call into libsgpo_hip.so.  PyTorch is plumbing (device memory, the current HIP stream, the autograd
 tape).  Every tensor is fp32 or bf16 device memory on the process's one GPU; a call runs on the stream that is current on that
 device, allocates its outputs and scratch from torch's allocator (so it can be captured into a graph and used on any stream), and
-does not synchronise.  There is no CPU fallback: bad arguments and host tensors raise SgpoError.
+does not synchronise.  There is no CPU fallback: bad arguments and host tensors raise SgpoError, and so do inputs with a forward-mode tangent
+everywhere but in rotary_positions.
 """
 import importlib
 import math
@@ -75,7 +76,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
 
 def rotary_positions(q, k, frequencies, positions=None, interleaved=False, scale=1.0):
     """q (B, L, Hq, D) and k (B, L, Hk, D) (or None) with the first 2 * len(frequencies) elements of every head turned by their
-    token's position; differentiable in q and k.  Returns new contiguous (q, k).
+    token's position; differentiable in q and k any number of times, in reverse and forward mode.  Returns new contiguous (q, k).
 
     frequencies and scale as rotary_frequencies gives them; positions int64 (L,), (B, L), (1, L) or None for 0 .. L - 1, of any size up to 2 ** 50; pairs are
     (j, j + rot / 2), or (2 j, 2 j + 1) if interleaved.  q and k may be views with any strides (of one packed projection, or of

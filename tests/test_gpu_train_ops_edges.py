@@ -3,6 +3,7 @@ import ctypes as C
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +89,52 @@ def test_updates_leave_what_lies_behind_their_workspace(dtype):
             assert rc == 0, lib.sgpo_last_error()
             torch.cuda.synchronize()
             assert ws.whole() and x.whole() and weight.whole() and buf.whole(), (batch, m, n, step)
+
+
+@pytest.mark.parametrize('dtype,interleaved', [(F32, False), (BF, True)])
+def test_rotation_in_forward_mode(dtype, interleaved):
+    """The rotation is linear: the tangent is the rotated tangent, alone, for q and k together, over a reverse pass and under one."""
+    from sgpo_amd import _lib as L
+    from sgpo_amd import train_ops as T
+    g = _gen(3)
+    q, dq, u = (torch.randn(2, 7, 3, 16, generator=g, device='cuda').to(dtype) for _ in range(3))
+    k, dk = (torch.randn(2, 7, 1, 16, generator=g, device='cuda').to(dtype) for _ in range(2))
+    freq, _ = T.rotary_frequencies(8)
+    pos = torch.randint(0, 100, (2, 7), generator=g, device='cuda')
+
+    def turn(a, b, **kw):
+        return T.rotary_positions(a, b, freq, pos, interleaved=interleaved, **kw)
+
+    want, dwant = turn(q, k), turn(dq, dk)
+    with fw.dual_level():
+        for a, b in ((1, 1), (1, 0), (0, 1)):
+            out = turn(fw.make_dual(q, dq) if a else q, fw.make_dual(k, dk) if b else k)
+            for x, y, dy, has in zip(out, want, dwant, (a, b)):
+                p, t = fw.unpack_dual(x)
+                assert torch.equal(p, y) and (torch.equal(t, dy) if has else t is None)
+        p, t = fw.unpack_dual(turn(fw.make_dual(q, dq), None)[0])
+        assert torch.equal(p, want[0]) and torch.equal(t, dwant[0])
+        # a tangent that is a lazy zero
+        p, t = fw.unpack_dual(turn(fw.make_dual(q, torch._efficientzerotensor(q.shape, dtype=dtype, device='cuda')), None)[0])
+        assert torch.equal(p, want[0]) and float(t.abs().max()) == 0.0
+        # the gradient's tangent: R^T of the upstream gradient's
+        leaf = q.clone().requires_grad_()
+        back, = torch.autograd.grad(turn(leaf, None)[0], leaf, fw.make_dual(u, dq))
+        p, t = fw.unpack_dual(back)
+        leaf2 = q.clone().requires_grad_()
+        y = turn(leaf2, None)[0]
+        assert torch.equal(p, torch.autograd.grad(y, leaf2, u, retain_graph=True)[0]) and torch.equal(t, torch.autograd.grad(y, leaf2, dq)[0])
+        # the tangent's gradient
+        leaf = dq.clone().requires_grad_()
+        t = fw.unpack_dual(turn(fw.make_dual(q, leaf), None)[0]).tangent
+        got, = torch.autograd.grad(t, leaf, u)
+        assert torch.equal(got, p)
+        # a leaf of both modes
+        leaf = q.clone().requires_grad_()
+        x, t = fw.unpack_dual(turn(fw.make_dual(leaf, dq), None)[0])
+        assert torch.equal(t, dwant[0]) and torch.equal(torch.autograd.grad(x, leaf, u)[0], p)
+        # the loss's gradient has none
+        h, w = torch.randn(4, 8, generator=g, device='cuda', requires_grad=True), torch.randn(9, 8, generator=g, device='cuda')
+        loss = T.linear_cross_entropy(h, w, torch.zeros(4, dtype=torch.int64, device='cuda'))
+        with pytest.raises((L.SgpoError, RuntimeError), match='forward-mode'):
+            torch.autograd.grad(loss, h, fw.make_dual(torch.ones((), device='cuda'), torch.ones((), device='cuda')))

@@ -1,6 +1,10 @@
 """CPU: the training operators at the edges of their arguments, without a device: room in workspaces, refusals."""
 import ctypes as C
 
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
 
 def test_head_workspace_has_a_row_of_column_sums_for_every_workgroup():
     """A head of at most 64 classes: the gradient runs over the tokens padded to 64, 16 of them a workgroup up to 8192 and 64 beyond, and each
@@ -25,3 +29,22 @@ def test_head_workspace_has_a_row_of_column_sums_for_every_workgroup():
                 assert got >= parts, (dtype, V, N)
                 a.N = rows
                 assert got >= need(ref, 1), (dtype, V, N)
+
+
+def test_tangents_are_refused_where_nothing_carries_them_on():
+    """Forward-mode inputs: without this, the result would have no tangent, i.e. a derivative of 0."""
+    from sgpo_amd import _lib as L
+    from sgpo_amd import train_ops as T
+    t = torch.zeros(3, dtype=torch.int64)
+    f = torch.zeros(4, dtype=torch.float64)
+    q = torch.zeros(1, 2, 2, 8)
+    with fw.dual_level():
+        def dual(x):
+            return fw.make_dual(x, torch.ones_like(x))
+
+        h, w, b = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(5)
+        for call in (lambda: T.rotary_positions(q, q, dual(f)), lambda: T.rotary_positions_(dual(q), None, f), lambda: T.rotary_positions_(q, dual(q), f),
+                     lambda: T.linear_cross_entropy(dual(h), w, t), lambda: T.linear_cross_entropy(h, dual(w), t), lambda: T.linear_cross_entropy(h, w, t, dual(b)),
+                     lambda: T.newton_schulz(dual(w)), lambda: T.muon_step(dual(w), w, w, 0.1), lambda: T.muon_step(w, dual(w), w, 0.1), lambda: T.muon_step(w, w, dual(w), 0.1)):
+            with pytest.raises(L.SgpoError, match='derivative'):
+                call()
