@@ -62,6 +62,8 @@ struct Call {
   c10::Device dev;
   c10::DeviceGuard guard;
   static c10::Device device_of(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+      if (t && t->defined()) REQUIRE(!t->is_neg(), "a lazily negated view ", t->sizes(), " ", t->dtype(), ": resolve_neg() it first");
     const Tensor* first = nullptr;
     for (const Tensor* t : ts) {
       if (!t || !t->defined()) continue;
@@ -83,7 +85,6 @@ struct Call {
 const Tensor* opt(const OptTensor& t) { return t && t->defined() ? &*t : nullptr; }
 
 int dtype_of(const Tensor& t, const char* what) {
-  REQUIRE(!t.is_neg(), what, " is a lazily negated view: resolve_neg() it first");
   if (t.scalar_type() == at::kFloat) return SGPO_DTYPE_F32;
   REQUIRE(t.scalar_type() == at::kBFloat16, what, " must be float32 or bfloat16, got ", t.dtype());
   return SGPO_DTYPE_BF16;
@@ -104,6 +105,9 @@ bool records(std::initializer_list<const Tensor*> ts) {
     if (t && t->defined() && t->requires_grad()) return true;
   return false;
 }
+
+// a gradient or tangent as memory that holds its values: autograd may hand over lazily negated views, and zeros that have none
+Tensor resolved(const Tensor& t) { return t._is_zerotensor() ? at::zeros(t.sizes(), at::TensorOptions().dtype(t.scalar_type()).device(t.device())) : t.resolve_neg(); }
 
 bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
 void no_tangents(std::initializer_list<const Tensor*> ts, const char* what) {
@@ -176,7 +180,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     const int64_t how = ctx->saved_data["how"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
     // the transposed rotation, itself differentiable where a second derivative is asked for
-    const variable_list d = turn(g[0], how & 4 ? g[1] : Tensor(), saved[0], saved[1], how & 1, scale, !(how & 2));
+    const variable_list d = turn(resolved(g[0]), how & 4 ? resolved(g[1]) : Tensor(), saved[0], saved[1], how & 1, scale, !(how & 2));
     return {d[0], d[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -188,7 +192,7 @@ variable_list turn(const Tensor& q, const Tensor& k, const Tensor& freq, const T
     for (int w = 0; w < 2; ++w) {
       if (!(w ? dk : dq)) continue;
       std::tie(value[w], tangent[w]) = at::_unpack_dual(value[w], 0);
-      if (tangent[w]._is_zerotensor()) tangent[w] = at::zeros(tangent[w].sizes(), value[w].options());   // a zero without memory
+      tangent[w] = resolved(tangent[w]);
     }
     variable_list out = turn(value[0], value[1], freq, pos, interleaved, scale, inverse);
     const variable_list t = turn(tangent[dq ? 0 : 1], dq ? tangent[1] : Tensor(), freq, pos, interleaved, scale, inverse);
@@ -279,7 +283,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
       no_tangents({&grads[0]}, "the gradient of linear_cross_entropy");
       const Call call({&s[0]});
       const sgpo_linear_ce_args a = ce_args(s[0], s[1], s[2], s[3], ctx->saved_data["ignore"].toInt(), how & 3);
-      const Tensor g = grads[0].contiguous();
+      const Tensor g = resolved(grads[0]).contiguous();
       void* out[3] = {nullptr, nullptr, nullptr};
       const Tensor* like[3] = {&s[0], &s[1], &s[3]};
       for (int i = 0; i < 3; ++i)

@@ -138,3 +138,29 @@ def test_rotation_in_forward_mode(dtype, interleaved):
         loss = T.linear_cross_entropy(h, w, torch.zeros(4, dtype=torch.int64, device='cuda'))
         with pytest.raises((L.SgpoError, RuntimeError), match='forward-mode'):
             torch.autograd.grad(loss, h, fw.make_dual(torch.ones((), device='cuda'), torch.ones((), device='cuda')))
+
+
+def test_lazily_negated_views():
+    """Refused as inputs; gradients that autograd hands over so are read with their sign."""
+    from sgpo_amd import _lib as L
+    from sgpo_amd import train_ops as T
+    g = _gen(4)
+    neg = torch._neg_view
+    q, u = (torch.randn(2, 5, 3, 16, generator=g, device='cuda') for _ in range(2))
+    freq, _ = T.rotary_frequencies(8)
+    h, w, b = (torch.randn(s, generator=g, device='cuda') for s in ((6, 16), (9, 16), (9,)))
+    t = torch.randint(0, 9, (6,), generator=g, device='cuda')
+    for call in (lambda: T.rotary_positions(q, neg(q), freq), lambda: T.rotary_positions(q, None, neg(freq)), lambda: T.rotary_positions_(q, neg(q), freq),
+                 lambda: T.linear_cross_entropy(neg(h), w, t), lambda: T.linear_cross_entropy(h, neg(w), t), lambda: T.linear_cross_entropy(h, w, t, neg(b)),
+                 lambda: T.newton_schulz(neg(w)), lambda: T.muon_step(neg(w), w, w.clone(), 0.1), lambda: T.muon_step(w, neg(h), w.clone(), 0.1),
+                 lambda: T.muon_step(w, h, neg(w), 0.1)):
+        with pytest.raises(L.SgpoError, match='negated'):
+            call()
+    leaf = q.clone().requires_grad_()
+    y, k = T.rotary_positions(leaf, leaf, freq)
+    assert torch.equal(torch.autograd.grad((y, k), leaf, (neg(u), u), retain_graph=True)[0], torch.autograd.grad((y, k), leaf, (-u, u))[0])
+    for red, up in (('none', torch.rand(6, generator=g, device='cuda')), ('mean', torch.rand((), generator=g, device='cuda'))):
+        leaves = [x.clone().requires_grad_() for x in (h, w, b)]
+        loss = T.linear_cross_entropy(*leaves[:2], t, leaves[2], reduction=red)
+        got, want = (torch.autograd.grad(loss, leaves, x, retain_graph=True) for x in (neg(up), -up))
+        assert all(torch.equal(x, y) for x, y in zip(got, want))

@@ -48,3 +48,19 @@ def test_tangents_are_refused_where_nothing_carries_them_on():
                      lambda: T.newton_schulz(dual(w)), lambda: T.muon_step(dual(w), w, w, 0.1), lambda: T.muon_step(w, dual(w), w, 0.1), lambda: T.muon_step(w, w, dual(w), 0.1)):
             with pytest.raises(L.SgpoError, match='derivative'):
                 call()
+
+
+def test_lazily_negated_views_are_refused():
+    """Their memory holds the values with the other sign."""
+    from sgpo_amd import _lib as L
+    from sgpo_amd import train_ops as T
+    neg = torch._neg_view
+    t = torch.zeros(3, dtype=torch.int64)
+    f = torch.zeros(4, dtype=torch.float64)
+    q, h, w, b = torch.zeros(1, 2, 2, 8), torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(5)
+    for call in (lambda: T.rotary_positions(neg(q), q, f), lambda: T.rotary_positions(q, neg(q), f), lambda: T.rotary_positions(q, None, neg(f)), lambda: T.rotary_positions_(neg(q), None, f),
+                 lambda: T.rotary_positions_(q, neg(q), f), lambda: T.linear_cross_entropy(neg(h), w, t), lambda: T.linear_cross_entropy(h, neg(w), t),
+                 lambda: T.linear_cross_entropy(h, w, t, neg(b)), lambda: T.newton_schulz(neg(w)), lambda: T.muon_step(neg(w), w, w, 0.1), lambda: T.muon_step(w, neg(w), w, 0.1),
+                 lambda: T.muon_step(w, w, neg(w), 0.1)):
+        with pytest.raises(L.SgpoError, match='negated'):
+            call()
