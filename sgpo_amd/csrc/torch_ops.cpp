@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <atomic>
@@ -62,6 +63,9 @@ struct Call {
   c10::Device dev;
   c10::DeviceGuard guard;
   static c10::Device device_of(std::initializer_list<const Tensor*> ts) {
+    REQUIRE(!torch::jit::tracer::isTracing(), "a trace would hold this call's result as a constant: trace around it");
+    for (const Tensor* t : ts)
+      if (t && t->defined()) REQUIRE(t->has_storage() && !t->_is_zerotensor(), "a tensor without memory of its own ", t->sizes(), " ", t->dtype(), " (of a torch.func transform, say, or sparse)");
     for (const Tensor* t : ts)
       if (t && t->defined()) REQUIRE(!t->is_neg(), "a lazily negated view ", t->sizes(), " ", t->dtype(), ": resolve_neg() it first");
     const Tensor* first = nullptr;
@@ -209,6 +213,7 @@ variable_list turn(const Tensor& q, const Tensor& k, const Tensor& freq, const T
 std::pair<Tensor, OptTensor> rotary_positions(const Tensor& q, const OptTensor& k, const Tensor& freq, const OptTensor& pos, bool interleaved, double scale) {
   REQUIRE(!records({&freq}), "rotary_positions has no gradient for the frequencies: detach them");
   REQUIRE(!has_tangent(freq), "rotary_positions has no derivative for the frequencies: detach them");
+  Call::device_of({&q, opt(k), &freq, opt(pos)});
   const variable_list out = turn(q, k.value_or(Tensor()), freq, pos.value_or(Tensor()), interleaved, scale, false);
   return {out[0], opt(k) ? OptTensor(out[1]) : std::nullopt};
 }

@@ -64,3 +64,21 @@ def test_lazily_negated_views_are_refused():
                  lambda: T.muon_step(w, w, neg(w), 0.1)):
         with pytest.raises(L.SgpoError, match='negated'):
             call()
+
+
+def test_transformed_and_traced_tensors_are_refused():
+    """A torch.func transform's tensor, a sparse one and a lazy zero have no memory to read; a trace would keep the call's result as a constant."""
+    from sgpo_amd import _lib as L
+    from sgpo_amd import train_ops as T
+    w, q, f = torch.ones(3, 5, 8), torch.ones(1, 2, 2, 8), torch.zeros(4, dtype=torch.float64)
+    t = torch.zeros(5, dtype=torch.int64)
+    one = torch.ones(5, 8)
+    for call in (lambda: torch.func.vmap(T.newton_schulz)(w), lambda: torch.func.vmap(lambda x: T.linear_cross_entropy(one, x, t))(w),
+                 lambda: torch.func.grad(lambda x: T.linear_cross_entropy(x, one, t))(one), lambda: torch.func.grad(lambda x: T.rotary_positions(x, None, f)[0].sum())(q),
+                 lambda: torch.func.vmap(lambda x: T.muon_step(x, one, one, 0.1))(w), lambda: T.newton_schulz(one.to_sparse()),
+                 lambda: T.rotary_positions(q, torch._efficientzerotensor(q.shape), f), lambda: T.newton_schulz(torch._efficientzerotensor((5, 8)))):
+        with pytest.raises(L.SgpoError, match='memory of its own'):
+            call()
+    for call, args in ((lambda x: T.newton_schulz(x), (one,)), (lambda x: T.rotary_positions(x, None, f)[0], (q,)), (lambda x: T.linear_cross_entropy(x, one, t), (one,))):
+        with pytest.raises(L.SgpoError, match='trace'):
+            torch.jit.trace(call, args)
