@@ -1013,12 +1013,17 @@ extern "C" int sgpo_linear_ce_backward(const sgpo_linear_ce_args* a, const float
   }
   SGPO_REQUIRE(a->hidden && a->weight && a->targets && lse && grad_out && workspace, "linear_ce_backward: null argument");
   SGPO_REQUIRE(a->reduction == SGPO_REDUCE_NONE || inv_count, "linear_ce_backward: null inv_count");
+  SGPO_REQUIRE((uintptr_t)workspace % 256 == 0, "linear_ce_backward: the workspace must be 256-byte aligned");
   const int64_t esz = a->dtype == SGPO_DTYPE_BF16 ? 2 : 4, hb = (int64_t)a->N * a->H * esz, wb = (int64_t)a->V * a->H * esz;
   const int64_t hin = ((a->N - 1) * a->ld_hidden + a->H) * esz, win = ((a->V - 1) * a->ld_weight + a->H) * esz;
-  SGPO_REQUIRE(!(overlap(dhidden, hb, a->hidden, hin) || overlap(dhidden, hb, a->weight, win) || overlap(dweight, wb, a->hidden, hin) || overlap(dweight, wb, a->weight, win) ||
-                 overlap(dhidden, hb, dweight, wb)), "linear_ce_backward: a gradient overlaps hidden, weight or the other gradient");
+  const struct { const void* p; int64_t n; } in[] = {{a->hidden, hin}, {a->weight, win}, {a->targets, (int64_t)a->N * 8}, {a->bias, (int64_t)a->V * 4}, {lse, (int64_t)a->N * 4},
+      {grad_out, a->reduction == SGPO_REDUCE_NONE ? (int64_t)a->N * 4 : 4}, {a->reduction == SGPO_REDUCE_NONE ? nullptr : inv_count, 4}},
+      out[] = {{dhidden, hb}, {dweight, wb}, {dbias, (int64_t)a->V * 4}};
+  for (int o = 0; o < 3; ++o) {
+    for (const auto& i : in) SGPO_REQUIRE(!overlap(out[o].p, out[o].n, i.p, i.n), "linear_ce_backward: a gradient overlaps an input");
+    SGPO_REQUIRE(!overlap(out[o].p, out[o].n, out[(o + 1) % 3].p, out[(o + 1) % 3].n), "linear_ce_backward: a gradient overlaps another one");
+  }
   const Plan q = make_plan(a, true);
-  SGPO_REQUIRE((uintptr_t)workspace % 256 == 0, "linear_ce_backward: the workspace must be 256-byte aligned");
   if (workspace_bytes < q.bytes) { sgpo_set_error("linear_ce_backward: workspace %zu < %zu", workspace_bytes, q.bytes); return SGPO_ERR_WORKSPACE; }
   const float* inv = a->reduction == SGPO_REDUCE_NONE ? nullptr : inv_count;
   return q.PL == 1 ? backward<1>(a, q, lse, grad_out, inv, dhidden, dweight, dbias, (char*)workspace, st)

@@ -82,3 +82,33 @@ def test_transformed_and_traced_tensors_are_refused():
     for call, args in ((lambda x: T.newton_schulz(x), (one,)), (lambda x: T.rotary_positions(x, None, f)[0], (q,)), (lambda x: T.linear_cross_entropy(x, one, t), (one,))):
         with pytest.raises(L.SgpoError, match='trace'):
             torch.jit.trace(call, args)
+
+
+def test_loss_gradients_that_overlap_are_refused():
+    """No output of the backward pass may lie over an input or another output; the places are numbers that no call gets to read."""
+    from sgpo_amd import _lib as L
+    lib = L.load()
+    N, H, V = 4, 8, 5
+    sizes = dict(hidden=N * H * 4, weight=V * H * 4, targets=N * 8, bias=V * 4, lse=N * 4, g=N * 4, inv=4, dh=N * H * 4, dw=V * H * 4, db=V * 4)
+    base = {k: (i + 1) << 20 for i, k in enumerate(sizes)}
+
+    def call(reduction, **moved):
+        p = dict(base, **moved)
+        a = L.LinearCeArgs(hidden=p['hidden'], weight=p['weight'], bias=p['bias'], targets=p['targets'], N=N, H=H, V=V, ld_hidden=H, ld_weight=H, reduction=reduction)
+        # the workspace is too small, which is found last
+        rc = lib.sgpo_linear_ce_backward(C.byref(a), p['lse'], p['g'], p['inv'], p['dh'], p['dw'], p['db'], 1 << 30, 16, None)
+        assert rc < 0
+        return lib.sgpo_last_error().decode()
+
+    for reduction in (L.REDUCE_NONE, L.REDUCE_SUM):
+        assert 'workspace' in call(reduction)
+        for out in ('dh', 'dw', 'db'):
+            assert 'workspace' in call(reduction, **{out: None})
+            for other in sizes:
+                if other == out or (reduction == L.REDUCE_NONE and other == 'inv'):
+                    continue
+                size = 4 if other == 'g' and reduction == L.REDUCE_SUM else sizes[other]
+                for at in (base[other], base[other] + size - 4, base[other] - sizes[out] + 4):
+                    assert 'overlaps' in call(reduction, **{out: at}), (reduction, out, other)
+                for at in (base[other] + size, base[other] - sizes[out]):
+                    assert 'workspace' in call(reduction, **{out: at}), (reduction, out, other)
