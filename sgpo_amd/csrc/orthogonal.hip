@@ -747,17 +747,6 @@ __global__ __launch_bounds__(256) void narrow_apply_kernel(NarrowArgs p, Result 
   }
 }
 
-template <typename K>
-int allow_lds(K kernel, int bytes) {
-  SGPO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  return SGPO_OK;
-}
-#define ALLOW(kernel, bytes)                                           \
-  do {                                                                 \
-    static bool done = false;                                          \
-    if (!done) { const int rc_ = allow_lds(kernel, bytes); if (rc_) return rc_; done = true; } \
-  } while (0)
-
 template <class S, int MODE>
 int symmetric(const Mats& q, int batch, const float* coef, const Slabs& slabs, int cuts, hipStream_t st) {
   const int t = (q.d + S::BM - 1) / S::BM;

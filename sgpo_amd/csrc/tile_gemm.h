@@ -17,6 +17,7 @@
 // row on the source address and again on the read.
 #pragma once
 #include "common.h"
+#include <atomic>
 #include <type_traits>
 
 namespace tg {
@@ -414,5 +415,20 @@ __device__ __forceinline__ void store_pair(bf16_t* row, int64_t e, const float (
     if (live) *reinterpret_cast<uint4*>(dst + p * 32) = make_uint4(a[0], b[0], a[1], b[1]);
   }
 }
+
+// A kernel may take more LDS than the default: asked for once per kernel, again if that failed.  Threads that come at the same time each ask, for the
+// same value.
+template <typename K>
+int allow_lds(K kernel, int bytes, std::atomic<bool>& done) {
+  if (done.load(std::memory_order_acquire)) return SGPO_OK;
+  SGPO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.store(true, std::memory_order_release);
+  return SGPO_OK;
+}
+#define ALLOW(kernel, bytes)                                           \
+  do {                                                                 \
+    static std::atomic<bool> done_{false};                             \
+    if (const int rc_ = tg::allow_lds(kernel, bytes, done_)) return rc_; \
+  } while (0)
 
 }  // namespace tg

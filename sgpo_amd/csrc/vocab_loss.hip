@@ -667,12 +667,6 @@ Cut cut_for(int PL, int64_t M, int64_t N, int64_t nk) {
   return best;
 }
 
-template <typename K>
-int allow_lds(K kernel, int bytes) {
-  SGPO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  return SGPO_OK;
-}
-
 // where everything lies in the workspace; the same for the size query and the run
 struct Plan {
   int PL, n_kstep, h_pad;                    // h_pad: features padded for a K step
@@ -781,11 +775,6 @@ int pack(const void* src, int64_t ld, int rows, int cols, bf16_t* dst, int64_t r
     case 1: { typedef typename Shapes<PLV>::M S; __VA_ARGS__ } break;         \
     default: { typedef typename Shapes<PLV>::S S; __VA_ARGS__ } break;        \
   }
-#define ALLOW(kernel, bytes)                                           \
-  do {                                                                 \
-    static bool done = false;                                          \
-    if (!done) { const int rc_ = allow_lds(kernel, bytes); if (rc_) return rc_; done = true; } \
-  } while (0)
 
 template <typename T, bool GRAD>
 int head(const HeadArgs& p, hipStream_t st) {
