@@ -283,7 +283,9 @@ extern "C" int sgpo_rotary(const sgpo_rotary_args* a, void* stream) {
   SGPO_REQUIRE(a->head_dim >= 1 && a->head_dim <= 4096 && a->rot >= 0 && a->rot % 2 == 0 && a->rot <= a->head_dim, "rotary: rot=%d must be even and at most head_dim=%d (1..4096)",
                a->rot, a->head_dim);
   SGPO_REQUIRE(a->dtype == SGPO_DTYPE_F32 || a->dtype == SGPO_DTYPE_BF16, "rotary: unknown dtype %d", a->dtype);
-  if ((int64_t)a->B * a->L == 0 || a->heads_q + a->heads_k == 0) return SGPO_OK;
+  const int64_t heads = (int64_t)a->heads_q + a->heads_k;
+  if ((int64_t)a->B * a->L == 0 || heads == 0) return SGPO_OK;
+  SGPO_REQUIRE(heads < 0x7fffffff, "rotary: %lld heads in one call", (long long)heads);
   SGPO_REQUIRE((int64_t)a->B * a->L < 0x7fffffff, "rotary: B * L = %lld tokens in one call", (long long)a->B * a->L);
   if (const int rc = check_memory(a)) return rc;
   SGPO_REQUIRE(a->rot == 0 || a->frequencies, "rotary: null frequencies");

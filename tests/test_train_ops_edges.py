@@ -112,3 +112,13 @@ def test_loss_gradients_that_overlap_are_refused():
                     assert 'overlaps' in call(reduction, **{out: at}), (reduction, out, other)
                 for at in (base[other] + size, base[other] - sizes[out]):
                     assert 'workspace' in call(reduction, **{out: at}), (reduction, out, other)
+
+
+def test_rotation_refuses_more_heads_than_it_can_count():
+    from sgpo_amd import _lib as L
+    lib = L.load()
+    n = 1 << 30
+    a = L.RotaryArgs(B=1, L=1, heads_q=n, heads_k=n, head_dim=1, rot=0, q=1 << 40, q_out=1 << 41, k=1 << 42, k_out=1 << 43)
+    for field in ('q', 'q_out', 'k', 'k_out'):
+        setattr(a, field + '_stride', (C.c_int64 * 3)(n, n, 1))
+    assert lib.sgpo_rotary(C.byref(a), None) < 0 and 'heads in one call' in lib.sgpo_last_error().decode()
