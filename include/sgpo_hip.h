@@ -395,7 +395,8 @@ int sgpo_rotary(const sgpo_rotary_args* args, void* stream);
  *   hidden [N][H] and weight [V][H] of `dtype`, rows ld_* elements apart; bias fp32 [V] or NULL (-inf closes a class);
  *   targets int64 [N]; a token with target ignore_index has loss and gradients 0 (its hidden row may hold anything); a
  *   target outside [0, V) gives NaN.
- * forward: nll [N], lse [N] fp32; loss [1] and inv_count [1] unless reduction is NONE (the mean over no token is 0).
+ * forward: nll [N], lse [N] fp32; loss [1] and inv_count [1] unless reduction is NONE (the mean over no token is 0).  inv_count: what
+ *   the backward pass multiplies grad_out by, 0 if no token has a loss.
  * backward: grad_out is [1] ([N] for NONE); lse and inv_count are the forward's; dhidden [N][H], dweight [V][H] of `dtype` and dbias fp32
  *   [V], contiguous, overlapping neither the inputs nor one another; any of them may be NULL.
  * The workspace is scratch: forward and backward each ask for their own. */

@@ -201,7 +201,8 @@ __global__ __launch_bounds__(256) void finish_kernel(const float2* part, int n_r
   }
 }
 
-// loss[0] = sum of nll (reduction 2) or its mean over the tokens with a loss (1; 0 if there are none); inv[0] = the factor on every token's gradient.
+// loss[0] = sum of nll (reduction 2) or its mean over the tokens with a loss (1; 0 if there are none); inv[0] = the factor on every token's gradient,
+// 0 if none has one.
 // Over TOTAL_ROWS tokens a workgroup to as many writes its part and one more adds the parts up (65536 tokens: 8.3 us; by one workgroup 20.6).
 constexpr int TOTAL_ROWS = 8192;
 struct Part { double sum; int64_t count; };
@@ -229,7 +230,7 @@ __device__ __forceinline__ Part rows_total(const float* nll, const int64_t* targ
 __device__ __forceinline__ void store_total(const Part& p, int mean, float* loss, float* inv) {
   const double n = mean ? (double)(p.count > 0 ? p.count : 1) : 1.0;
   loss[0] = (float)(p.sum / n);
-  inv[0] = (float)(1.0 / n);
+  inv[0] = p.count > 0 ? (float)(1.0 / n) : 0.f;
 }
 __global__ __launch_bounds__(1024) void total_kernel(const float* nll, const int64_t* targets, int64_t ignore, int N, int mean, float* loss, float* inv) {
   const Part p = rows_total(nll, targets, ignore, 0, N);
@@ -249,10 +250,10 @@ __global__ __launch_bounds__(1024) void join_total_kernel(const Part* parts, int
 }
 
 // ----------------------------------------------------------------------------------------------------------- backward
-// The factor common to all tokens' gradients; 1 where each has its own.
+// The factor common to all tokens' gradients; 1 where each has its own.  No token with a loss: 0, whatever the upstream gradient is.
 struct Factor {
   const float *g, *inv;   // null: 1
-  __device__ __forceinline__ float get() const { return g ? g[0] * (inv ? inv[0] : 1.f) : 1.f; }
+  __device__ __forceinline__ float get() const { return !g ? 1.f : inv[0] == 0.f ? 0.f : g[0] * inv[0]; }
 };
 
 // d (without the common factor) of a piece of the vocabulary into d [rows_pad][cols_pad] planes (zero beyond the tokens and classes); column sums per row tile
@@ -522,6 +523,8 @@ struct MmArgs {
   void* out;
   int64_t ldo, slab;
   Factor factor;            // on the sums
+  const int64_t* targets;   // or null: rows whose target is ignore get the factor 0 (an infinite one would make their zeros NaN)
+  int64_t ignore;
   int out_bf16, add;
 };
 
@@ -542,11 +545,12 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void mm_kernel(MmArgs p, int tm, 
   for (int x = 0; x < S::MT; ++x) {
     const int m = m0 + (wm * S::MT + x) * 16 + l16;
     if (m >= p.M) continue;
+    const float f = p.targets && p.targets[m] == p.ignore ? 0.f : factor;
 #pragma unroll
     for (int y = 0; y < S::NT; ++y) {
       if (!S::owns(x, y)) continue;
       const int n = n0 + (wn * S::NT + y) * 16 + 4 * l4;
-      f32x4 v = acc[x][y] * factor;
+      f32x4 v = acc[x][y] * f;
       // four at a time, whatever the row's alignment (dhidden of 56377 x 1143 bf16, 31 classes: 109 us element by element, 49 so)
       if (p.out_bf16) {
         bf16_t* o = reinterpret_cast<bf16_t*>(p.out) + m * p.ldo + n;
@@ -937,7 +941,7 @@ int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, cons
     if (dh) {
       // the first piece decides how many slabs there are; later ones add to them
       MmArgs m{{d, (int64_t)nc_pad * PL, a->N, 0}, {w.p + v0 * w.ld, w.ld, nc, q.h_pad * PL}, a->N, a->H, nc_pad / kstep, 0,
-               via ? (void*)acc : dh, via ? ldf : a->H, via ? (int64_t)a->N * ldf : 0, factor, !via && bf, v0 > 0};
+               via ? (void*)acc : dh, via ? ldf : a->H, via ? (int64_t)a->N * ldf : 0, factor, a->targets, a->ignore_index, !via && bf, v0 > 0};
       const int used = product<PL, tg::KC, tg::KM>(m, q.h_cut.shape, v0 == 0 ? q.h_cut.splits : h_used, st);
       if (used < 0) return used;
       if (v0 == 0) h_used = used;
@@ -947,7 +951,7 @@ int backward(const sgpo_linear_ce_args* a, const Plan& q, const float* lse, cons
       const bool slabs = q.w_cut.splits > 1;
       void* out = (char*)dw + v0 * a->H * esz;
       MmArgs m{{d, (int64_t)nc_pad * PL, (int)q.rows_pad, nc_pad * PL}, {hp, (int64_t)q.h_pad * PL, (int)q.rows_pad, q.h_pad * PL}, nc, a->H, (int)(q.rows_pad / kstep), 0,
-               slabs ? (void*)wacc : out, slabs ? ldf : a->H, slabs ? (int64_t)nc * ldf : 0, factor, !slabs && bf, 0};
+               slabs ? (void*)wacc : out, slabs ? ldf : a->H, slabs ? (int64_t)nc * ldf : 0, factor, nullptr, 0, !slabs && bf, 0};
       if (q.turned) m.b = tg::Operand{ht, q.rows_pad, q.h_pad, 0};
       const int used = q.turned ? product<PL, tg::KM, tg::KC>(m, q.w_cut.shape, q.w_cut.splits, st) : product<PL, tg::KM, tg::KM>(m, q.w_cut.shape, q.w_cut.splits, st);
       if (used < 0) return used;

@@ -1,5 +1,6 @@
 """GPU: the training operators at the edges of their arguments: workspaces of exactly the size asked for, tensors that are more than plain memory."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -164,3 +165,24 @@ def test_lazily_negated_views():
         loss = T.linear_cross_entropy(*leaves[:2], t, leaves[2], reduction=red)
         got, want = (torch.autograd.grad(loss, leaves, x, retain_graph=True) for x in (neg(up), -up))
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF])
+@pytest.mark.parametrize('N,H,V', [(100, 64, 31), (9000, 40, 31), (130, 72, 257), (1000, 96, 3000)])
+def test_an_infinite_upstream_gradient_does_not_reach_ignored_tokens(N, H, V, dtype):
+    """As a loss scale that overflowed hands over: an ignored token's gradient is 0 all the same, and every gradient is if no token has a loss."""
+    from sgpo_amd import train_ops as T
+    g = _gen(5)
+    h, w = torch.randn(N, H, generator=g, device='cuda').to(dtype).requires_grad_(), torch.randn(V, H, generator=g, device='cuda').to(dtype).requires_grad_()
+    b = torch.zeros(V, device='cuda', requires_grad=True)
+    t = torch.randint(0, V, (N,), generator=g, device='cuda')
+    drop = torch.rand(N, generator=g, device='cuda') < 0.3
+    t[drop] = -100
+    for up in (math.inf, math.nan):
+        for red in ('mean', 'sum', 'none'):
+            out = T.linear_cross_entropy(h, w, t, b, reduction=red)
+            dh, dw, db = torch.autograd.grad(out, (h, w, b), torch.full_like(out, up))
+            assert bool((dh[drop] == 0).all()), (up, red)
+            assert not bool(dh[~drop].isfinite().any()) and not bool(dw.isfinite().any()) and not bool(db.isfinite().any()), (up, red)
+            out = T.linear_cross_entropy(h, w, torch.full_like(t, -100), b, reduction=red)
+            assert all(bool((x == 0).all()) for x in torch.autograd.grad(out, (h, w, b), torch.full_like(out, up))), (up, red)
