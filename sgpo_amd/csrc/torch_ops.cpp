@@ -320,13 +320,14 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
   REQUIRE(hidden.dim() >= 1 && weight.dim() == 2 && hidden.size(-1) == weight.size(1) && weight.numel() > 0, "hidden ", hidden.sizes(), " does not match weight ", weight.sizes());
   REQUIRE(weight.scalar_type() == hidden.scalar_type(), "hidden is ", hidden.dtype(), " and weight ", weight.dtype());
   REQUIRE(targets.scalar_type() == at::kLong && targets.sizes() == hidden.sizes().slice(0, hidden.dim() - 1), "targets ", targets.sizes(), " ", targets.dtype(), " for hidden ", hidden.sizes());
-  REQUIRE(!opt(bias) || (bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == weight.size(0)), "bias must be float32 with one value per class");
+  REQUIRE(!opt(bias) || ((bias->scalar_type() == at::kFloat || bias->scalar_type() == weight.scalar_type()) && bias->dim() == 1 && bias->size(0) == weight.size(0)),
+          "bias must be float32 or of weight's type, with one value per class");
   const int64_t red = reduction == "none" ? SGPO_REDUCE_NONE : reduction == "mean" ? SGPO_REDUCE_MEAN : reduction == "sum" ? SGPO_REDUCE_SUM : -1;
   REQUIRE(red >= 0, "unknown reduction '", reduction, "'");
   REQUIRE(targets.numel() <= (1 << 30) && weight.size(0) <= (1 << 30) && weight.size(1) <= (1 << 20), "hidden ", hidden.sizes(), " and weight ", weight.sizes(), " over the supported range");
   const Tensor h = rows(hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)})), w = rows(weight);
   const Tensor t = targets.dim() == 1 && targets.is_contiguous() ? targets : targets.reshape({-1}).contiguous();
-  const OptTensor b = opt(bias) ? OptTensor(bias->contiguous()) : std::nullopt;
+  const OptTensor b = opt(bias) ? OptTensor(bias->to(at::kFloat).contiguous()) : std::nullopt;   // bf16: its gradient is rounded by the same step on the tape
   Tensor out = records({&hidden, &weight, opt(bias)}) ? LinearCrossEntropy::apply(h, w, t, b, ignore, red) : ce_forward(h, w, t, b.value_or(Tensor()), ignore, red).first;
   return red == SGPO_REDUCE_NONE && targets.dim() != 1 ? out.view(targets.sizes()) : out;
 }

@@ -96,8 +96,8 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
     """Cross entropy of softmax(hidden weight^T + bias) at targets without storing the logits; differentiable in hidden, weight
     and bias (once).
 
-    hidden (..., H) and weight (V, H), both fp32 or both bf16; targets int64 of hidden's leading shape; bias fp32 (V,) or None, where -inf
-    closes a class (the mask class of an absorbing-state model, mdlm_diffusion.py:325-341).  reduction 'none' gives fp32 losses of
+    hidden (..., H) and weight (V, H), both fp32 or both bf16; targets int64 of hidden's leading shape; bias (V,), fp32 or of weight's type, or None,
+    where -inf closes a class (the mask class of an absorbing-state model, mdlm_diffusion.py:325-341).  reduction 'none' gives fp32 losses of
     targets' shape; 'sum' and 'mean' (over the targets that are not ignore_index; 0 if there are none) give a scalar.  An ignored token has loss
     and gradients 0 whatever its features hold; a target outside [0, V) gives NaN, as no check on the host waits for the GPU."""
     return (_ops or _load()).linear_cross_entropy(hidden, weight, targets, bias, ignore_index, reduction)

@@ -186,3 +186,24 @@ def test_an_infinite_upstream_gradient_does_not_reach_ignored_tokens(N, H, V, dt
             assert not bool(dh[~drop].isfinite().any()) and not bool(dw.isfinite().any()) and not bool(db.isfinite().any()), (up, red)
             out = T.linear_cross_entropy(h, w, torch.full_like(t, -100), b, reduction=red)
             assert all(bool((x == 0).all()) for x in torch.autograd.grad(out, (h, w, b), torch.full_like(out, up))), (up, red)
+
+
+@pytest.mark.parametrize('V', [31, 300])
+def test_head_whose_bias_has_the_weights_type(V):
+    """A linear layer in bf16 as it is: the bias is read as it stands (bf16 values are fp32 values), and its gradient rounded once."""
+    from sgpo_amd import _lib as L
+    from sgpo_amd import train_ops as T
+    g = _gen(6)
+    head = torch.nn.Linear(64, V, dtype=BF, device='cuda')
+    h, t = torch.randn(50, 64, generator=g, device='cuda').to(BF), torch.randint(0, V - 1, (50,), generator=g, device='cuda')
+    with torch.no_grad():
+        head.bias[V - 1] = -math.inf
+    T.linear_cross_entropy(h, head.weight, t, head.bias).backward()
+    w, b = head.weight.detach().requires_grad_(), head.bias.detach().float().requires_grad_()
+    want = torch.autograd.grad(T.linear_cross_entropy(h, w, t, b), (w, b))
+    assert torch.equal(head.weight.grad, want[0]) and head.bias.grad.dtype == BF and torch.equal(head.bias.grad, want[1].to(BF))
+    for bad in (head.bias.detach().half(), head.bias.detach().double()):
+        with pytest.raises(L.SgpoError, match='bias'):
+            T.linear_cross_entropy(h, head.weight, t, bad)
+    with pytest.raises(L.SgpoError, match='bias'):
+        T.linear_cross_entropy(h.float(), head.weight.float(), t, head.bias)
