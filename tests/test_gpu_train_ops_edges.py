@@ -207,3 +207,26 @@ def test_head_whose_bias_has_the_weights_type(V):
             T.linear_cross_entropy(h, head.weight, t, bad)
     with pytest.raises(L.SgpoError, match='bias'):
         T.linear_cross_entropy(h.float(), head.weight.float(), t, head.bias)
+
+
+@pytest.mark.parametrize('shape', [(31, 128), (64, 300), (20, 90), (500, 48)])
+def test_low_rank_updates_of_few_rows_or_columns_stay_in_32_bits(shape):
+    """Updates of five directions whose iteration runs on d x d matrices, seen through an fp32 weight that takes them unrounded.  X_0 has norm 1 and is rounded by
+    2^-24; a product adds d terms, each sum rounded by 2^-24 / sqrt(3) with a random sign; what the five triples leave outside of the five directions
+    grows by 3.4445^5 = 485 at most: 5 x 485 x 2^-24 sqrt(d / 3), 3.7e-4 to 6.7e-4 of a result of norm 2.  (With Q mirrored from one triangle, instead of
+    multiplied whole, the same arithmetic on the CPU is off by 6e-4 to 3e-3; whole, by 2e-5 to 9e-5.)"""
+    from sgpo_amd import train_ops as T
+    g = _gen(7)
+    m, n = shape
+    u = torch.randn(m, 5, generator=g, device='cuda') @ torch.randn(5, n, generator=g, device='cuda')
+    u[::7] = 0
+    for x in (u, u * torch.logspace(0, -3, m, device='cuda')[:, None], u.to(BF)):
+        want = x.double() / (x.double().norm() + 1e-7)
+        for _ in range(5):
+            a, b, c = T.NS_COEFFICIENTS
+            gram = want @ want.T if m < n else want.T @ want
+            p = b * gram + c * gram @ gram
+            want = a * want + (p @ want if m < n else want @ p)
+        w = torch.zeros(shape, device='cuda')
+        T.muon_step(w, x, torch.zeros(shape, device='cuda'), lr=1 / math.sqrt(max(1, m / n)), momentum=0.0, nesterov=False)
+        assert float((w.double() + want).norm()) <= 5 * 485 * 2.0 ** -24 * math.sqrt(min(m, n) / 3) + 4 * 2.0 ** -24 * float(want.norm())
