@@ -374,7 +374,7 @@ int sgpo_daps_mh(sgpo_mlp* m, const int64_t* x0hat, int N, int L, int S, const i
 #define SGPO_DTYPE_BF16 1
 
 /* Rotation of query and key heads by their positions.  Pair j < rot / 2 of a head -- elements (j, j + rot / 2), or (2j, 2j + 1)
- * if interleaved -- turns by position * frequencies[j] (formed in 64 bits) and is multiplied by scale; elements from rot on are
+ * if interleaved -- turns by position * frequencies[j] (rounded to 64 bits; |position| up to 2^50) and is multiplied by scale; elements from rot on are
  * copied.  inverse: the transposed rotation, i.e. the gradient.  Strides in elements: batch, token, head; a head's elements
  * are contiguous.  q_out may be q and k_out may be k (in place); any other overlap of an output with itself, the other one or an input is
  * refused (views of different strides count as overlapping where their address ranges meet).  heads_k 0: no keys.

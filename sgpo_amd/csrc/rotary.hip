@@ -6,7 +6,8 @@
 //
 // Bound by memory: every element is read and written once (q and k in one launch).  The angles of a token are formed once for
 // all of its heads, in 64 bits -- at position 2^22 an fp32 product is off by a quarter radian -- reduced to one turn in 64 bits and only then
-// rounded to fp32 for sin / cos.
+// rounded to fp32 for sin / cos.  The angle meant is the product position * frequency as 64 bits hold it, as in any 64-bit formula of the rotation: it
+// is off by up to 2^-53 of itself, i.e. 2^-24 of a radian (as much as fp32's rounding of the reduced angle) at 2^29 radians and 2^-4 at 2^49.
 #include <algorithm>
 
 #include "../../include/sgpo_hip.h"
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(Args p) {
     const int64_t b = div_by(p.by_len, (uint32_t)t0 + tok, l);
     const int64_t at = p.pos ? p.pos[b * p.pos_sb + l * p.pos_sl] : l;
     const double a = (double)at * p.freq[j];
-    // one turn taken off in two pieces of 2 pi: exact to 2^-50 of a radian for any position below 2^50
+    // one turn taken off in two pieces of 2 pi: the rest of the rounded product is exact to 2^-50 of a radian for any angle below 2^50
     const double n = rint(a * 0.15915494309189535);
     const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, a));
     float s, c;

@@ -230,3 +230,38 @@ def test_low_rank_updates_of_few_rows_or_columns_stay_in_32_bits(shape):
         w = torch.zeros(shape, device='cuda')
         T.muon_step(w, x, torch.zeros(shape, device='cuda'), lr=1 / math.sqrt(max(1, m / n)), momentum=0.0, nesterov=False)
         assert float((w.double() + want).norm()) <= 5 * 485 * 2.0 ** -24 * math.sqrt(min(m, n) / 3) + 4 * 2.0 ** -24 * float(want.norm())
+
+
+def _pi(bits):
+    """pi 2^bits as a whole number, by Machin's formula."""
+    def inverse_arctan(n):
+        total, term, k = 0, (1 << bits + 32) // n, 0
+        while term:
+            total += -(term // (2 * k + 1)) if k & 1 else term // (2 * k + 1)
+            term //= n * n
+            k += 1
+        return total
+    return 4 * (4 * inverse_arctan(5) - inverse_arctan(239)) >> 32
+
+
+def test_rotation_angles_against_whole_number_arithmetic():
+    """Angles whose product is not rounded: a frequency is a whole number of 2^-e, the angle's rest after whole turns is formed in whole numbers.  The kernel's
+    is off by the product's rounding, 2^-53 of the angle, besides 10 units of fp32 (angle rounded within half a turn, sin, cos, products and sum)."""
+    from fractions import Fraction
+    from sgpo_amd import train_ops as T
+    g = _gen(8)
+    rot, places = 16, 1 << 160
+    freq, _ = T.rotary_frequencies(rot)
+    pos = [0, 1, 4095, (1 << 22) + 1, (1 << 29) - 1, (1 << 31) + 7, 123456789012, (1 << 40) - 3, (1 << 50) - 1, -(1 << 30) - 1]
+    q = torch.randn(1, len(pos), 2, rot, generator=g, device='cuda')
+    got = T.rotary_positions(q, None, freq, torch.tensor(pos, device='cuda'))[0].double().cpu()
+    q = q.double().cpu()
+    turn = Fraction(2 * _pi(160), places)
+    for i, p in enumerate(pos):
+        for j, f in enumerate(freq.tolist()):
+            angle = p * Fraction(f)
+            rest = angle - round(angle / turn) * turn
+            c, s = math.cos(rest), math.sin(rest)
+            a, b = q[0, i, :, j], q[0, i, :, j + rot // 2]
+            tol = (10 * 2.0 ** -24 + abs(float(angle)) * 2.0 ** -53) * (a.abs() + b.abs())
+            assert bool(((got[0, i, :, j] - (a * c - b * s)).abs() <= tol).all()) and bool(((got[0, i, :, j + rot // 2] - (a * s + b * c)).abs() <= tol).all()), (p, j)
