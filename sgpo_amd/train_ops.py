@@ -49,7 +49,9 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
 
     scaling None; 'linear': every angle / factor; 'ntk': base * factor ** (rotary_dim / (rotary_dim - 2)), which keeps the fastest pair
     and divides the slowest by factor; 'yarn': pairs that turn more than beta_fast times within original_length positions stay, those
-    below beta_slow turns are divided by factor, linearly in between, and rotated elements are scaled by 0.1 ln(factor) + 1."""
+    below beta_slow turns are divided by factor, in between linearly in the number of turns, and rotated elements are scaled by 0.1 ln(factor) + 1.
+    That is the published formula.  Programs that ramp linearly in the pair's index, between the rounded indices of the two bounds, give the pairs
+    in between other frequencies: for a model trained so, pass its own float64 tensor to rotary_positions."""
     if rotary_dim < 0 or rotary_dim % 2:
         _refuse(f'rotary_dim must be even, got {rotary_dim}')
     if not (base > 0 and factor >= 1):

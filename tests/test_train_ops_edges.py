@@ -122,3 +122,16 @@ def test_rotation_refuses_more_heads_than_it_can_count():
     for field in ('q', 'q_out', 'k', 'k_out'):
         setattr(a, field + '_stride', (C.c_int64 * 3)(n, n, 1))
     assert lib.sgpo_rotary(C.byref(a), None) < 0 and 'heads in one call' in lib.sgpo_last_error().decode()
+
+
+def test_stretched_frequencies_ramp_in_turns():
+    """The pairs between beta_slow and beta_fast turns: the share that is kept is linear in the turns, not in the pair's index."""
+    from sgpo_amd import train_ops as T
+    rot, factor, length = 64, 8.0, 4096
+    f, _ = T.rotary_frequencies(rot, device='cpu')
+    got, _ = T.rotary_frequencies(rot, scaling='yarn', factor=factor, original_length=length, device='cpu')
+    turns = length * f / (2 * torch.pi)
+    keep = (got / f - 1 / factor) / (1 - 1 / factor)
+    between = (turns > 1) & (turns < 32)
+    assert int(between.sum()) >= 10 and bool((keep[turns >= 32] > 1 - 1e-12).all()) and bool((keep[turns <= 1].abs() < 1e-12).all())
+    torch.testing.assert_close(keep[between], (turns[between] - 1) / 31, rtol=1e-12, atol=1e-12)
