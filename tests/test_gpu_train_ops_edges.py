@@ -265,3 +265,39 @@ def test_rotation_angles_against_whole_number_arithmetic():
             a, b = q[0, i, :, j], q[0, i, :, j + rot // 2]
             tol = (10 * 2.0 ** -24 + abs(float(angle)) * 2.0 ** -53) * (a.abs() + b.abs())
             assert bool(((got[0, i, :, j] - (a * c - b * s)).abs() <= tol).all()) and bool(((got[0, i, :, j + rot // 2] - (a * s + b * c)).abs() <= tol).all()), (p, j)
+
+
+def test_hooks_and_checkpoints():
+    """What autograd lets a program do around a call: tensors saved on the host between the passes (where they lose their strides), gradients changed by hooks,
+    the forward pass run again in the backward pass."""
+    from torch.utils.checkpoint import checkpoint
+    from sgpo_amd import train_ops as T
+    g = _gen(9)
+    wide = torch.randn(300, 72, generator=g, device='cuda').to(BF)
+    h, w = wide[:200, :64], wide[200:, 8:]
+    b, t = torch.randn(100, generator=g, device='cuda'), torch.randint(0, 100, (200,), generator=g, device='cuda')
+    qkv = torch.randn(2, 9, 3, 4, 16, generator=g, device='cuda')
+    freq, _ = T.rotary_frequencies(16)
+
+    def loss(hh, ww, bb):
+        return T.linear_cross_entropy(hh, ww, t, bb)
+
+    def turned(x):
+        q, k = T.rotary_positions(x[:, :, 0], x[:, :, 1], freq)
+        return (q * k).sum()
+
+    for call, args in ((loss, (h, w, b)), (turned, (qkv,))):
+        leaves = [x.detach().requires_grad_() for x in args]
+        want = torch.autograd.grad(call(*leaves), leaves)
+        with torch.autograd.graph.save_on_cpu():
+            out = call(*leaves)
+        assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(out, leaves), want))
+        assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(checkpoint(call, *leaves, use_reentrant=False), leaves), want))
+        out = call(*leaves)
+        seen = []
+        leaves[0].register_hook(lambda x: seen.append(x) or -x)
+        out.register_hook(lambda x: x * 2)
+        got = torch.autograd.grad(out, leaves)
+        assert len(seen) == 1 and bool((got[0] == -seen[0]).all())
+        for x, y in zip(got, want):             # twice the gradient, exactly: a factor of 2 rounds nothing
+            assert torch.equal(x.abs(), (2 * y).abs())
