@@ -253,7 +253,11 @@ __global__ __launch_bounds__(1024) void join_total_kernel(const Part* parts, int
 // The factor common to all tokens' gradients; 1 where each has its own.  No token with a loss: 0, whatever the upstream gradient is.
 struct Factor {
   const float *g, *inv;   // null: 1
-  __device__ __forceinline__ float get() const { return !g ? 1.f : inv[0] == 0.f ? 0.f : g[0] * inv[0]; }
+  __device__ __forceinline__ float get() const {
+    if (!g) return 1.f;
+    const float up = g[0], i = inv[0];   // both on their way at once
+    return i == 0.f ? 0.f : up * i;
+  }
 };
 
 // d (without the common factor) of a piece of the vocabulary into d [rows_pad][cols_pad] planes (zero beyond the tokens and classes); column sums per row tile
@@ -535,17 +539,20 @@ __global__ __launch_bounds__(S::WG_THREADS, 2) void mm_kernel(MmArgs p, int tm, 
   tg::tile_of(blockIdx.x, tm, tn, im, in);
   const int m0 = im * S::BM, n0 = in * S::BN;
   const int k0 = blockIdx.y * p.nk_split, nk = min(p.nk_split, p.nk - k0);
+  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
+  const int wm = S::wave() / S::WN, wn = S::wave() % S::WN;
+  int64_t target[S::MT];   // of all rows, on their way during the products
+#pragma unroll
+  for (int x = 0; x < S::MT; ++x) target[x] = p.targets ? p.targets[min(m0 + (wm * S::MT + x) * 16 + l16, p.M - 1)] : 0;
   f32x4 acc[S::MT][S::NT];
   tg::clear<S>(acc);
   tg::run<S, KA, KB>(p.a, p.b, m0, n0, k0, nk, smem, acc);
-  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
-  const int wm = S::wave() / S::WN, wn = S::wave() % S::WN;
   const float factor = p.factor.get();
 #pragma unroll
   for (int x = 0; x < S::MT; ++x) {
     const int m = m0 + (wm * S::MT + x) * 16 + l16;
     if (m >= p.M) continue;
-    const float f = p.targets && p.targets[m] == p.ignore ? 0.f : factor;
+    const float f = p.targets && target[x] == p.ignore ? 0.f : factor;
 #pragma unroll
     for (int y = 0; y < S::NT; ++y) {
       if (!S::owns(x, y)) continue;
