@@ -7,7 +7,7 @@
 //   step:  buf <- mu buf + grad,  U = grad + mu buf (or buf),  W <- (1 - lr wd) W - lr sqrt(max(1, rows / cols)) X
 //
 // Bound by the matrix cores: per triple m^2 n + m^3 + 2 m^2 n operations, the two symmetric products at half (one triangle of tiles,
-// each written twice).  X, G and P are held as two bf16 planes, about 17 bits (tile_gemm.h): in one plane the rounding of X
+// each written twice).  X, G and P are held as two bf16 planes, about 17 bits (tile_gemm.h; fp32 on the second way below): in one plane the rounding of X
 // pollutes the directions of small singular values, which the polynomial then multiplies by up to a^5 = 485 (relative error of
 // the result 2e-2 on Gaussian updates, against 3e-5 with two planes; the result is rounded to bf16, 2e-3).
 // The squared norm is summed in 64 bits: it neither overflows nor depends on how the update is cut.  An infinity or NaN in an update

@@ -12,7 +12,8 @@
 // or three), and one plane is the ordinary row-major layout.  An operand is read either way round:
 //   KC  rows are m (or n), k contiguous: fragments by ds_read_b128, 8 consecutive k of a row per lane;
 //   KM  rows are k, m (or n) contiguous: fragments by ds_read_b64_tr_b16 (the LDS transposes 4 x 16 blocks on the way to the
-//       registers), so that no transposed copy of any operand ever exists in memory.
+//       registers), so that no operand needs a transposed copy in memory (two KM operands are slower than one, though: the loss makes
+//       a transposed copy of its features where a product would have two).
 // LDS images are filled by LDS-DMA, 16 B per lane, lane-linear; bank conflicts are avoided by permuting the 16-B chunks of a
 // row on the source address and again on the read.
 #pragma once

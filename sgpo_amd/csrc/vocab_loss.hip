@@ -8,7 +8,8 @@
 // (maximum, sum of exponentials) pair per token; a second kernel joins a token's pairs.  Backward: the vocabulary in pieces;
 // for each piece the logits again, d (rounded to the operands' precision) into a buffer that every piece reuses, then the two products
 // that read it -- d as rows (dhidden) and d as columns (dweight) come from the same buffer (tile_gemm.h, KC and KM).
-// 2 N V H operations forward and 6 backward; everything but the operands and gradients stays in caches or registers.
+// 2 N V H operations forward and 6 backward.  Logits stay in registers; a piece of d goes through memory: 8192 tokens by 16384 classes of bf16 are 256 MB
+// written, and each of the two products reads about three times that, operands included (770 and 830 MB in 0.41 ms, 2.1 TB/s).
 //
 // bf16 operands: one plane; d is rounded to bf16 once (2^-8 of a term at most, of the size of the outputs' own rounding), sums in
 // fp32.  A factor common to all tokens (mean, sum) is left out of d and applied to the products' sums: rounded into d it would be off

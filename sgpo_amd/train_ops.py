@@ -130,7 +130,7 @@ def _coefficients(coefficients, steps):
 def newton_schulz(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
     """The update (..., m, n) with every singular value moved towards 1 and its singular vectors kept: X = U / (|U|_F + eps), then
     X <- a X + (b X X^T + c (X X^T)^2) X per coefficient triple (one triple for all steps, or one each).  Leading dimensions are independent matrices.
-    update fp32 or bf16; returns bf16, contiguous.  Iterates carry 17 bits, sums 32, the norm 64.  Not differentiable."""
+    update fp32 or bf16; returns bf16, contiguous.  Iterates carry at least 17 bits, sums 32, the norm 64.  Not differentiable."""
     return (_ops or _load()).newton_schulz(update, steps, _coefficients(coefficients, steps), eps)
 
 
